@@ -654,6 +654,106 @@ int afiv_ensemble_stats_groups(const double *iv, const uint8_t *select, int64_t 
     return afiv_launch_ensemble(iv, select, N, (int)points, groups, stats_out, as_stream(stream));
 }
 
+// ---- layer operators: sizes and enums are checked before any device call ------------------------
+static bool bad_layer(int dtype, int act)
+{
+    return dtype < AFIV_F32 || dtype > AFIV_F16 || act < AFIV_ACT_NONE || act > AFIV_ACT_SILU;
+}
+static const int64_t MAX_WIDTH = (int64_t)1 << 24, MAX_ROWS = (int64_t)1 << 36;
+
+// rows and columns whose element offsets stay in range; a launch has fewer than 2^32 work items, so the
+// 128 x 128 tiles of 256 threads number less than 2^24
+static bool bad_sizes(int64_t rows, int64_t cols)
+{
+    return rows < 0 || rows > MAX_ROWS || cols < 1 || cols > MAX_WIDTH || (rows + 127) / 128 * ((cols + 127) / 128) >= (1 << 24);
+}
+
+int afiv_checkpoint8_pack(const void *x, int dtype, int64_t rows, int64_t cols, int8_t *codes, uint8_t *scales, void *stream)
+{
+    if (bad_layer(dtype, 0)) return AFIV_E_ARG;
+    if (bad_sizes(rows, cols)) return AFIV_E_SHAPE;
+    if (rows == 0) return AFIV_OK;
+    if (!x || !codes || !scales) return AFIV_E_NULL;
+    return afiv_launch_checkpoint8_pack(x, dtype, rows, cols, codes, scales, as_stream(stream));
+}
+
+int afiv_checkpoint8_restore(const int8_t *codes, const uint8_t *scales, int dtype, int64_t rows, int64_t cols, void *x_out, void *stream)
+{
+    if (bad_layer(dtype, 0)) return AFIV_E_ARG;
+    if (bad_sizes(rows, cols)) return AFIV_E_SHAPE;
+    if (rows == 0) return AFIV_OK;
+    if (!x_out || !codes || !scales) return AFIV_E_NULL;
+    return afiv_launch_checkpoint8_restore(codes, scales, dtype, rows, cols, x_out, as_stream(stream));
+}
+
+static bool bad_linear(int64_t M, int64_t N, int64_t K)
+{
+    return bad_sizes(M, N) || bad_sizes(M, K) || bad_sizes(N, K);
+}
+
+int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K)
+{
+    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_forward_scratch(M, N, K);
+}
+
+int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K)
+{
+    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_backward_scratch(M, N, K);
+}
+
+int afiv_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
+                    int64_t K, void *y, void *pre_out, uint8_t *dcodes_out, void *scratch, int64_t scratch_bytes, void *stream)
+{
+    if (bad_layer(dtype, act)) return AFIV_E_ARG;
+    if (bad_linear(M, N, K)) return AFIV_E_SHAPE;
+    if (M == 0) return AFIV_OK;
+    if (!x || !w || !y) return AFIV_E_NULL;
+    const int64_t need = afiv_linear_forward_scratch(M, N, K);
+    if (need > 0 && (!scratch || scratch_bytes < need)) return AFIV_E_WORKSPACE;
+    return afiv_launch_linear_act(x, w, bias, residual, dtype, act, M, N, K, y, pre_out, dcodes_out, (float *)scratch, as_stream(stream));
+}
+
+int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w, const void *pre,
+                             const uint8_t *dcodes, int dtype, int act, int64_t M, int64_t N, int64_t K, void *dx, void *dw, void *db,
+                             void *scratch, int64_t scratch_bytes, void *stream)
+{
+    if (bad_layer(dtype, act)) return AFIV_E_ARG;
+    if (bad_linear(M, N, K)) return AFIV_E_SHAPE;
+    if (M > 0) {                                       // no rows: dw and db are zeros
+        if (!dy || (dx && !w) || (dw && !x && (!codes || !scales))) return AFIV_E_NULL;
+        if (act != AFIV_ACT_NONE && !pre && !dcodes) return AFIV_E_NULL;
+    }
+    const int64_t need = afiv_linear_backward_scratch(M, N, K);
+    if (need > 0 && (!scratch || scratch_bytes < need)) return AFIV_E_WORKSPACE;
+    return afiv_launch_linear_act_backward(dy, x, x ? nullptr : codes, x ? nullptr : scales, w, pre, pre ? nullptr : dcodes, dtype, act, M,
+                                           N, K, dx, dw, db, (float *)scratch, as_stream(stream));
+}
+
+int afiv_norm_act(const void *x, const float *gamma, const float *beta, const uint8_t *keep, int dtype, int act, int64_t M, int64_t N,
+                  double eps, double momentum, double drop_p, float *running_mean, float *running_var, void *y, double *stats_out,
+                  int8_t *codes_out, uint8_t *scales_out, double *scratch, void *stream)
+{
+    if (bad_layer(dtype, act)) return AFIV_E_ARG;
+    if (!(drop_p >= 0.0 && drop_p < 1.0) || (!keep && drop_p != 0.0) || !(eps >= 0.0) || !std::isfinite(momentum)) return AFIV_E_ARG;
+    if (M < 2 || bad_sizes(M, N)) return AFIV_E_SHAPE;
+    if (!x || !gamma || !beta || !y || !stats_out || !scratch || !running_mean != !running_var || !codes_out != !scales_out)
+        return AFIV_E_NULL;
+    return afiv_launch_norm_act(x, gamma, beta, keep, dtype, act, M, N, eps, momentum, drop_p, running_mean, running_var, y, stats_out,
+                                codes_out, scales_out, scratch, as_stream(stream));
+}
+
+int afiv_norm_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const float *gamma,
+                           const float *beta, const uint8_t *keep, const double *stats, int dtype, int act, int64_t M, int64_t N,
+                           double drop_p, void *dx, float *dgamma, float *dbeta, double *scratch, void *stream)
+{
+    if (bad_layer(dtype, act)) return AFIV_E_ARG;
+    if (!(drop_p >= 0.0 && drop_p < 1.0) || (!keep && drop_p != 0.0)) return AFIV_E_ARG;
+    if (M < 2 || bad_sizes(M, N)) return AFIV_E_SHAPE;
+    if (!dy || (!x && (!codes || !scales)) || !gamma || !beta || !stats || !dgamma || !dbeta || !scratch) return AFIV_E_NULL;
+    return afiv_launch_norm_act_backward(dy, x, x ? nullptr : codes, x ? nullptr : scales, gamma, beta, keep, stats, dtype, act, M, N,
+                                         drop_p, dx, dgamma, dbeta, scratch, as_stream(stream));
+}
+
 int afiv_debug_math(int op, const double *x, const double *y, int64_t n, double *out0, double *out1,
                     void *stream)
 {

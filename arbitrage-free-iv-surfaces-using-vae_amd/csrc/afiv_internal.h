@@ -127,3 +127,19 @@ int afiv_launch_ensemble(const double *iv, const uint8_t *select, int64_t N, int
 int afiv_launch_density_wasserstein(const GridView &g, const double *model_ratio, int64_t C,
                                     const double *market_ratio, int64_t D, double *scratch, double *dist,
                                     hipStream_t s);
+int afiv_launch_checkpoint8_pack(const void *x, int dtype, int64_t rows, int64_t cols, int8_t *codes, uint8_t *scales, hipStream_t s);
+int afiv_launch_checkpoint8_restore(const int8_t *codes, const uint8_t *scales, int dtype, int64_t rows, int64_t cols, void *x,
+                                    hipStream_t s);
+int64_t afiv_linear_forward_scratch(int64_t M, int64_t N, int64_t K);      // bytes
+int64_t afiv_linear_backward_scratch(int64_t M, int64_t N, int64_t K);
+int afiv_launch_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
+                           int64_t K, void *y, void *pre, uint8_t *dcodes, float *scratch, hipStream_t s);
+int afiv_launch_linear_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w,
+                                    const void *pre, const uint8_t *dcodes, int dtype, int act, int64_t M, int64_t N, int64_t K, void *dx,
+                                    void *dw, void *db, float *scratch, hipStream_t s);
+int afiv_launch_norm_act(const void *x, const float *gamma, const float *beta, const uint8_t *keep, int dtype, int act, int64_t M,
+                         int64_t N, double eps, double momentum, double drop_p, float *run_mean, float *run_var, void *y, double *stats,
+                         int8_t *codes, uint8_t *scales, double *scratch, hipStream_t s);
+int afiv_launch_norm_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const float *gamma,
+                                  const float *beta, const uint8_t *keep, const double *stats, int dtype, int act, int64_t M, int64_t N,
+                                  double drop_p, void *dx, float *dgamma, float *dbeta, double *scratch, hipStream_t s);

@@ -9,9 +9,11 @@ keys.  What changes is where the hot-path methods run:
 * ``compute_arbitrage_penalty`` prices its 5-strike x 2-maturity lattice with the pricing
   kernel (``afiv_arbitrage_penalty``) instead of one QuantLib call per point.
 
-Encoder, re-parameterisation, Feller penalty and the loss arithmetic are ordinary torch code
-(training is outside the accelerated path); ``decode`` also stays differentiable torch code
-whenever autograd needs a graph.
+Encoder, re-parameterisation, Feller penalty and the loss arithmetic are ordinary torch code;
+``decode`` also stays differentiable torch code whenever autograd needs a graph.  With
+``layer_kernels=True`` the encoder and the differentiable decoder run their layers on the layer
+operators instead (``afiv.linear_act``, ``afiv.batch_norm_act``), and with ``checkpoint8=True`` those
+keep their activations in 8 bits until the backward pass.
 """
 from __future__ import annotations
 
@@ -34,6 +36,7 @@ from heston_model_ql import cached_grid  # noqa: E402
 _afiv = afiv_bootstrap.load()
 
 _ACTIVATIONS = {"relu": nn.ReLU, "leaky_relu": lambda: nn.LeakyReLU(0.2), "tanh": nn.Tanh}
+_ACTIVATION_TYPES = {"relu": nn.ReLU, "leaky_relu": nn.LeakyReLU, "tanh": nn.Tanh}      # for the layer operators
 
 # lattice of the training-time penalty (cvae_model.py:245-246)
 _PENALTY_LOGM = np.array([-0.1, -0.05, 0.0, 0.05, 0.1])
@@ -53,8 +56,13 @@ def _stack(widths, act, dropout):
 class ConditionalVAE_SingleHeston(nn.Module):
     def __init__(self, param_dim=5, conditioning_dim=8, latent_dim=4, hidden_dims=[128, 64, 32],
                  encoder_activation="tanh", decoder_activation="relu", dropout=0.15,
-                 feller_penalty_weight=1.0, beta=0.1, arbitrage_penalty_weight=2.0):
+                 feller_penalty_weight=1.0, beta=0.1, arbitrage_penalty_weight=2.0,
+                 layer_kernels=False, checkpoint8=False):
         super().__init__()
+        if checkpoint8 and not layer_kernels:
+            raise ValueError("checkpoint8 needs layer_kernels=True")
+        self.layer_kernels = layer_kernels
+        self.checkpoint8 = checkpoint8
         self.param_dim = param_dim
         self.conditioning_dim = conditioning_dim
         self.latent_dim = latent_dim
@@ -84,8 +92,49 @@ class ConditionalVAE_SingleHeston(nn.Module):
         except KeyError:
             raise ValueError(f"Unknown activation: {name}")
 
-    # ---- encoder side: plain torch --------------------------------------------------------
+    # ---- stacks on the layer operators -----------------------------------------------------
+    def _linear(self, layer, h, act="none"):
+        return _afiv.linear_act(h, layer.weight, layer.bias, act=act, checkpoint8=self.checkpoint8)
+
+    def _run_stack(self, stack, h):
+        """``stack(h)`` on the layer operators.  A block is [Linear, BatchNorm1d, activation, Dropout]:
+        training takes the linear layer, then normalisation, activation and dropout in one operator; with
+        frozen statistics the normalisation is an affine map of the linear layer's output, folded into
+        its weight and bias, and the activation is that layer's epilogue."""
+        layers, i = list(stack), 0
+        while i < len(layers):
+            lin, bn = layers[i], layers[i + 1] if i + 1 < len(layers) else None
+            if not isinstance(bn, nn.BatchNorm1d):
+                h, i = self._linear(lin, h), i + 1
+                continue
+            name = next(k for k, kind in _ACTIVATION_TYPES.items() if isinstance(layers[i + 2], kind))
+            drop = layers[i + 3].p if i + 3 < len(layers) and isinstance(layers[i + 3], nn.Dropout) else None
+            if bn.training:
+                h = self._linear(lin, h)
+                keep = torch.rand(h.shape, device=h.device) >= drop if drop else None
+                bn.num_batches_tracked.add_(1)
+                h = _afiv.batch_norm_act(h, bn.weight, bn.bias, bn.running_mean, bn.running_var, act=name, keep=keep,
+                                         drop_p=drop or 0.0, momentum=bn.momentum, eps=bn.eps, checkpoint8=self.checkpoint8)
+            else:
+                a = bn.weight * torch.rsqrt(bn.running_var + bn.eps)
+                h = _afiv.linear_act(h, lin.weight * a[:, None], (lin.bias - bn.running_mean) * a + bn.bias, act=name,
+                                     checkpoint8=self.checkpoint8)
+            i += 3 if drop is None else 4
+        return h
+
+    def _stack_inputs(self, *parts):
+        """The stacks' input on the layer operators' terms: CUDA, in the weights' type."""
+        h = torch.cat(parts, dim=1)
+        if not h.is_cuda:
+            raise RuntimeError("layer_kernels=True runs the HIP layer operators and needs the model and its "
+                               "inputs on a GPU (no CPU fallback)")
+        return h
+
+    # ---- encoder side ------------------------------------------------------------------------
     def encode(self, x, c):
+        if self.layer_kernels:
+            h = self._run_stack(self.encoder, self._stack_inputs(x, c))
+            return self._linear(self.fc_mu, h), self._linear(self.fc_logvar, h)
         h = self.encoder(torch.cat([x, c], dim=1))
         return self.fc_mu(h), self.fc_logvar(h)
 
@@ -157,6 +206,8 @@ class ConditionalVAE_SingleHeston(nn.Module):
             self.training or z.requires_grad or c.requires_grad
             or any(p.requires_grad for p in self.decoder.parameters()))
         if self.training or needs_graph:
+            if self.layer_kernels:
+                return self._run_stack(self.decoder, self._stack_inputs(z, c))
             return self.decoder(torch.cat([z, c], dim=1))          # autograd / batch statistics
         where, zf, cf = self._inference_inputs(z, c)
         out = self._decoder_handle(where).decode(zf, cf, want=("normalized",))

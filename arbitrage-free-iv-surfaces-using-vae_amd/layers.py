@@ -1,0 +1,339 @@
+"""Layer operators over the C ABI: a linear layer with bias, activation and residual; training-mode
+batch normalisation with activation and dropout; 8-bit activation checkpoints.
+
+These are the pieces of the conditional VAE's [Linear, BatchNorm1d, activation, Dropout] stacks
+(cvae_model.py:64-105), forward and backward, for layers of any width.  ``linear_act`` and
+``batch_norm_act`` are differentiable; their ``_forward`` / ``_backward`` halves are for training loops
+that hold the backward pass themselves (graph capture, pipelines).  Every function takes CUDA tensors
+in float32, bfloat16 or float16, enqueues on torch's current stream of the tensors' device and does not
+synchronise.  Inputs that are not contiguous are copied first.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .api import _ptr, _stream
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "tanh": 3, "gelu": 4, "silu": 5}
+NORM_SCRATCH_DOUBLES = 2 * 256 + 2      # afiv.h: AFIV_NORM_SCRATCH_DOUBLES, per column
+
+
+def _act(name: str) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
+
+
+def _first(x, what: str) -> torch.Tensor:
+    """The operand that sets the device and the element type."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what} must be a torch.Tensor")
+    if not x.is_cuda:
+        raise ValueError(f"{what} is on {x.device}: the layer kernels need a GPU (no CPU fallback)")
+    if x.dtype not in DTYPES:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {x.dtype}")
+    return x.detach().contiguous()
+
+
+def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = False) -> torch.Tensor:
+    """Another operand: on x's device, of x's type (or one of ``dtypes``), of the given shape."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a torch.Tensor")
+    if t.device != x.device:
+        raise ValueError(f"{what} is on {t.device}, expected {x.device}")
+    if t.dtype not in (dtypes or (x.dtype,)):
+        raise TypeError(f"{what} must be {' or '.join(map(str, dtypes or (x.dtype,)))}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {list(shape)}, got {list(t.shape)}")
+    if output and not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous: the kernels write into it in place")
+    return t.detach().contiguous()
+
+
+def _rows(x: torch.Tensor, what: str) -> int:
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what} must be [..., features] with at least one feature, got {list(x.shape)}")
+    return x.numel() // x.shape[-1]
+
+
+# ---- 8-bit checkpoints -----------------------------------------------------------------------
+@dataclass(frozen=True)
+class Checkpoint8:
+    """A tensor in 8 bits (see afiv_checkpoint8_pack): ``codes`` int8 of its shape and one ``scales``
+    byte per 32 elements of a row."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    dtype: torch.dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def restore(self) -> torch.Tensor:
+        """The tensor the codes stand for, in the type it was packed from."""
+        out = torch.empty(self.codes.shape, dtype=self.dtype, device=self.codes.device)
+        cols = self.codes.shape[-1]
+        with torch.cuda.device(out.device):
+            rc = _lib.lib().afiv_checkpoint8_restore(_ptr(self.codes), _ptr(self.scales), DTYPES[self.dtype],
+                                                     out.numel() // cols, cols, _ptr(out), _stream())
+        _lib.check(rc, "afiv_checkpoint8_restore")
+        return out
+
+
+def _empty_checkpoint(x: torch.Tensor) -> Checkpoint8:
+    cols = x.shape[-1]
+    return Checkpoint8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
+                       torch.empty(tuple(x.shape[:-1]) + ((cols + 31) // 32,), dtype=torch.uint8, device=x.device), x.dtype)
+
+
+def checkpoint8(x: torch.Tensor) -> Checkpoint8:
+    """x [..., cols] in 8 bits: blocks of 32 elements of a row share a power-of-two step, 1/64 of the
+    binade of their largest magnitude.  Elements that are not finite come back as NaN."""
+    return _pack(_first(x, "x"))
+
+
+def _pack(v: torch.Tensor) -> Checkpoint8:
+    rows, cols = _rows(v, "x"), v.shape[-1]
+    out = _empty_checkpoint(v)
+    with torch.cuda.device(v.device):
+        rc = _lib.lib().afiv_checkpoint8_pack(_ptr(v), DTYPES[v.dtype], rows, cols, _ptr(out.codes), _ptr(out.scales), _stream())
+    _lib.check(rc, "afiv_checkpoint8_pack")
+    return out
+
+
+# ---- linear layer ----------------------------------------------------------------------------
+@dataclass(frozen=True)
+class LinearSaved:
+    """What ``linear_act_backward`` needs besides the weight: the input (``x``, or ``eight``), and the
+    pre-activation (``pre``) or the derivative's codes (``dcodes``); neither for act "none"."""
+    x: torch.Tensor | None
+    eight: Checkpoint8 | None
+    pre: torch.Tensor | None
+    dcodes: torch.Tensor | None
+    act: str
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.x.shape if self.eight is None else self.eight.shape
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.x.dtype if self.eight is None else self.eight.dtype
+
+
+def _scratch(nbytes: int, device) -> torch.Tensor | None:
+    if nbytes < 0:
+        _lib.check(int(nbytes), "afiv_linear_act_scratch")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _linear(x, weight, bias, residual, act, want_pre: bool, want_codes: bool):
+    code = _act(act)
+    v = _first(x, "x")
+    m, k = _rows(v, "x"), v.shape[-1]
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] < 1:
+        raise ValueError("weight must be [out features, in features] with at least one of each")
+    n = weight.shape[0]
+    w = _like(weight, v, (n, k), "weight")
+    shape = tuple(v.shape[:-1]) + (n,)
+    b = None if bias is None else _like(bias, v, (n,), "bias")
+    r = None if residual is None else _like(residual, v, shape, "residual")
+    y = torch.empty(shape, dtype=v.dtype, device=v.device)
+    pre = torch.empty_like(y) if want_pre else None
+    dcodes = torch.empty(shape, dtype=torch.uint8, device=v.device) if want_codes else None
+    L = _lib.lib()
+    nbytes = L.afiv_linear_act_scratch(m, n, k)
+    with torch.cuda.device(v.device):
+        scratch = _scratch(nbytes, v.device)
+        rc = L.afiv_linear_act(_ptr(v), _ptr(w), _ptr(b), _ptr(r), DTYPES[v.dtype], code, m, n, k, _ptr(y), _ptr(pre), _ptr(dcodes),
+                               _ptr(scratch), nbytes, _stream())
+    _lib.check(rc, "afiv_linear_act")
+    return v, y, pre, dcodes
+
+
+def linear_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                       residual: torch.Tensor | None = None, act: str = "none", checkpoint8: bool = False):
+    """``act(x @ weight.T + bias) + residual`` and what its backward pass needs: (y, LinearSaved).
+    x [..., in], weight [out, in], bias [out], residual [..., out], all of one type.  With ``checkpoint8``
+    the input and the activation's derivative are kept in 8 bits (33/32 and 1 byte an element);
+    otherwise they are the input itself and the pre-activation in x's type (relu, leaky_relu: its sign,
+    one byte)."""
+    signs = act in ("relu", "leaky_relu")
+    want_codes = signs or (checkpoint8 and act != "none")
+    v, y, pre, dcodes = _linear(x, weight, bias, residual, act, act != "none" and not want_codes, want_codes)
+    eight = _pack(v) if checkpoint8 else None
+    return y, LinearSaved(None if checkpoint8 else v, eight, pre, dcodes, act)
+
+
+def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSaved, need=(True, True, True)):
+    """(dx, dweight, dbias) of ``linear_act_forward`` for the output gradient dy, each None where ``need`` is
+    false.  The residual's gradient is dy."""
+    g = _first(dy, "dy")
+    k, n = saved.shape[-1], weight.shape[0]
+    if g.dtype != saved.dtype:
+        raise TypeError(f"dy must be {saved.dtype}, got {g.dtype}")
+    g = _like(g, g, tuple(saved.shape[:-1]) + (n,), "dy")
+    w = _like(weight, g, (n, k), "weight")
+    m = g.numel() // n
+    dx = torch.empty(saved.shape, dtype=g.dtype, device=g.device) if need[0] else None
+    dw = torch.empty((n, k), dtype=g.dtype, device=g.device) if need[1] else None
+    db = torch.empty((n,), dtype=g.dtype, device=g.device) if need[2] else None
+    ran_on = (saved.x if saved.eight is None else saved.eight.codes).device
+    if g.device != ran_on:
+        raise ValueError(f"dy is on {g.device}, the forward pass ran on {ran_on}")
+    L = _lib.lib()
+    nbytes = L.afiv_linear_act_backward_scratch(m, n, k)
+    with torch.cuda.device(g.device):
+        scratch = _scratch(nbytes, g.device)
+        rc = L.afiv_linear_act_backward(_ptr(g), _ptr(saved.x), _ptr(saved.eight.codes if saved.eight else None),
+                                        _ptr(saved.eight.scales if saved.eight else None), _ptr(w), _ptr(saved.pre), _ptr(saved.dcodes),
+                                        DTYPES[g.dtype], _act(saved.act), m, n, k, _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), nbytes,
+                                        _stream())
+    _lib.check(rc, "afiv_linear_act_backward")
+    return dx, dw, db
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, eight):
+        y, s = linear_act_forward(x, weight, bias, residual, act, eight)
+        ctx.save_for_backward(weight, s.x, s.pre, s.dcodes, *((s.eight.codes, s.eight.scales) if eight else (None, None)))
+        ctx.act, ctx.dtype = act, y.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        weight, x, pre, dcodes, codes, scales = ctx.saved_tensors
+        saved = LinearSaved(x, None if codes is None else Checkpoint8(codes, scales, ctx.dtype), pre, dcodes, ctx.act)
+        need = ctx.needs_input_grad
+        grads = linear_act_backward(dy, weight, saved, need[:3]) if any(need[:3]) else (None, None, None)
+        return (*grads, dy if need[3] else None, None, None)
+
+
+def _graph(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+               act: str = "none", checkpoint8: bool = False) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``, differentiable once; arguments as ``linear_act_forward``."""
+    if _graph(x, weight, bias, residual):
+        return _LinearAct.apply(x, weight, bias, residual, act, bool(checkpoint8))
+    return _linear(x, weight, bias, residual, act, False, False)[1]
+
+
+# ---- batch normalisation, activation, dropout ---------------------------------------------------
+@dataclass(frozen=True)
+class NormSaved:
+    """What ``batch_norm_act_backward`` needs besides gamma and beta."""
+    x: torch.Tensor | None
+    eight: Checkpoint8 | None
+    stats: torch.Tensor                  # [2, features] float64: mean, 1 / sqrt(var + eps)
+    keep: torch.Tensor | None
+    act: str
+    drop_p: float
+
+
+def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, running_mean: torch.Tensor | None = None,
+                           running_var: torch.Tensor | None = None, act: str = "none", keep: torch.Tensor | None = None,
+                           drop_p: float = 0.0, momentum: float = 0.1, eps: float = 1e-5, checkpoint8: bool = False):
+    """``keep / (1 - drop_p) * act(batch_norm(x))`` with the batch's own statistics, and what its backward pass
+    needs: (y, NormSaved).  x [rows, features]; weight (gamma) and bias (beta) float32 [features]; running_mean and
+    running_var (both or none) float32 [features], updated in place as nn.BatchNorm1d does; keep: bool or
+    uint8 mask of x's shape, needed where drop_p > 0.  With ``checkpoint8`` x is kept in 8 bits."""
+    code = _act(act)
+    v = _first(x, "x")
+    if v.dim() != 2 or v.shape[1] < 1:
+        raise ValueError(f"x must be [rows, features], got {list(v.shape)}")
+    m, n = v.shape
+    if m < 2:
+        raise ValueError(f"batch statistics need more than one row, got {m}")
+    f32 = (torch.float32,)
+    gamma, beta = _like(weight, v, (n,), "weight", f32), _like(bias, v, (n,), "bias", f32)
+    if (running_mean is None) != (running_var is None):
+        raise ValueError("running_mean and running_var come together")
+    if running_mean is not None:
+        _like(running_mean, v, (n,), "running_mean", f32, output=True)
+        _like(running_var, v, (n,), "running_var", f32, output=True)
+    drop_p = float(drop_p)
+    if not 0.0 <= drop_p < 1.0:
+        raise ValueError(f"drop_p must lie in [0, 1), got {drop_p}")
+    if keep is None and drop_p > 0.0:
+        raise ValueError("drop_p > 0 needs a keep mask")
+    if keep is not None:
+        keep = _like(keep, v, (m, n), "keep", (torch.bool, torch.uint8))
+    y = torch.empty_like(v)
+    stats = torch.empty((2, n), dtype=torch.float64, device=v.device)
+    eight = _empty_checkpoint(v) if checkpoint8 else None
+    with torch.cuda.device(v.device):
+        scratch = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=v.device)
+        rc = _lib.lib().afiv_norm_act(_ptr(v), _ptr(gamma), _ptr(beta), _ptr(keep), DTYPES[v.dtype], code, m, n, float(eps), float(momentum),
+                                      drop_p, _ptr(running_mean), _ptr(running_var), _ptr(y), _ptr(stats),
+                                      _ptr(eight.codes if eight else None), _ptr(eight.scales if eight else None), _ptr(scratch), _stream())
+    _lib.check(rc, "afiv_norm_act")
+    if running_mean is not None:         # written behind torch's back: caches keyed on versions must see it
+        torch.autograd.graph.increment_version(running_mean)
+        torch.autograd.graph.increment_version(running_var)
+    return y, NormSaved(None if checkpoint8 else v, eight, stats, keep, act, drop_p)
+
+
+def batch_norm_act_backward(dy: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, saved: NormSaved, need_dx: bool = True):
+    """(dx, dweight, dbias) of ``batch_norm_act_forward`` for the output gradient dy; dx is None without ``need_dx``."""
+    g = _first(dy, "dy")
+    held = saved.x if saved.eight is None else saved.eight
+    if g.dtype != held.dtype:
+        raise TypeError(f"dy must be {held.dtype}, got {g.dtype}")
+    if g.device != saved.stats.device:
+        raise ValueError(f"dy is on {g.device}, the forward pass ran on {saved.stats.device}")
+    g = _like(g, g, held.shape, "dy")
+    m, n = g.shape
+    f32 = (torch.float32,)
+    gamma, beta = _like(weight, g, (n,), "weight", f32), _like(bias, g, (n,), "bias", f32)
+    dx = torch.empty_like(g) if need_dx else None
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
+    with torch.cuda.device(g.device):
+        scratch = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=g.device)
+        rc = _lib.lib().afiv_norm_act_backward(_ptr(g), _ptr(saved.x), _ptr(saved.eight.codes if saved.eight else None),
+                                               _ptr(saved.eight.scales if saved.eight else None), _ptr(gamma), _ptr(beta), _ptr(saved.keep),
+                                               _ptr(saved.stats), DTYPES[g.dtype], _act(saved.act), m, n, saved.drop_p, _ptr(dx),
+                                               _ptr(dgamma), _ptr(dbeta), _ptr(scratch), _stream())
+    _lib.check(rc, "afiv_norm_act_backward")
+    return dx, dgamma, dbeta
+
+
+class _BatchNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, running_mean, running_var, act, keep, drop_p, momentum, eps, eight):
+        y, s = batch_norm_act_forward(x, weight, bias, running_mean, running_var, act, keep, drop_p, momentum, eps, eight)
+        ctx.save_for_backward(weight, bias, s.x, s.stats, s.keep, *((s.eight.codes, s.eight.scales) if eight else (None, None)))
+        ctx.act, ctx.drop_p, ctx.dtype = act, s.drop_p, y.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        weight, bias, x, stats, keep, codes, scales = ctx.saved_tensors
+        saved = NormSaved(x, None if codes is None else Checkpoint8(codes, scales, ctx.dtype), stats, keep, ctx.act, ctx.drop_p)
+        need = ctx.needs_input_grad
+        dx, dgamma, dbeta = batch_norm_act_backward(dy, weight, bias, saved, need[0])
+        return (dx, dgamma if need[1] else None, dbeta if need[2] else None) + (None,) * 8
+
+
+def batch_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, running_mean: torch.Tensor | None = None,
+                   running_var: torch.Tensor | None = None, act: str = "none", keep: torch.Tensor | None = None, drop_p: float = 0.0,
+                   momentum: float = 0.1, eps: float = 1e-5, checkpoint8: bool = False) -> torch.Tensor:
+    """``keep / (1 - drop_p) * act(batch_norm(x))`` with the batch's own statistics, differentiable once;
+    arguments as ``batch_norm_act_forward``."""
+    if _graph(x, weight, bias):
+        return _BatchNormAct.apply(x, weight, bias, running_mean, running_var, act, keep, drop_p, momentum, eps, bool(checkpoint8))
+    return batch_norm_act_forward(x, weight, bias, running_mean, running_var, act, keep, drop_p, momentum, eps)[0]

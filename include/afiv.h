@@ -248,6 +248,71 @@ int afiv_ensemble_stats(const double *iv, const uint8_t *select, int64_t N, int6
 int afiv_ensemble_stats_groups(const double *iv, const uint8_t *select, int64_t groups, int64_t N,
                                int64_t points, double *stats_out, void *stream);
 
+/* ---- layer operators ---------------------------------------------------------------------------
+ * The pieces of the reference's [Linear, BatchNorm1d, activation, Dropout] stacks
+ * (cvae_model.py:64-105), forward and backward, for layers of any width and batches from one row.
+ * The reference runs them, and their gradients, in PyTorch on the CPU.  No object: weights are the
+ * caller's device arrays, scratch too.  Outputs must not overlap inputs or each other, except where
+ * said.  Arrays need no alignment beyond their elements'.  `dtype` is the element type of the arrays
+ * written as [..] T; sums and everything between input and output are FP32 or wider. */
+enum { AFIV_F32 = 0, AFIV_BF16 = 1, AFIV_F16 = 2 };
+enum {
+    AFIV_ACT_NONE = 0,
+    AFIV_ACT_RELU = 1,
+    AFIV_ACT_LEAKY_RELU = 2,   /* slope 0.2 (cvae_model.py:118) */
+    AFIV_ACT_TANH = 3,
+    AFIV_ACT_GELU = 4,         /* z Phi(z) */
+    AFIV_ACT_SILU = 5          /* z / (1 + exp(-z)) */
+};
+
+/* 8-bit checkpoint of x [rows,cols] T, to be kept between the passes of a training step instead of x:
+ * codes [rows,cols] and one scale byte per 32 elements of a row, scales [rows,ceil(cols/32)].  With E
+ * the biased exponent of the 32's largest finite magnitude (at least 1) an element is the nearest
+ * q 2^(E-133), q = -127..127, ties to even: off by at most 2^(E-134), or by less than
+ * 2^(E-133) above 127.5 steps.  Elements that are not finite are code -128 and come back as NaN.
+ * Restoring is exact in T. */
+int afiv_checkpoint8_pack(const void *x, int dtype, int64_t rows, int64_t cols, int8_t *codes, uint8_t *scales, void *stream);
+int afiv_checkpoint8_restore(const int8_t *codes, const uint8_t *scales, int dtype, int64_t rows, int64_t cols, void *x_out,
+                             void *stream);
+
+/* y [M,N] = act(x [M,K] w [N,K]^T + bias [N]) + residual [M,N], all T; bias and residual may be NULL.
+ * For the backward pass one of these is kept, or both NULL: pre_out [M,N] T = the pre-activation, or
+ * dcodes_out [M,N] = the activation's derivative in 8 bits (multiples of 1/200; relu and leaky_relu:
+ * the sign; unused and may be NULL for AFIV_ACT_NONE).  M >= 0; 1 <= N, K <= 2^24.
+ * scratch: device memory of at least afiv_linear_act_scratch(M, N, K) bytes (NULL where that is 0). */
+int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K);
+int afiv_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
+                    int64_t K, void *y, void *pre_out, uint8_t *dcodes_out, void *scratch, int64_t scratch_bytes, void *stream);
+
+/* Gradients of afiv_linear_act from dy [M,N] T: dx [M,K], dw [N,K], db [N], all T, each NULL if not
+ * wanted (the residual's gradient is dy).  The layer's input comes as x [M,K] T or, with x == NULL, as
+ * its 8-bit checkpoint (codes, scales); the derivative from pre [M,N] T or, with pre == NULL, from
+ * dcodes [M,N] (neither for AFIV_ACT_NONE).  w is needed for dx, the input for dw.  dy times the
+ * derivative is rounded to T before the products (FP32: not rounded), db is summed before that rounding. */
+int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K);
+int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w, const void *pre,
+                             const uint8_t *dcodes, int dtype, int act, int64_t M, int64_t N, int64_t K, void *dx, void *dw, void *db,
+                             void *scratch, int64_t scratch_bytes, void *stream);
+
+/* Training-mode BatchNorm1d, activation and dropout of x [M,N] T, M >= 2:
+ *   y = keep / (1 - drop_p) * act(gamma (x - mean) / sqrt(var + eps) + beta)
+ * with the batch's column means and biased variances.  keep: [M,N] bytes (0 = dropped, whatever the value
+ * was), or NULL for no dropout (drop_p = 0 then).  gamma, beta [N] float.  running_mean, running_var: both NULL, or
+ * [N] float, updated in place with `momentum` and the unbiased variance.  stats_out: [2,N] doubles,
+ * mean and 1/sqrt(var + eps), for the backward pass.  codes_out, scales_out: both NULL, or the 8-bit
+ * checkpoint of x.  1 <= N <= 2^24.  scratch: AFIV_NORM_SCRATCH_DOUBLES * N doubles. */
+#define AFIV_NORM_CHUNKS 256
+#define AFIV_NORM_SCRATCH_DOUBLES (2 * AFIV_NORM_CHUNKS + 2)
+int afiv_norm_act(const void *x, const float *gamma, const float *beta, const uint8_t *keep, int dtype, int act, int64_t M, int64_t N,
+                  double eps, double momentum, double drop_p, float *running_mean, float *running_var, void *y, double *stats_out,
+                  int8_t *codes_out, uint8_t *scales_out, double *scratch, void *stream);
+
+/* Gradients of afiv_norm_act from dy [M,N] T: dx [M,N] T (or NULL), dgamma, dbeta [N] float.  The input comes as
+ * x [M,N] T or, with x == NULL, as its 8-bit checkpoint (codes, scales). */
+int afiv_norm_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const float *gamma,
+                           const float *beta, const uint8_t *keep, const double *stats, int dtype, int act, int64_t M, int64_t N,
+                           double drop_p, void *dx, float *dgamma, float *dbeta, double *scratch, void *stream);
+
 /* ---- diagnostics: the kernels' own FP64 elementary functions, element-wise, so that unit tests
  * can check them against high-precision references.  No counterpart in the reference (which
  * calls libm / SciPy).  x, y, out0, out1: device [n]; y only for AFIV_MATH_ATAN2 (atan2(x, y));
