@@ -696,9 +696,10 @@ int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K)
     return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_forward_scratch(M, N, K);
 }
 
-int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K)
+int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype)
 {
-    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_backward_scratch(M, N, K);
+    if (bad_layer(dtype, 0)) return AFIV_E_ARG;
+    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_backward_scratch(M, N, K, dtype);
 }
 
 int afiv_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
@@ -723,7 +724,7 @@ int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes,
         if (!dy || (dx && !w) || (dw && !x && (!codes || !scales))) return AFIV_E_NULL;
         if (act != AFIV_ACT_NONE && !pre && !dcodes) return AFIV_E_NULL;
     }
-    const int64_t need = afiv_linear_backward_scratch(M, N, K);
+    const int64_t need = afiv_linear_backward_scratch(M, N, K, dtype);
     if (need > 0 && (!scratch || scratch_bytes < need)) return AFIV_E_WORKSPACE;
     return afiv_launch_linear_act_backward(dy, x, x ? nullptr : codes, x ? nullptr : scales, w, pre, pre ? nullptr : dcodes, dtype, act, M,
                                            N, K, dx, dw, db, (float *)scratch, as_stream(stream));

@@ -49,35 +49,68 @@ __device__ __forceinline__ void store_some(T *p, const Pack<T, N> &r, int n)
 // ---- activations ---------------------------------------------------------------------------
 constexpr float AFIV_SLOPE = 0.2f;      // leaky_relu: the slope of the reference's stacks (cvae_model.py:118)
 
-__device__ __forceinline__ float act_value(float z, int act)
+// f(z) and f'(z); whichever the caller drops costs nothing.  Built on the hardware's 2^x and reciprocal (1 ulp
+// each) and, for erfc, a polynomial: within 7e-7 of the value (12 FP32 half steps) at a third of the library
+// functions' instructions, which an epilogue of 128 outputs a lane feels.
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float &f, float &d)
 {
-    switch (act) {
-        case AFIV_ACT_RELU: return z > 0.0f ? z : (z == z ? 0.0f : z);
-        case AFIV_ACT_LEAKY_RELU: return z > 0.0f ? z : AFIV_SLOPE * z;
-        case AFIV_ACT_TANH: return tanhf(z);
-        case AFIV_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678f);
-        case AFIV_ACT_SILU: return z / (1.0f + expf(-z));
-        default: return z;
+    if constexpr (ACT == AFIV_ACT_RELU) {
+        f = z > 0.0f ? z : (z == z ? 0.0f : z);
+        d = z > 0.0f ? 1.0f : 0.0f;
+    } else if constexpr (ACT == AFIV_ACT_LEAKY_RELU) {
+        f = z > 0.0f ? z : AFIV_SLOPE * z;
+        d = z > 0.0f ? 1.0f : AFIV_SLOPE;
+    } else if constexpr (ACT == AFIV_ACT_TANH) {
+        // e = exp(-2 |z|): f = (1 - e) / (1 + e), f' = 4 e / (1 + e)^2, neither of which cancels far from zero;
+        // near zero f is its Taylor polynomial (next term under 1e-8 of it at 1/4)
+        const float a = fabsf(z);
+        const float e = __builtin_amdgcn_exp2f(a * -2.88539008f), r = __builtin_amdgcn_rcpf(1.0f + e), q = a * a;
+        const float near = a + a * q * (-0.333333333f + q * (0.133333333f + q * (-0.0539682540f + q * 0.0218694885f)));
+        f = copysignf(a < 0.25f ? near : (1.0f - e) * r, z);
+        if (z != z) f = z;
+        d = 4.0f * e * r * r;
+    } else if constexpr (ACT == AFIV_ACT_GELU) {
+        // Phi(-|z|) = exp(-z^2/2) erfcx(|z|/sqrt 2) / 2, erfcx(x) = P(t), t = 1 / (1 + 0.45 x): least squares fit of
+        // equal relative error, degree 8
+        const float a = fabsf(z);
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.318198052f * a);
+        const float dens = __builtin_amdgcn_exp2f(z * z * -0.721347520f);          // exp(-z^2/2)
+        float p = 0.0694841657f;
+        p = p * t - 0.251303992f;
+        p = p * t + 0.228051490f;
+        p = p * t + 0.0224661360f;
+        p = p * t + 0.198119277f;
+        p = p * t + 0.225212867f;
+        p = p * t + 0.254090404f;
+        p = p * t + 0.253880022f;
+        const float tail = 0.5f * p * t * dens, phi = z > 0.0f ? 1.0f - tail : tail;
+        // z Phi and z exp(-z^2/2) vanish at -infinity
+        f = z == -__builtin_inff() ? 0.0f : z * phi;
+        d = phi + (a == __builtin_inff() ? 0.0f : z * dens * 0.39894228f);
+    } else if constexpr (ACT == AFIV_ACT_SILU) {
+        // p = 1 / (1 + exp(-z)): f = z p, f' = p + z p (1 - p), from e = exp(-|z|)
+        const float e = __builtin_amdgcn_exp2f(fabsf(z) * -1.44269504f), r = __builtin_amdgcn_rcpf(1.0f + e);
+        const float p = z >= 0.0f ? r : e * r, q = z >= 0.0f ? e * r : r;
+        f = z == -__builtin_inff() ? 0.0f : z * p;
+        d = p + (fabsf(z) == __builtin_inff() ? 0.0f : z * (p * q));
+    } else {
+        f = z;
+        d = 1.0f;
     }
 }
 
-__device__ __forceinline__ float act_derivative(float z, int act)
+// calls f with the activation as a compile-time constant, so that loops stand inside the choice
+template <class F>
+__device__ __forceinline__ void with_act(int act, F &&f)
 {
     switch (act) {
-        case AFIV_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case AFIV_ACT_LEAKY_RELU: return z > 0.0f ? 1.0f : AFIV_SLOPE;
-        case AFIV_ACT_TANH: {                              // 4 e / (1 + e)^2, e = exp(-2 |z|): no cancellation at the ends
-            const float e = expf(-2.0f * fabsf(z)), s = 1.0f + e;
-            return 4.0f * e / (s * s);
-        }
-        case AFIV_ACT_GELU:
-            return 0.5f * erfcf(z * -0.70710678f) + z * expf(-0.5f * z * z) * 0.39894228f;
-        case AFIV_ACT_SILU: {                              // p (1 + z (1 - p)), 1 - p = e / (1 + e) at z >= 0
-            const float e = expf(-fabsf(z)), r = 1.0f / (1.0f + e);
-            const float p = z >= 0.0f ? r : e * r, q = z >= 0.0f ? e * r : r;
-            return p + z * (p * q);
-        }
-        default: return 1.0f;
+        case AFIV_ACT_RELU: f(std::integral_constant<int, AFIV_ACT_RELU>()); break;
+        case AFIV_ACT_LEAKY_RELU: f(std::integral_constant<int, AFIV_ACT_LEAKY_RELU>()); break;
+        case AFIV_ACT_TANH: f(std::integral_constant<int, AFIV_ACT_TANH>()); break;
+        case AFIV_ACT_GELU: f(std::integral_constant<int, AFIV_ACT_GELU>()); break;
+        case AFIV_ACT_SILU: f(std::integral_constant<int, AFIV_ACT_SILU>()); break;
+        default: f(std::integral_constant<int, AFIV_ACT_NONE>()); break;
     }
 }
 
@@ -85,17 +118,18 @@ __device__ __forceinline__ float act_derivative(float z, int act)
 // relu, leaky_relu: 1 where z > 0, else 0.  The others: the derivative lies in [-0.13, 1.13]; steps
 // of 1/200 put it at codes 1..253 around 27 = 0, with 0 and 1 exact and an error of at most 1/400
 // (a third of what e4m3 loses near 1).  255 = NaN.
-__device__ __forceinline__ uint8_t derivative_code(float z, int act)
+template <int ACT>
+__device__ __forceinline__ uint8_t derivative_code(float z, float d)
 {
-    if (act == AFIV_ACT_RELU || act == AFIV_ACT_LEAKY_RELU) return z > 0.0f ? 1 : 0;
-    const float d = act_derivative(z, act);
+    if constexpr (ACT == AFIV_ACT_RELU || ACT == AFIV_ACT_LEAKY_RELU) return z > 0.0f ? 1 : 0;
     return d == d ? (uint8_t)(int)(rintf(d * 200.0f) + 27.0f) : (uint8_t)255;
 }
-__device__ __forceinline__ float derivative_of_code(uint8_t c, int act)
+template <int ACT>
+__device__ __forceinline__ float derivative_of_code(uint8_t c)
 {
-    if (act == AFIV_ACT_RELU) return (float)c;
-    if (act == AFIV_ACT_LEAKY_RELU) return c ? 1.0f : AFIV_SLOPE;
-    return c == 255 ? __builtin_nanf("") : ((float)c - 27.0f) / 200.0f;
+    if constexpr (ACT == AFIV_ACT_RELU) return (float)c;
+    if constexpr (ACT == AFIV_ACT_LEAKY_RELU) return c ? 1.0f : AFIV_SLOPE;
+    return c == 255 ? __builtin_nanf("") : ((float)c - 27.0f) * 0.005f;      // within one FP32 rounding of the quotient
 }
 
 // ---- 8-bit checkpoints -----------------------------------------------------------------------

@@ -1,0 +1,4 @@
+// The linear layer's kernels for BF16 (a translation unit per element type: they compile side by side).
+#include "afiv_linear_kernels.h"
+
+AFIV_LINEAR_TYPE(__bf16, bf16)

@@ -1,0 +1,912 @@
+// A linear layer with its epilogue, y = f(x W^T + b) + r, and its backward products, for FP32, BF16
+// and FP16.  Replaces nn.Linear (+ activation) of the reference's stacks and their autograd
+// (cvae_model.py:64-105), for layers of any width.
+//
+//   forward    z[m,n] = sum_k x[m,k] W[n,k] + b[n];   y = f(z) + r
+//   backward   dz = dy f'(z);   dx = dz W;   dW = dz^T x;   db = sum_m dz
+//
+// The three products are one tiled kernel: C[i,j] = sum_l A[i,l] B[j,l], where an operand is stored
+// along l (x and W forward, dz for dx) or across it (W for dx; dz and x for dW).  Either way it
+// lies in LDS along l, 32 steps of l a row of 64 bytes, so one matrix instruction's operand is one
+// 16-byte LDS read; operands stored across l are transposed in registers, 4 x 4 elements at a time, on
+// their way in.  dz is formed there too (dy, and z or its 8-bit derivative codes), and so is an 8-bit
+// x: neither ever exists in memory.
+//
+// 16-bit types go to v_mfma_f32_16x16x32.  FP32 operands are split into three BF16 parts,
+// a = a1 + a2 + a3 (8 bits each, every difference exact), and the six products a1 b1, a1 b2, a2 b1,
+// a1 b3, a2 b2, a3 b1 are summed in FP32: what is dropped is 2^-26 of the product, a quarter of an FP32
+// rounding, and six BF16 products cost 6/16 of one FP32 matrix instruction's time.  Magnitudes
+// of 2^127 and above (infinities too) do not split; a workgroup that has loaded one does its
+// tile again with FP32 multiply-adds.  Parts below 2^-133 are lost, that is, an element under 2^-110
+// keeps fewer than 24 bits.
+//
+// Few rows (up to 16) take another kernel: W is read once, straight from memory into the matrix
+// instruction, by as many waves as the layer has.
+#pragma once
+
+#include "afiv_layer.h"
+
+#include <type_traits>
+
+#include "afiv_linear_plan.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+struct LinArgs {
+    // operands: A stored along l [R,L] or across [L,R]; B likewise [C,L] or [L,C]
+    const void *A, *B;
+    const void *pre;                      // A is dy: z, in the element type, or
+    const uint8_t *dcodes;                // its derivative codes (both NULL: dz = dy)
+    const int8_t *codes;                  // B is an 8-bit checkpoint
+    const uint8_t *scales;
+    int64_t R, C, L;
+    int act;
+    int64_t splits, l_per;                // the sum is cut into `splits` runs of l_per (a multiple of BK)
+    // epilogue of C[i,j]: + bias[j], activation (act_out), + residual[i,j]
+    const void *bias, *residual;
+    int act_out;
+    void *out, *pre_out;
+    uint8_t *dcodes_out;
+    float *partial;                       // splits > 1: [splits,R,C], finished by another kernel
+    void *db;                             // dW: db[i] = sum over l of A, by the workgroups of the first tile column
+    float *db_partial;                    // splits > 1: [splits,R]
+};
+
+enum Kind { ALONG, ALONG_DZ, ACROSS, ACROSS_DZ, ACROSS_EIGHT };
+constexpr bool across(Kind k) { return k >= ACROSS; }
+constexpr bool is_dz(Kind k) { return k == ALONG_DZ || k == ACROSS_DZ; }
+
+// what a thread holds of an operand between its global loads and its LDS stores: 8 steps of l of one
+// row (along) or 4 steps of 4 rows (across)
+template <class T, Kind K> struct Held {
+    static constexpr int N = across(K) ? 16 : 8;
+    Pack<T, (K == ACROSS_EIGHT ? 1 : N)> v;
+    Pack<T, (is_dz(K) ? N : 1)> z;                        // z, or the derivative codes in its first bytes
+    Pack<int8_t, (K == ACROSS_EIGHT ? 16 : 1)> q;
+    uint8_t e[4];
+};
+
+template <class T, Kind K>
+__device__ __forceinline__ void fetch(const LinArgs &a, const void *base, int64_t R, int64_t row, int64_t l, int64_t l_end, Held<T, K> &h)
+{
+    if constexpr (!across(K)) {
+        const int n = row < R ? (int)(l_end - l < 8 ? l_end - l : 8) : 0;      // may be negative
+        if (n <= 0) {
+            h.v = {};
+            if (is_dz(K)) h.z = {};
+            return;
+        }
+        const int64_t at = row * a.L + l;
+        h.v = load_some<T, 8>((const T *)base + at, n);
+        if constexpr (is_dz(K)) {
+            if (a.pre) h.z = load_some<T, 8>((const T *)a.pre + at, n);
+            else if (a.dcodes) {
+                const Pack<uint8_t, 8> c = load_some<uint8_t, 8>(a.dcodes + at, n);
+                __builtin_memcpy(&h.z, &c, 8);
+            }
+        }
+    } else {
+        const int n = (int)(R - row < 4 ? R - row : 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = l + i < l_end && n > 0;
+            const int64_t at = (l + i) * R + row;
+            if constexpr (K == ACROSS_EIGHT) {
+                Pack<int8_t, 4> q = {};
+                uint8_t e = 1;
+                if (in) {
+                    q = load_some<int8_t, 4>(a.codes + at, n);
+                    e = a.scales[(l + i) * ((R + 31) / 32) + row / 32];
+                }
+                __builtin_memcpy(&h.q.v[4 * i], &q, 4);
+                h.e[i] = e;
+            } else {
+                Pack<T, 4> v = {};
+                if (in) v = load_some<T, 4>((const T *)base + at, n);
+                __builtin_memcpy(&h.v.v[4 * i], &v, sizeof v);
+                if constexpr (is_dz(K)) {
+                    if (a.pre) {
+                        Pack<T, 4> z = {};
+                        if (in) z = load_some<T, 4>((const T *)a.pre + at, n);
+                        __builtin_memcpy(&h.z.v[4 * i], &z, sizeof z);
+                    } else if (a.dcodes) {
+                        Pack<uint8_t, 4> c = {};
+                        if (in) c = load_some<uint8_t, 4>(a.dcodes + at, n);
+                        __builtin_memcpy((char *)&h.z + 4 * i, &c, 4);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// the held elements in FP32
+template <class T, Kind K>
+__device__ __forceinline__ void values(const LinArgs &a, const Held<T, K> &h, float (&f)[Held<T, K>::N])
+{
+    constexpr int N = Held<T, K>::N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (K == ACROSS_EIGHT) f[i] = eight_value(h.q.v[i], h.e[i / 4]);
+        else f[i] = (float)h.v.v[i];
+    }
+    if constexpr (is_dz(K)) {
+        if (a.pre || a.dcodes)
+            with_act(a.act, [&](auto act) {
+                constexpr int ACT = decltype(act)::value;
+                if (a.pre) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        float y, d;
+                        act_both<ACT>((float)h.z.v[i], y, d);
+                        f[i] *= d;
+                    }
+                } else {
+                    uint8_t c[N];
+                    __builtin_memcpy(c, &h.z, N);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) f[i] *= derivative_of_code<ACT>(c[i]);
+                }
+            });
+    }
+}
+
+// one element, for the FP32 path of unsplittable tiles
+template <class T, Kind K>
+__device__ __forceinline__ float element(const LinArgs &a, const void *base, int64_t R, int64_t row, int64_t l)
+{
+    const int64_t at = across(K) ? l * R + row : row * a.L + l;
+    float f;
+    if constexpr (K == ACROSS_EIGHT) f = eight_value(a.codes[at], a.scales[l * ((R + 31) / 32) + row / 32]);
+    else f = (float)((const T *)base)[at];
+    if constexpr (is_dz(K)) {
+        if (a.pre || a.dcodes)
+            with_act(a.act, [&](auto act) {
+                float y, d = 1.0f;
+                if (a.pre) act_both<decltype(act)::value>((float)((const T *)a.pre)[at], y, d);
+                else d = derivative_of_code<decltype(act)::value>(a.dcodes[at]);
+                f *= d;
+            });
+    }
+    return f;
+}
+
+// LDS: row r's 16-byte chunk c (8 steps of l) of a tile stands at chunk c ^ swizzle(r): the 8 rows a
+// read touches at once, and the rows 4 apart that a transposing store does, fall on different banks
+__device__ __forceinline__ int swizzle(int r) { return ((r >> 1) ^ (r >> 3)) & 3; }
+__device__ __forceinline__ int lds_at(int r, int l) { return r * BK + (((l >> 3) ^ swizzle(r)) << 3) + (l & 7); }
+
+template <class T> struct Mma;
+template <> struct Mma<__bf16> {
+    static constexpr int PARTS = 1;
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<_Float16> {
+    static constexpr int PARTS = 1;
+    typedef f16x8 frag;
+    static __device__ __forceinline__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<float> : Mma<__bf16> { static constexpr int PARTS = 3; };
+
+// element type in LDS
+template <class T> struct Part { typedef T type; };
+template <> struct Part<float> { typedef __bf16 type; };
+
+// N values to consecutive places of each part's plane
+template <class T, int N>
+__device__ __forceinline__ void put(typename Part<T>::type *lds, int plane, const float (&f)[N])
+{
+    typedef typename Part<T>::type P;
+    if constexpr (Mma<T>::PARTS == 1) {
+        Pack<P, N> o;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o.v[i] = (P)f[i];
+        __builtin_memcpy(__builtin_assume_aligned(lds, sizeof o), &o, sizeof o);
+    } else {
+        Pack<P, N> o[3];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const P a = (P)f[i];
+            const float r = f[i] - (float)a;
+            const P b = (P)r;
+            o[0].v[i] = a;
+            o[1].v[i] = b;
+            o[2].v[i] = (P)(r - (float)b);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + p * plane, sizeof o[0]), &o[p], sizeof o[0]);
+    }
+}
+
+template <class T, Kind K, int ROWS>
+struct Operand {
+    // units of work of a tile: 8 steps x 1 row, or 4 steps x 4 rows
+    static constexpr int UNITS = across(K) ? (BK / 4) * (ROWS / 4) : (BK / 8) * ROWS;
+    static constexpr int PER = (UNITS + THREADS - 1) / THREADS;
+    Held<T, K> h[PER];
+
+    static __device__ __forceinline__ void place(int u, int &row, int &l)
+    {
+        if (across(K)) {                  // neighbouring lanes: neighbouring rows, in pairs of l for the LDS stores
+            row = (u % (ROWS / 4)) * 4;
+            l = (u / (ROWS / 4)) * 4;
+        } else {
+            row = u / (BK / 8);
+            l = (u % (BK / 8)) * 8;
+        }
+    }
+    __device__ __forceinline__ void load(const LinArgs &a, const void *base, int64_t R, int64_t row0, int64_t l0, int64_t l_end, int tid)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int u = i * THREADS + tid;
+            if (UNITS % THREADS == 0 || u < UNITS) {
+                int row, l;
+                place(u, row, l);
+                fetch<T, K>(a, base, R, row0 + row, l0 + l, l_end, h[i]);
+            }
+        }
+    }
+    // to LDS; sums[4 i + j]: running sums over l of the four rows of unit i (across only)
+    template <bool SUMS>
+    __device__ __forceinline__ void store(const LinArgs &a, typename Part<T>::type *lds, int tid, float &amax, float *sums)
+    {
+        constexpr int N = Held<T, K>::N, PLANE = ROWS * BK;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int u = i * THREADS + tid;
+            if (UNITS % THREADS == 0 || u < UNITS) {
+                int row, l;
+                place(u, row, l);
+                float f[N];
+                values<T, K>(a, h[i], f);
+                if constexpr (Mma<T>::PARTS == 3) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(f[j]));
+                }
+                if constexpr (!across(K)) put<T, 8>(lds + lds_at(row, l), PLANE, f);
+                else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float t[4] = {f[j], f[4 + j], f[8 + j], f[12 + j]};
+                        put<T, 4>(lds + lds_at(row + j, l), PLANE, t);
+                        if (SUMS) sums[4 * i + j] += (t[0] + t[1]) + (t[2] + t[3]);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// W outputs of row i from column j on, from their sums z.  EPI: the forward epilogue.
+template <class T, bool EPI, int W>
+__device__ __forceinline__ void finish(const LinArgs &a, int64_t i, int64_t j, float (&z)[W])
+{
+    const int n = (int)(a.C - j < W ? a.C - j : W);
+    const int64_t at = i * a.C + j;
+    if constexpr (EPI) {
+        if (a.bias) {
+            const Pack<T, W> b = load_some<T, W>((const T *)a.bias + j, n);
+#pragma unroll
+            for (int q = 0; q < W; ++q) z[q] += (float)b.v[q];
+        }
+        if (a.pre_out) {
+            Pack<T, W> o;
+#pragma unroll
+            for (int q = 0; q < W; ++q) o.v[q] = (T)z[q];
+            store_some<T, W>((T *)a.pre_out + at, o, n);
+        }
+        Pack<uint8_t, W> c = {};
+        with_act(a.act_out, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+#pragma unroll
+            for (int q = 0; q < W; ++q) {
+                float y, d;
+                act_both<ACT>(z[q], y, d);
+                if (a.dcodes_out) c.v[q] = derivative_code<ACT>(z[q], d);
+                z[q] = y;
+            }
+        });
+        if (a.dcodes_out) store_some<uint8_t, W>(a.dcodes_out + at, c, n);
+        if (a.residual) {
+            const Pack<T, W> r = load_some<T, W>((const T *)a.residual + at, n);
+#pragma unroll
+            for (int q = 0; q < W; ++q) z[q] += (float)r.v[q];
+        }
+    }
+    Pack<T, W> o;
+#pragma unroll
+    for (int q = 0; q < W; ++q) o.v[q] = (T)z[q];
+    if (EPI || a.out) store_some<T, W>((T *)a.out + at, o, n);      // no out: only db was asked for
+}
+
+// A wave's 16 TR x 16 TC outputs from its accumulators (lane = row lane & 15, four columns from 4 (lane >> 4) of
+// each 16 x 16 block) by way of LDS, SLABS blocks of 16 rows at a time in the wave's own room: a lane then
+// has 8 neighbouring columns, the memory accesses are whole lines, and the epilogue's code stands once.
+// The 16-byte chunks of a row are permuted by the row so that a column of writes meets all banks.
+template <class T, bool EPI, int TR, int TC, int SLABS>
+__device__ __forceinline__ void write_out(const LinArgs &a, const f32x4 (&acc)[TR][TC], int64_t row0, int64_t col0, int64_t split, int lane,
+                                          float *room)
+{
+    constexpr int COLS = 16 * TC, CHUNKS = COLS / 4, UNITS = 16 * COLS / 8;      // of a slab
+    static_assert(TR % SLABS == 0 && UNITS % 64 == 0, "whole passes");
+#pragma unroll 1
+    for (int phase = 0; phase < TR / SLABS; ++phase) {
+#pragma unroll
+        for (int ph = 0; ph < TR / SLABS; ++ph)
+            if (ph == phase) {
+#pragma unroll
+                for (int i = 0; i < SLABS; ++i)
+#pragma unroll
+                    for (int j = 0; j < TC; ++j) {
+                        const int r = lane & 15, c = (4 * j + (lane >> 4)) ^ (r & (CHUNKS - 1));
+                        *(f32x4 *)&room[(i * 16 + r) * COLS + c * 4] = acc[ph * SLABS + i][j];
+                    }
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int u = lane; u < SLABS * UNITS; u += 64) {
+            const int r = u / (COLS / 8), c = u % (COLS / 8) * 2;
+            const int64_t row = row0 + phase * SLABS * 16 + r, col = col0 + c * 4;
+            if (row < a.R && col < a.C) {
+                float z[8];
+                const f32x4 lo = *(const f32x4 *)&room[r * COLS + ((c ^ (r & (CHUNKS - 1))) * 4)];
+                const f32x4 hi = *(const f32x4 *)&room[r * COLS + (((c + 1) ^ (r & (CHUNKS - 1))) * 4)];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    z[q] = lo[q];
+                    z[4 + q] = hi[q];
+                }
+                if (a.splits > 1) {
+                    Pack<float, 8> o;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) o.v[q] = z[q];
+                    store_some<float, 8>(a.partial + (split * a.R + row) * a.C + col, o, (int)(a.C - col < 8 ? a.C - col : 8));
+                } else finish<T, EPI, 8>(a, row, col, z);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// workgroup -> split and tile: tile columns run fastest within a band of 8 tile rows, so that workgroups at work
+// together share both operands' tiles; consecutive workgroups go round the 8 XCDs, each with an L2 of its own, so
+// each XCD is given a run of consecutive tiles
+__device__ __forceinline__ void place_tile(const LinArgs &a, int br, int bc, int64_t &split, int64_t &tr, int64_t &tc)
+{
+    const int64_t tiles_r = (a.R + br - 1) / br, tiles_c = (a.C + bc - 1) / bc, tiles = tiles_r * tiles_c;
+    const int64_t all = gridDim.x, each = all / 8, spare = all % 8, xcd = blockIdx.x % 8;
+    int64_t b = xcd * each + (xcd < spare ? xcd : spare) + blockIdx.x / 8;
+    split = b / tiles;
+    b -= split * tiles;
+    const int64_t band = b / (8 * tiles_c), in = b - band * 8 * tiles_c;
+    const int64_t rows_here = tiles_r - band * 8 < 8 ? tiles_r - band * 8 : 8;
+    tr = band * 8 + in % rows_here;
+    tc = in / rows_here;
+}
+
+// Tile of 32 TR x 32 TC outputs, four waves of 16 TR x 16 TC.  The matrix instruction gets B as its
+// first operand: a lane then holds four neighbouring columns of one row of C.
+template <class T, Kind KA, Kind KB, int TR, int TC>
+__global__ __launch_bounds__(THREADS) void tile_kernel(LinArgs a)
+{
+    constexpr int BR = 32 * TR, BC = 32 * TC, PARTS = Mma<T>::PARTS;
+    typedef typename Part<T>::type P;
+    typedef typename Mma<T>::frag frag;
+    constexpr bool SUMS = KA == ACROSS_DZ;
+    constexpr int ROOM = 16 * 16 * TC;                                      // floats of a wave's epilogue
+    constexpr int BYTES = PARTS * (BR + BC) * BK * 2;
+    static_assert(BYTES >= 4 * ROOM * 4, "the epilogue's room");
+    __shared__ __align__(16) char lds[BYTES];
+    P *const sA = (P *)lds, *const sB = sA + PARTS * BR * BK;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wr = (wave & 1) * 16 * TR, wc = (wave >> 1) * 16 * TC;
+
+    int64_t split, tr, tc;
+    place_tile(a, BR, BC, split, tr, tc);
+    const int64_t row0 = tr * BR, col0 = tc * BC;
+    const int64_t l_begin = split * a.l_per, l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
+
+    f32x4 acc[TR][TC] = {};
+    Operand<T, KA, BR> oa;
+    Operand<T, KB, BC> ob;
+    float amax = 0.0f;
+    float sums[SUMS ? 4 * Operand<T, KA, BR>::PER : 1] = {};
+    const bool want_sums = SUMS && a.db && tc == 0;
+
+    if (l_begin < l_end) {
+        oa.load(a, a.A, a.R, row0, l_begin, l_end, tid);
+        ob.load(a, a.B, a.C, col0, l_begin, l_end, tid);
+    }
+    for (int64_t l0 = l_begin; l0 < l_end; l0 += BK) {
+        __syncthreads();
+        oa.template store<SUMS>(a, sA, tid, amax, sums);
+        ob.template store<false>(a, sB, tid, amax, nullptr);
+        __syncthreads();
+        if (l0 + BK < l_end) {
+            oa.load(a, a.A, a.R, row0, l0 + BK, l_end, tid);
+            ob.load(a, a.B, a.C, col0, l0 + BK, l_end, tid);
+        }
+        frag fa[PARTS][TR], fb[PARTS][TC];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+            for (int i = 0; i < TR; ++i) fa[p][i] = *(const frag *)&sA[p * BR * BK + lds_at(wr + 16 * i + (lane & 15), (lane >> 4) * 8)];
+#pragma unroll
+            for (int j = 0; j < TC; ++j) fb[p][j] = *(const frag *)&sB[p * BC * BK + lds_at(wc + 16 * j + (lane & 15), (lane >> 4) * 8)];
+        }
+#pragma unroll
+        for (int p = PARTS - 1; p >= 0; --p)                  // small products first
+#pragma unroll
+            for (int q = 0; q <= p; ++q)
+#pragma unroll
+                for (int i = 0; i < TR; ++i)
+#pragma unroll
+                    for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[q][j], fa[p - q][i], acc[i][j]);
+    }
+
+    if constexpr (PARTS == 3) {
+        if (__syncthreads_or(!(amax < 0x1p127f))) {
+#pragma unroll 1
+            for (int i = 0; i < TR; ++i)
+#pragma unroll 1
+                for (int j = 0; j < TC; ++j)
+#pragma unroll 1
+                    for (int q = 0; q < 4; ++q) {
+                        const int64_t row = row0 + wr + 16 * i + (lane & 15), col = col0 + wc + 16 * j + (lane >> 4) * 4 + q;
+                        float s = 0.0f;
+                        if (row < a.R && col < a.C)
+                            for (int64_t l = l_begin; l < l_end; ++l)
+                                s = __builtin_fmaf(element<T, KA>(a, a.A, a.R, row, l), element<T, KB>(a, a.B, a.C, col, l), s);
+#pragma unroll
+                        for (int ii = 0; ii < TR; ++ii)
+#pragma unroll
+                            for (int jj = 0; jj < TC; ++jj)
+#pragma unroll
+                                for (int qq = 0; qq < 4; ++qq)
+                                    if (ii == i && jj == j && qq == q) acc[ii][jj][qq] = s;
+                    }
+        }
+    }
+
+    if (want_sums) {                       // the same for the whole workgroup
+        float *s = (float *)sA;            // [BK / 4][BR]
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < Operand<T, KA, BR>::PER; ++i) {
+            const int u = i * THREADS + tid;
+            if (u < Operand<T, KA, BR>::UNITS) {
+                int row, l;
+                Operand<T, KA, BR>::place(u, row, l);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[(l / 4) * BR + row + j] = sums[4 * i + j];
+            }
+        }
+        __syncthreads();
+        for (int r = tid; r < BR; r += THREADS)
+            if (row0 + r < a.R) {
+                float t = 0.0f;
+                for (int i = 0; i < BK / 4; ++i) t += s[i * BR + r];
+                if (a.splits > 1) a.db_partial[split * a.R + row0 + r] = t;
+                else ((T *)a.db)[row0 + r] = (T)t;
+            }
+    }
+
+    __syncthreads();
+    write_out<T, KA == ALONG, TR, TC, 1>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)lds + wave * ROOM);
+}
+
+// the splits' sums, in their order, and the epilogue
+template <class T, bool EPI>
+__global__ __launch_bounds__(THREADS) void join_kernel(LinArgs a)
+{
+    const int64_t quads = (a.C + 3) / 4, total = a.R * quads;
+    for (int64_t u = (int64_t)blockIdx.x * THREADS + threadIdx.x; u < total; u += (int64_t)gridDim.x * THREADS) {
+        const int64_t i = u / quads, j = (u - i * quads) * 4;
+        const int n = (int)(a.C - j < 4 ? a.C - j : 4);
+        float z[4] = {};
+#pragma unroll 4
+        for (int64_t s = 0; s < a.splits; ++s) {
+            const Pack<float, 4> v = load_some<float, 4>(a.partial + (s * a.R + i) * a.C + j, n);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[q] += v.v[q];
+        }
+        finish<T, EPI, 4>(a, i, j, z);
+    }
+    if (a.db)
+        for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < a.R; i += (int64_t)gridDim.x * THREADS) {
+            float t = 0.0f;
+            for (int64_t s = 0; s < a.splits; ++s) t += a.db_partial[s * a.R + i];
+            ((T *)a.db)[i] = (T)t;
+        }
+}
+
+// ---- large products of 16-bit operands ---------------------------------------------------------
+// The same product for operands that can go from memory to LDS as they are (16-bit types, rows of a
+// multiple of 16 bytes, no dz, no checkpoint).  Steps of 64: a tile's rows are 128 bytes (along l) or
+// its 64 steps of l are rows of 2 BR bytes (across), and lie in LDS as the loads leave them, 1024 consecutive
+// bytes an instruction; what keeps the reads off each other's banks is therefore a permutation of the
+// global addresses: 16-byte chunk c of row r stands at c ^ (r & 7), 32-byte block c of step l at
+// c ^ key(l).  Operands across l are transposed by the LDS read itself (ds_read_b64_tr_b16).
+// Two buffers; one barrier a step: the loads of the next step run behind this one's products.
+__device__ __forceinline__ int across_key(int l) { return (l & 3) | ((l >> 1) & 4); }
+
+typedef __attribute__((address_space(3))) void *lds_ptr;
+
+template <class T, bool XS, int ROWS, int WAVES, int TN>
+struct Direct {
+    typedef typename Mma<T>::frag frag;
+    static constexpr int PER = ROWS * FK * 2 / 1024 / WAVES;      // loads of a wave
+    static_assert(PER * WAVES * 1024 == ROWS * FK * 2, "whole loads");
+    static constexpr int LSTEP = XS ? 1024 / (2 * ROWS) : 0;      // steps of l from one load of a wave to the next
+    static constexpr int BASES = XS ? TN : FK / 32;
+    uint32_t off[PER];                    // byte offset from the tile's corner; beyond the matrix: out of range
+    uint32_t l_first;                     // step of l of the first load
+    uint32_t at[BASES];                   // where a lane's reads start
+
+    // w0: first of the wave's 16 TN rows (a multiple of 8 blocks of 16, or of TN of them)
+    __device__ __forceinline__ void init(int64_t R, int64_t L, int64_t row0, int w0, int wave, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int byte = (wave * PER + i) * 1024 + lane * 16;
+            if (!XS) {
+                const int r = byte / 128, c = (lane & 7) ^ (lane >> 3);
+                off[i] = row0 + r < R ? (uint32_t)(r * L * 2 + c * 16) : 0x80000000u;
+            } else {
+                const int l = byte / (2 * ROWS), pos = byte % (2 * ROWS) / 16;
+                const int col = ((pos >> 1) ^ across_key(l)) * 16 + (pos & 1) * 8;
+                off[i] = row0 + col < R ? (uint32_t)((l * R + col) * 2) : 0x80000000u;
+            }
+        }
+        if (!XS) {
+            l_first = ((lane & 7) ^ (lane >> 3)) * 8;
+#pragma unroll
+            for (int kk = 0; kk < FK / 32; ++kk) at[kk] = (w0 + (lane & 15)) * 128 + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
+        } else {
+            l_first = (wave * PER * 1024 + lane * 16) / (2 * ROWS);
+            // 16 lanes read 4 steps x 16 rows, 8 bytes each, and get 4 steps of a row each
+            const int l = (lane >> 4) * 8 + ((lane >> 2) & 3);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) at[i] = l * (2 * ROWS) + ((((w0 >> 4) + i) ^ across_key(l)) << 5) + (lane & 3) * 8;
+        }
+    }
+    __device__ __forceinline__ void load(const T *base, int64_t R, int64_t L, int64_t row0, int64_t l0, int64_t l_end, char *lds, int wave) const
+    {
+#if defined(__HIP_DEVICE_COMPILE__)             // buffer resources have no host type
+        const T *corner = base + (XS ? l0 * R + row0 : row0 * L + l0);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)corner, 0, 0x7fffffff, 0x00020000);
+        const int left = (int)(l_end - l0 < FK ? l_end - l0 : FK);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (wave * PER + i) * 1024), 16,
+                                                     (int)l_first < left - i * LSTEP ? off[i] : 0x80000000u, 0, 0, 0);
+#endif
+    }
+    // rows 16 i + (lane & 15) of the wave's, steps 32 kk + 8 (lane >> 4) ..+7
+    __device__ __forceinline__ frag read(const char *lds, int i, int kk) const
+    {
+        frag f;
+        if constexpr (!XS) f = *(const frag *)(lds + at[kk] + i * 2048);
+        else {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            s16x4 h[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds + at[i] + (kk * 32 + p * 4) * (2 * ROWS)));
+            __builtin_memcpy(&f, h, 16);
+        }
+        return f;
+    }
+};
+
+// WR x WC waves of 16 TR x 16 TC outputs
+template <class T, bool XA, bool XB, int WR, int WC, int TR, int TC>
+__global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a)
+{
+    constexpr int W = WR * WC, BR = 16 * TR * WR, BC = 16 * TC * WC;
+    typedef typename Mma<T>::frag frag;
+    constexpr int STAGE = (BR + BC) * FK * 2;
+    __shared__ __align__(1024) char lds[2 * STAGE];
+    constexpr int ROOM = 2 * STAGE / W / 4, SLABS = ROOM / (16 * 16 * TC) < TR ? ROOM / (16 * 16 * TC) : TR;   // floats a wave
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = (wave % WR) * 16 * TR, wc = (wave / WR) * 16 * TC;
+    int64_t split, tr, tc;
+    place_tile(a, BR, BC, split, tr, tc);
+    const int64_t row0 = tr * BR, col0 = tc * BC;
+    const int64_t l_begin = split * a.l_per, l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
+    Direct<T, XA, BR, W, TR> da;
+    Direct<T, XB, BC, W, TC> db;
+    da.init(a.R, a.L, row0, wr, wave, lane);
+    db.init(a.C, a.L, col0, wc, wave, lane);
+    f32x4 acc[TR][TC] = {};
+
+    auto load = [&](char *s, int64_t l0) {
+        if (l0 < l_end) {
+            da.load((const T *)a.A, a.R, a.L, row0, l0, l_end, s, wave);
+            db.load((const T *)a.B, a.C, a.L, col0, l0, l_end, s + BR * FK * 2, wave);
+        }
+    };
+    auto multiply = [&](const char *s) {
+#pragma unroll
+        for (int kk = 0; kk < FK / 32; ++kk) {
+            frag fa[TR], fb[TC];
+#pragma unroll
+            for (int j = 0; j < TC; ++j) fb[j] = db.read(s + BR * FK * 2, j, kk);
+#pragma unroll
+            for (int i = 0; i < TR; ++i) fa[i] = da.read(s, i, kk);
+#pragma unroll
+            for (int i = 0; i < TR; ++i)
+#pragma unroll
+                for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
+        }
+    };
+    // every load of this wave has arrived (vmcnt 0) before any wave reads the tile, and every read of the
+    // other buffer is done before any wave loads into it
+    auto meet = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();
+    };
+    int here = 0;
+    load(lds, l_begin);
+#pragma unroll 1
+    for (int64_t l0 = l_begin; l0 < l_end; l0 += FK) {
+        meet();
+        load(lds + (STAGE - here), l0 + FK);
+        multiply(lds + here);
+        here = STAGE - here;
+    }
+    __syncthreads();
+    write_out<T, !XA && !XB, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)lds + wave * ROOM);
+}
+
+// dz = dy f'(z) for the direct products, and the partial sums of db: rows_per rows a workgroup of 64 lanes
+// (8 columns each) by 4 rows.  dz may be NULL (no activation: db alone).
+template <class T>
+__global__ __launch_bounds__(THREADS) void dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, const uint8_t *__restrict__ dcodes, int act,
+                                                     int64_t M, int64_t N, int64_t rows_per, T *__restrict__ dz, float *__restrict__ partial)
+{
+    __shared__ float lds[4][512];
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int64_t col = ((int64_t)blockIdx.x * 64 + tx) * 8;
+    const int n = (int)(N - col < 8 ? N - col : 8);
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per, r1 = r0 + rows_per < M ? r0 + rows_per : M;
+    float sum[8] = {};
+    if (n > 0)
+        with_act(act, [&](auto actc) {
+            constexpr int ACT = decltype(actc)::value;
+#pragma unroll 2
+            for (int64_t r = r0 + ty; r < r1; r += 4) {
+                const int64_t at = r * N + col;
+                const Pack<T, 8> v = load_some<T, 8>(dy + at, n);
+                float f[8];
+                if constexpr (ACT == AFIV_ACT_NONE) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = (float)v.v[i];
+                } else if (pre) {
+                    const Pack<T, 8> z = load_some<T, 8>(pre + at, n);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float y, d;
+                        act_both<ACT>((float)z.v[i], y, d);
+                        f[i] = (float)v.v[i] * d;
+                    }
+                } else {
+                    const Pack<uint8_t, 8> c = load_some<uint8_t, 8>(dcodes + at, n);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = (float)v.v[i] * derivative_of_code<ACT>(c.v[i]);
+                }
+                Pack<T, 8> o;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    sum[i] += f[i];
+                    o.v[i] = (T)f[i];
+                }
+                if (ACT != AFIV_ACT_NONE && dz) store_some<T, 8>(dz + at, o, n);
+            }
+        });
+    if (!partial) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lds[ty][tx * 8 + i] = sum[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 512; c += THREADS)
+        if ((int64_t)blockIdx.x * 512 + c < N)
+            partial[(int64_t)blockIdx.y * N + (int64_t)blockIdx.x * 512 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
+}
+
+// db from the partial sums: 16 columns a workgroup, 16 threads each over the chunks
+template <class T>
+__global__ __launch_bounds__(THREADS) void db_kernel(const float *__restrict__ partial, int64_t chunks, int64_t N, T *__restrict__ db)
+{
+    __shared__ float lds[16][16];
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int64_t col = (int64_t)blockIdx.x * 16 + tx;
+    float s = 0.0f;
+    if (col < N)
+        for (int64_t c = ty; c < chunks; c += 16) s += partial[c * N + col];
+    lds[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && col < N) {
+        for (int i = 1; i < 16; ++i) s += lds[i][tx];
+        db[col] = (T)s;
+    }
+}
+
+// ---- few rows ----------------------------------------------------------------------------------
+// R <= 16 rows of A (stored along l) against 16 rows of B a workgroup: the matrix instruction's 16 columns
+// are the rows of A, its rows those of B, and both operands go from memory to registers 16 bytes a
+// lane.  The workgroup's waves take steps of l in turn and are summed in LDS, wave by wave.
+template <class T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinArgs a)
+{
+    __shared__ float part[WAVES][16][FEW + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t col0 = (int64_t)blockIdx.x * 16, col = col0 + (lane & 15), row = lane & 15;
+    f32x4 acc = {};
+    constexpr int STEP = 32;
+    const T *pa = (const T *)a.A + row * a.L, *pb = (const T *)a.B + col * a.L;
+    const bool ina = row < a.R, inb = col < a.C;
+#pragma unroll 4
+    for (int64_t l = (int64_t)wave * STEP + (lane >> 4) * 8; l - (lane >> 4) * 8 < a.L; l += WAVES * STEP) {
+        const int n = (int)(a.L - l < 8 ? a.L - l : 8);
+        Pack<T, 8> va = {}, vb = {};
+        if (n > 0 && ina) va = load_some<T, 8>(pa + l, n);
+        if (n > 0 && inb) vb = load_some<T, 8>(pb + l, n);
+        if constexpr (sizeof(T) == 2) {
+            typename Mma<T>::frag fa, fb;
+            __builtin_memcpy(&fa, &va, 16);
+            __builtin_memcpy(&fb, &vb, 16);
+            acc = Mma<T>::mul(fb, fa, acc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(vb.v[i], va.v[i], acc, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) part[wave][(lane >> 4) * 4 + q][lane & 15] = acc[q];
+    __syncthreads();
+    if (tid < 64) {                                            // lane: row = lane & 15, four columns
+        float z[4] = {};
+        for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[q] += part[w][(lane >> 4) * 4 + q][lane & 15];
+        const int64_t j = col0 + (lane >> 4) * 4;
+        if (ina && j < a.C) finish<T, true, 4>(a, row, j, z);
+    }
+}
+
+// ---- launches ----------------------------------------------------------------------------------
+int ok() { return hipGetLastError() == hipSuccess ? AFIV_OK : AFIV_E_HIP; }
+
+template <class T, bool EPI>
+void join(const LinArgs &a, hipStream_t s)
+{
+    const int64_t units = a.R * ((a.C + 3) / 4), blocks = (units + THREADS - 1) / THREADS;
+    hipLaunchKernelGGL((join_kernel<T, EPI>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(THREADS), 0, s, a);
+}
+
+template <class T, Kind KA, Kind KB>
+int product(LinArgs a, float *scratch, hipStream_t s)
+{
+    const Plan p = plan_for(a.R, a.C, a.L);
+    if (p.tiles == 0) return AFIV_OK;
+    a.splits = p.splits;
+    a.l_per = p.l_per;
+    a.partial = scratch;
+    a.db_partial = scratch + p.splits * a.R * a.C;
+    const dim3 grid((unsigned)(p.tiles * p.splits));
+    if (big_tiles(a.R, a.C)) hipLaunchKernelGGL((tile_kernel<T, KA, KB, 4, 4>), grid, dim3(THREADS), 0, s, a);
+    else hipLaunchKernelGGL((tile_kernel<T, KA, KB, 2, 2>), grid, dim3(THREADS), 0, s, a);
+    if (p.splits > 1) join<T, KA == ALONG>(a, s);
+    return ok();
+}
+
+template <class T, bool XA, bool XB>
+int direct(LinArgs a, float *scratch, hipStream_t s)
+{
+    const Plan p = direct_plan(a.R, a.C, a.L);
+    a.splits = p.splits;
+    a.l_per = p.l_per;
+    a.partial = scratch;
+    const dim3 grid((unsigned)(p.tiles * p.splits));
+    if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, XA, XB, 2, 4, 8, 4>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((direct_kernel<T, XA, XB, 2, 2, 4, 4>), grid, dim3(256), 0, s, a);
+    if (p.splits > 1) join<T, !XA && !XB>(a, s);
+    return ok();
+}
+
+template <class T>
+int forward(const LinArgs &a, float *scratch, hipStream_t s)
+{
+    if (a.R <= FEW && a.R > 0 && a.C > 0) {
+        const dim3 grid((unsigned)((a.C + 15) / 16));
+        // 16 waves where the layer has few workgroups to fill the chip with
+        if (grid.x < 512 && a.L >= 512) hipLaunchKernelGGL((few_rows_kernel<T, 16>), grid, dim3(1024), 0, s, a);
+        else hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, dim3(256), 0, s, a);
+        return ok();
+    }
+    if constexpr (sizeof(T) == 2)
+        if (direct_rows(a.L) && direct_pays(a.R, a.C, a.L) && aligned(a.A) && aligned(a.B)) return direct<T, false, false>(a, scratch, s);
+    return product<T, ALONG, ALONG>(a, scratch, s);
+}
+
+template <class T>
+int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w, const void *pre,
+             const uint8_t *dcodes, int act, int64_t M, int64_t N, int64_t K, void *dx, void *dw, void *db, float *scratch, hipStream_t s)
+{
+    LinArgs a = {};
+    a.A = dy; a.act = act;
+    if (act != AFIV_ACT_NONE) { a.pre = pre; a.dcodes = dcodes; }
+    LinArgs d = a;
+    d.B = w; d.R = M; d.C = K; d.L = N; d.out = dx;
+    if constexpr (sizeof(T) == 2)
+        if (direct_backward(M, N, K) && aligned(dy) && aligned(w) && aligned(x) && aligned(scratch)) {
+            const Places p = places(M, N, K);
+            char *at = (char *)scratch;
+            T *dz = (T *)(at + p.dz);
+            float *partial = db ? (float *)(at + p.db) : nullptr;
+            if (act != AFIV_ACT_NONE || db) {
+                const int64_t cb = (N + 511) / 512, chunks = std::min(DB_CHUNKS, std::max<int64_t>(1, std::min((2048 + cb - 1) / cb, (M + 15) / 16)));
+                hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)cb, (unsigned)chunks), dim3(THREADS), 0, s, (const T *)dy, (const T *)a.pre, a.dcodes,
+                                   act, M, N, (M + chunks - 1) / chunks, dz, partial);
+                if (db) hipLaunchKernelGGL(db_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(THREADS), 0, s, partial, chunks, N, (T *)db);
+            }
+            if (act != AFIV_ACT_NONE) d.A = dz;
+            d.pre = nullptr;
+            d.dcodes = nullptr;
+            int rc = ok();
+            if (!rc && dx) rc = direct<T, false, true>(d, scratch, s);
+            if (!rc && dw) {
+                d.B = x;
+                if (codes) {
+                    rc = afiv_launch_checkpoint8_restore(codes, scales, std::is_same<T, __bf16>::value ? AFIV_BF16 : AFIV_F16, M, K, at + p.x, s);
+                    d.B = at + p.x;
+                }
+                d.R = N; d.C = K; d.L = M; d.out = dw;
+                if (!rc) rc = direct<T, true, true>(d, scratch, s);
+            }
+            return rc;
+        }
+    if (dx) {
+        const int rc = product<T, ALONG_DZ, ACROSS>(d, scratch, s);
+        if (rc) return rc;
+    }
+    if (dw || db) {
+        LinArgs e = a;
+        e.B = x; e.codes = codes; e.scales = scales;
+        e.R = N; e.C = K; e.L = M; e.out = dw; e.db = db;
+        return codes ? product<T, ACROSS_DZ, ACROSS_EIGHT>(e, scratch, s) : product<T, ACROSS_DZ, ACROSS>(e, scratch, s);
+    }
+    return AFIV_OK;
+}
+
+// ---- one translation unit per element type instantiates these ------------------------------------
+template <class T>
+int linear_forward(const void *x, const void *w, const void *bias, const void *residual, int act, int64_t M, int64_t N, int64_t K, void *y,
+                   void *pre, uint8_t *dcodes, float *scratch, hipStream_t s)
+{
+    LinArgs a = {};
+    a.A = x; a.B = w; a.R = M; a.C = N; a.L = K;
+    a.bias = bias; a.residual = residual; a.act_out = act; a.out = y; a.pre_out = pre; a.dcodes_out = dcodes;
+    return forward<T>(a, scratch, s);
+}
+
+}  // namespace
+
+#define AFIV_LINEAR_TYPE(T, NAME)                                                                                                      \
+    int afiv_linear_forward_##NAME(const void *x, const void *w, const void *bias, const void *residual, int act, int64_t M, int64_t N, \
+                                   int64_t K, void *y, void *pre, uint8_t *dcodes, float *scratch, hipStream_t s)                       \
+    {                                                                                                                                  \
+        return linear_forward<T>(x, w, bias, residual, act, M, N, K, y, pre, dcodes, scratch, s);                                      \
+    }                                                                                                                                  \
+    int afiv_linear_backward_##NAME(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w,           \
+                                    const void *pre, const uint8_t *dcodes, int act, int64_t M, int64_t N, int64_t K, void *dx,        \
+                                    void *dw, void *db, float *scratch, hipStream_t s)                                                 \
+    {                                                                                                                                  \
+        return backward<T>(dy, x, codes, scales, w, pre, dcodes, act, M, N, K, dx, dw, db, scratch, s);                                \
+    }

@@ -120,13 +120,22 @@ __device__ __forceinline__ void apply_rows(const NormArgs &p, const T *__restric
         Pack<uint8_t, V> k;
         if (p.keep && n > 0) k = load_some<uint8_t, V>(p.keep + at, n);
         Pack<T, V> out;
-        float f[V];
+        float f[V], z[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             f[i] = (float)v.v[i];
-            const float o = act_value((float)__builtin_fma((double)f[i] - mu[i], a[i], (double)beta[i]), p.act);
-            out.v[i] = (T)(p.keep ? (k.v[i] ? o * p.scale : 0.0f) : o);
+            z[i] = (float)__builtin_fma((double)f[i] - mu[i], a[i], (double)beta[i]);
         }
+        with_act(p.act, [&](auto act) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float o, d;
+                act_both<decltype(act)::value>(z[i], o, d);
+                z[i] = o;
+            }
+        });
+#pragma unroll
+        for (int i = 0; i < V; ++i) out.v[i] = (T)(p.keep ? (k.v[i] ? z[i] * p.scale : 0.0f) : z[i]);
         if (n > 0) store_some<T, V>(y + at, out, n);
         if (p.codes) {
             float amax = 0.0f;
@@ -295,7 +304,7 @@ __device__ __forceinline__ void g_and_h(const NormArgs &p, const T *__restrict__
     const Pack<T, V> d = load_some<T, V>(dy + at, n);
     Pack<uint8_t, V> m;
     if (p.keep) m = load_some<uint8_t, V>(p.keep + at, n);
-    float f[V];
+    float f[V], z[V];
     if (EIGHT) {
         const Pack<int8_t, V> q = load_some<int8_t, V>(p.codes + at, n);
         const int e = p.scales[r * nb + col / 32];
@@ -311,8 +320,20 @@ __device__ __forceinline__ void g_and_h(const NormArgs &p, const T *__restrict__
         const double hd = ((double)f[i] - k.mu[i]) * k.rstd[i];
         h[i] = (float)hd;
         g[i] = (float)d.v[i];
-        if (p.act != AFIV_ACT_NONE) g[i] *= act_derivative((float)__builtin_fma(hd, (double)k.gamma[i], (double)k.beta[i]), p.act);
-        if (p.keep) g[i] = m.v[i] ? g[i] * p.scale : 0.0f;
+        z[i] = (float)__builtin_fma(hd, (double)k.gamma[i], (double)k.beta[i]);
+    }
+    if (p.act != AFIV_ACT_NONE)
+        with_act(p.act, [&](auto act) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float f, d;
+                act_both<decltype(act)::value>(z[i], f, d);
+                g[i] *= d;
+            }
+        });
+    if (p.keep) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = m.v[i] ? g[i] * p.scale : 0.0f;
     }
 }
 

@@ -191,7 +191,7 @@ def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSav
     if g.device != ran_on:
         raise ValueError(f"dy is on {g.device}, the forward pass ran on {ran_on}")
     L = _lib.lib()
-    nbytes = L.afiv_linear_act_backward_scratch(m, n, k)
+    nbytes = L.afiv_linear_act_backward_scratch(m, n, k, DTYPES[g.dtype])
     with torch.cuda.device(g.device):
         scratch = _scratch(nbytes, g.device)
         rc = L.afiv_linear_act_backward(_ptr(g), _ptr(saved.x), _ptr(saved.eight.codes if saved.eight else None),

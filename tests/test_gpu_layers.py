@@ -122,7 +122,8 @@ def test_linear_forward_and_backward(afiv, typ, m, k, n):
 
 
 @pytest.mark.parametrize("typ,m,k,n", [("bf16", 2048, 1024, 2048), ("f16", 4096, 512, 1024), ("f32", 2048, 512, 2304), ("bf16", 2300, 1096, 2056),
-                                       ("bf16", 40000, 64, 72), ("f32", 40000, 24, 40)])
+                                       ("bf16", 40000, 64, 72), ("f32", 40000, 24, 40), ("bf16", 4104, 200, 4112), ("f16", 4104, 4120, 136),
+                                       ("bf16", 1000, 4096, 4200), ("f16", 136, 1288, 6008)])
 def test_linear_large_tiles(afiv, typ, m, k, n):
     x, w, b, r, dy = inputs(TYPES[typ], m, k, n, 5, residual=True)
     for act, eight in (("gelu", True), ("tanh", False)):
