@@ -60,7 +60,7 @@ SIGNATURES = {
     "afiv_ensemble_stats_groups": (c_int, [c_void_p, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_void_p]),
     "afiv_checkpoint8_pack": (c_int, [c_void_p, c_int, c_i64, c_i64, c_void_p, c_void_p, c_void_p]),
     "afiv_checkpoint8_restore": (c_int, [c_void_p, c_void_p, c_int, c_i64, c_i64, c_void_p, c_void_p]),
-    "afiv_linear_act_scratch": (c_i64, [c_i64, c_i64, c_i64]),
+    "afiv_linear_act_scratch": (c_i64, [c_i64, c_i64, c_i64, c_int]),
     "afiv_linear_act": (c_int, [c_void_p] * 4 + [c_int, c_int, c_i64, c_i64, c_i64] + [c_void_p] * 4 + [c_i64, c_void_p]),
     "afiv_linear_act_backward_scratch": (c_i64, [c_i64, c_i64, c_i64, c_int]),
     "afiv_linear_act_backward": (c_int, [c_void_p] * 7 + [c_int, c_int, c_i64, c_i64, c_i64] + [c_void_p] * 4 + [c_i64, c_void_p]),

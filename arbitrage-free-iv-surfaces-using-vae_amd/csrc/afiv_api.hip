@@ -691,9 +691,10 @@ static bool bad_linear(int64_t M, int64_t N, int64_t K)
     return bad_sizes(M, N) || bad_sizes(M, K) || bad_sizes(N, K);
 }
 
-int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K)
+int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K, int dtype)
 {
-    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_forward_scratch(M, N, K);
+    if (bad_layer(dtype, 0)) return AFIV_E_ARG;
+    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_forward_scratch(M, N, K, dtype);
 }
 
 int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype)
@@ -709,7 +710,7 @@ int afiv_linear_act(const void *x, const void *w, const void *bias, const void *
     if (bad_linear(M, N, K)) return AFIV_E_SHAPE;
     if (M == 0) return AFIV_OK;
     if (!x || !w || !y) return AFIV_E_NULL;
-    const int64_t need = afiv_linear_forward_scratch(M, N, K);
+    const int64_t need = afiv_linear_forward_scratch(M, N, K, dtype);
     if (need > 0 && (!scratch || scratch_bytes < need)) return AFIV_E_WORKSPACE;
     return afiv_launch_linear_act(x, w, bias, residual, dtype, act, M, N, K, y, pre_out, dcodes_out, (float *)scratch, as_stream(stream));
 }

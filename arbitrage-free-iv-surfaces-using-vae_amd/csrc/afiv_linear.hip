@@ -11,13 +11,8 @@ DECLARE(f32)
 DECLARE(bf16)
 DECLARE(f16)
 
-int64_t afiv_linear_forward_scratch(int64_t M, int64_t N, int64_t K) { return M <= FEW ? 0 : scratch_floats(M, N, K) * 4; }
-
-int64_t afiv_linear_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype)
-{
-    const Places p = places(M, N, K);
-    return dtype == AFIV_F32 ? p.dz : p.bytes;
-}
+int64_t afiv_linear_forward_scratch(int64_t M, int64_t N, int64_t K, int dtype) { return forward_places(M, N, K, dtype == AFIV_F32).bytes; }
+int64_t afiv_linear_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype) { return backward_places(M, N, K, dtype == AFIV_F32).bytes; }
 
 int afiv_launch_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
                            int64_t K, void *y, void *pre, uint8_t *dcodes, float *scratch, hipStream_t s)

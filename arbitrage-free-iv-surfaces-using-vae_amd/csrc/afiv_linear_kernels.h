@@ -390,6 +390,32 @@ __device__ __forceinline__ void place_tile(const LinArgs &a, int br, int bc, int
     tc = in / rows_here;
 }
 
+// sums over l for a tile's outputs one by one, in FP32: for operands that do not split into parts
+template <class T, Kind KA, Kind KB, int TR, int TC>
+__device__ __forceinline__ void plain_sums(const LinArgs &a, f32x4 (&acc)[TR][TC], int64_t row0, int64_t col0, int64_t l_begin, int64_t l_end,
+                                           int lane)
+{
+#pragma unroll 1
+    for (int i = 0; i < TR; ++i)
+#pragma unroll 1
+        for (int j = 0; j < TC; ++j)
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+                const int64_t row = row0 + 16 * i + (lane & 15), col = col0 + 16 * j + (lane >> 4) * 4 + q;
+                float s = 0.0f;
+                if (row < a.R && col < a.C)
+                    for (int64_t l = l_begin; l < l_end; ++l)
+                        s = __builtin_fmaf(element<T, KA>(a, a.A, a.R, row, l), element<T, KB>(a, a.B, a.C, col, l), s);
+#pragma unroll
+                for (int ii = 0; ii < TR; ++ii)
+#pragma unroll
+                    for (int jj = 0; jj < TC; ++jj)
+#pragma unroll
+                        for (int qq = 0; qq < 4; ++qq)
+                            if (ii == i && jj == j && qq == q) acc[ii][jj][qq] = s;
+            }
+}
+
 // Tile of 32 TR x 32 TC outputs, four waves of 16 TR x 16 TC.  The matrix instruction gets B as its
 // first operand: a lane then holds four neighbouring columns of one row of C.
 template <class T, Kind KA, Kind KB, int TR, int TC>
@@ -451,27 +477,8 @@ __global__ __launch_bounds__(THREADS) void tile_kernel(LinArgs a)
     }
 
     if constexpr (PARTS == 3) {
-        if (__syncthreads_or(!(amax < 0x1p127f))) {
-#pragma unroll 1
-            for (int i = 0; i < TR; ++i)
-#pragma unroll 1
-                for (int j = 0; j < TC; ++j)
-#pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {
-                        const int64_t row = row0 + wr + 16 * i + (lane & 15), col = col0 + wc + 16 * j + (lane >> 4) * 4 + q;
-                        float s = 0.0f;
-                        if (row < a.R && col < a.C)
-                            for (int64_t l = l_begin; l < l_end; ++l)
-                                s = __builtin_fmaf(element<T, KA>(a, a.A, a.R, row, l), element<T, KB>(a, a.B, a.C, col, l), s);
-#pragma unroll
-                        for (int ii = 0; ii < TR; ++ii)
-#pragma unroll
-                            for (int jj = 0; jj < TC; ++jj)
-#pragma unroll
-                                for (int qq = 0; qq < 4; ++qq)
-                                    if (ii == i && jj == j && qq == q) acc[ii][jj][qq] = s;
-                    }
-        }
+        if (__syncthreads_or(!(amax < 0x1p127f)))
+            plain_sums<T, KA, KB, TR, TC>(a, acc, row0 + wr, col0 + wc, l_begin, l_end, lane);
     }
 
     if (want_sums) {                       // the same for the whole workgroup
@@ -526,48 +533,55 @@ __global__ __launch_bounds__(THREADS) void join_kernel(LinArgs a)
         }
 }
 
-// ---- large products of 16-bit operands ---------------------------------------------------------
-// The same product for operands that can go from memory to LDS as they are (16-bit types, rows of a
-// multiple of 16 bytes, no dz, no checkpoint).  Steps of 64: a tile's rows are 128 bytes (along l) or
-// its 64 steps of l are rows of 2 BR bytes (across), and lie in LDS as the loads leave them, 1024 consecutive
-// bytes an instruction; what keeps the reads off each other's banks is therefore a permutation of the
-// global addresses: 16-byte chunk c of row r stands at c ^ (r & 7), 32-byte block c of step l at
-// c ^ key(l).  Operands across l are transposed by the LDS read itself (ds_read_b64_tr_b16).
+// ---- large products -------------------------------------------------------------------------------
+// The same product from operands that go from memory to LDS as they are: 16-bit elements, rows of whole
+// 16-byte chunks.  Operands of that kind are read where they stand; others are written so first, by
+// prepare_kernel: rows of another length, dz, an 8-bit x, and FP32 as its three BF16 parts (a plane each; a
+// fragment of each part is then read once for the six products).
+// Steps of 64 (FP32: 32): a tile's rows are 128 (64) bytes along l, or its steps of l are rows of 2 BR bytes
+// (across), and lie in LDS as the loads leave them, 1024 consecutive bytes an instruction; what keeps the
+// reads off each other's banks is therefore a permutation of the global addresses: 16-byte chunk c of row r stands
+// at c ^ (r & 7) (64-byte rows: c ^ ((r >> 1) & 3)), 32-byte block c of step l at c ^ key(l).  Operands across l are
+// transposed by the LDS read itself (ds_read_b64_tr_b16).
 // Two buffers; one barrier a step: the loads of the next step run behind this one's products.
 __device__ __forceinline__ int across_key(int l) { return (l & 3) | ((l >> 1) & 4); }
 
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
-template <class T, bool XS, int ROWS, int WAVES, int TN>
+// P: 16-bit element, FK: steps of l, ROWS: rows of the tile, TN: blocks of 16 rows of a wave
+template <class P, bool XS, int FK, int ROWS, int WAVES, int TN>
 struct Direct {
-    typedef typename Mma<T>::frag frag;
-    static constexpr int PER = ROWS * FK * 2 / 1024 / WAVES;      // loads of a wave
-    static_assert(PER * WAVES * 1024 == ROWS * FK * 2, "whole loads");
+    typedef typename Mma<P>::frag frag;
+    static constexpr int BYTES = ROWS * FK * 2, PER = BYTES / 1024 / WAVES;      // loads of a wave
+    static_assert(PER * WAVES * 1024 == BYTES, "whole loads");
     static constexpr int LSTEP = XS ? 1024 / (2 * ROWS) : 0;      // steps of l from one load of a wave to the next
     static constexpr int BASES = XS ? TN : FK / 32;
     uint32_t off[PER];                    // byte offset from the tile's corner; beyond the matrix: out of range
     uint32_t l_first;                     // step of l of the first load
     uint32_t at[BASES];                   // where a lane's reads start
 
-    // w0: first of the wave's 16 TN rows (a multiple of 8 blocks of 16, or of TN of them)
-    __device__ __forceinline__ void init(int64_t R, int64_t L, int64_t row0, int w0, int wave, int lane)
+    static __device__ __forceinline__ int chunk_key(int r) { return FK == 64 ? r & 7 : (r >> 1) & 3; }
+
+    // w0: first of the wave's 16 TN rows
+    __device__ __forceinline__ void init(int64_t R, int64_t ld, int64_t row0, int w0, int wave, int lane)
     {
+        constexpr int ROWB = FK * 2, CH = ROWB / 16;              // bytes and chunks of a row along l
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int byte = (wave * PER + i) * 1024 + lane * 16;
             if (!XS) {
-                const int r = byte / 128, c = (lane & 7) ^ (lane >> 3);
-                off[i] = row0 + r < R ? (uint32_t)(r * L * 2 + c * 16) : 0x80000000u;
+                const int r = byte / ROWB, c = (lane & (CH - 1)) ^ chunk_key(lane / CH);
+                off[i] = row0 + r < R ? (uint32_t)(r * ld * 2 + c * 16) : 0x80000000u;
             } else {
                 const int l = byte / (2 * ROWS), pos = byte % (2 * ROWS) / 16;
                 const int col = ((pos >> 1) ^ across_key(l)) * 16 + (pos & 1) * 8;
-                off[i] = row0 + col < R ? (uint32_t)((l * R + col) * 2) : 0x80000000u;
+                off[i] = row0 + col < R ? (uint32_t)((l * ld + col) * 2) : 0x80000000u;
             }
         }
         if (!XS) {
-            l_first = ((lane & 7) ^ (lane >> 3)) * 8;
+            l_first = ((lane & (CH - 1)) ^ chunk_key(lane / CH)) * 8;
 #pragma unroll
-            for (int kk = 0; kk < FK / 32; ++kk) at[kk] = (w0 + (lane & 15)) * 128 + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
+            for (int kk = 0; kk < FK / 32; ++kk) at[kk] = (w0 + (lane & 15)) * ROWB + (((kk * 4 + (lane >> 4)) ^ chunk_key(lane & 15)) << 4);
         } else {
             l_first = (wave * PER * 1024 + lane * 16) / (2 * ROWS);
             // 16 lanes read 4 steps x 16 rows, 8 bytes each, and get 4 steps of a row each
@@ -576,10 +590,10 @@ struct Direct {
             for (int i = 0; i < TN; ++i) at[i] = l * (2 * ROWS) + ((((w0 >> 4) + i) ^ across_key(l)) << 5) + (lane & 3) * 8;
         }
     }
-    __device__ __forceinline__ void load(const T *base, int64_t R, int64_t L, int64_t row0, int64_t l0, int64_t l_end, char *lds, int wave) const
+    __device__ __forceinline__ void load(const P *base, int64_t ld, int64_t row0, int64_t l0, int64_t l_end, char *lds, int wave) const
     {
 #if defined(__HIP_DEVICE_COMPILE__)             // buffer resources have no host type
-        const T *corner = base + (XS ? l0 * R + row0 : row0 * L + l0);
+        const P *corner = base + (XS ? l0 * ld + row0 : row0 * ld + l0);
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)corner, 0, 0x7fffffff, 0x00020000);
         const int left = (int)(l_end - l0 < FK ? l_end - l0 : FK);
 #pragma unroll
@@ -592,7 +606,7 @@ struct Direct {
     __device__ __forceinline__ frag read(const char *lds, int i, int kk) const
     {
         frag f;
-        if constexpr (!XS) f = *(const frag *)(lds + at[kk] + i * 2048);
+        if constexpr (!XS) f = *(const frag *)(lds + at[kk] + i * (32 * FK));
         else {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             s16x4 h[2];
@@ -605,45 +619,82 @@ struct Direct {
     }
 };
 
-// WR x WC waves of 16 TR x 16 TC outputs
-template <class T, bool XA, bool XB, int WR, int WC, int TR, int TC>
-__global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a)
+// what the direct kernel reads of an operand
+struct Source {
+    const void *p;                        // 16-bit elements, plane after plane
+    int64_t ld, plane;                    // elements from row to row (of l across), and from plane to plane
+    // FP32: words [chunks, blocks]: whether rows_per rows by 512 columns hold values that do not split
+    const uint32_t *flags;
+    int64_t rows_per, chunks, blocks;
+};
+
+// whether a tile of `rows` rows from row0 on has such values in its operand
+template <bool XS>
+__device__ __forceinline__ bool unsplittable(const Source &s, int64_t row0, int rows)
 {
-    constexpr int W = WR * WC, BR = 16 * TR * WR, BC = 16 * TC * WC;
+    const int64_t first = row0 / (XS ? 512 : s.rows_per), most = XS ? s.blocks : s.chunks;
+    const int64_t end = std::min<int64_t>(most, (row0 + rows - 1) / (XS ? 512 : s.rows_per) + 1), other = XS ? s.chunks : s.blocks;
+    uint32_t any = 0;
+    for (int64_t i = threadIdx.x; i < (end - first) * other; i += blockDim.x) {
+        const int64_t a = first + i / other, b = i % other;
+        any |= XS ? s.flags[b * s.blocks + a] : s.flags[a * s.blocks + b];
+    }
+    return any != 0;
+}
+
+// WR x WC waves of 16 TR x 16 TC outputs.  `a` describes the operands as they came, sa and sb as they are read.
+template <class T, Kind KA, Kind KB, int FK, int WR, int WC, int TR, int TC>
+__global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source sa, Source sb)
+{
+    constexpr int W = WR * WC, BR = 16 * TR * WR, BC = 16 * TC * WC, PARTS = Mma<T>::PARTS;
+    constexpr bool EPI = KA == ALONG && KB == ALONG;
+    typedef typename Part<T>::type P;
     typedef typename Mma<T>::frag frag;
-    constexpr int STAGE = (BR + BC) * FK * 2;
+    typedef Direct<P, across(KA), FK, BR, W, TR> DA;
+    typedef Direct<P, across(KB), FK, BC, W, TC> DB;
+    constexpr int STAGE = PARTS * (DA::BYTES + DB::BYTES);
     __shared__ __align__(1024) char lds[2 * STAGE];
-    constexpr int ROOM = 2 * STAGE / W / 4, SLABS = ROOM / (16 * 16 * TC) < TR ? ROOM / (16 * 16 * TC) : TR;   // floats a wave
+    constexpr int SLAB = 16 * 16 * TC, FIT = 2 * STAGE / W / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = (wave % WR) * 16 * TR, wc = (wave / WR) * 16 * TC;
     int64_t split, tr, tc;
     place_tile(a, BR, BC, split, tr, tc);
     const int64_t row0 = tr * BR, col0 = tc * BC;
     const int64_t l_begin = split * a.l_per, l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
-    Direct<T, XA, BR, W, TR> da;
-    Direct<T, XB, BC, W, TC> db;
-    da.init(a.R, a.L, row0, wr, wave, lane);
-    db.init(a.C, a.L, col0, wc, wave, lane);
+    DA da;
+    DB db;
+    da.init(a.R, sa.ld, row0, wr, wave, lane);
+    db.init(a.C, sb.ld, col0, wc, wave, lane);
     f32x4 acc[TR][TC] = {};
 
     auto load = [&](char *s, int64_t l0) {
         if (l0 < l_end) {
-            da.load((const T *)a.A, a.R, a.L, row0, l0, l_end, s, wave);
-            db.load((const T *)a.B, a.C, a.L, col0, l0, l_end, s + BR * FK * 2, wave);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                da.load((const P *)sa.p + p * sa.plane, sa.ld, row0, l0, l_end, s + p * DA::BYTES, wave);
+                db.load((const P *)sb.p + p * sb.plane, sb.ld, col0, l0, l_end, s + PARTS * DA::BYTES + p * DB::BYTES, wave);
+            }
         }
     };
     auto multiply = [&](const char *s) {
 #pragma unroll
         for (int kk = 0; kk < FK / 32; ++kk) {
-            frag fa[TR], fb[TC];
+            frag fa[PARTS][TR], fb[PARTS][TC];
 #pragma unroll
-            for (int j = 0; j < TC; ++j) fb[j] = db.read(s + BR * FK * 2, j, kk);
+            for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
-            for (int i = 0; i < TR; ++i) fa[i] = da.read(s, i, kk);
+                for (int j = 0; j < TC; ++j) fb[p][j] = db.read(s + PARTS * DA::BYTES + p * DB::BYTES, j, kk);
 #pragma unroll
-            for (int i = 0; i < TR; ++i)
+                for (int i = 0; i < TR; ++i) fa[p][i] = da.read(s + p * DA::BYTES, i, kk);
+            }
 #pragma unroll
-                for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
+            for (int p = PARTS - 1; p >= 0; --p)                  // small products first
+#pragma unroll
+                for (int q = 0; q <= p; ++q)
+#pragma unroll
+                    for (int i = 0; i < TR; ++i)
+#pragma unroll
+                        for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[q][j], fa[p - q][i], acc[i][j]);
         }
     };
     // every load of this wave has arrived (vmcnt 0) before any wave reads the tile, and every read of the
@@ -661,62 +712,130 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a)
         multiply(lds + here);
         here = STAGE - here;
     }
+    if constexpr (PARTS == 3) {
+        if (__syncthreads_or(unsplittable<across(KA)>(sa, row0, BR) || unsplittable<across(KB)>(sb, col0, BC)))
+            plain_sums<T, KA, KB, TR, TC>(a, acc, row0 + wr, col0 + wc, l_begin, l_end, lane);
+    }
     __syncthreads();
-    write_out<T, !XA && !XB, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)lds + wave * ROOM);
+    write_out<T, EPI, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)lds + wave * SLABS * SLAB);
 }
 
-// dz = dy f'(z) for the direct products, and the partial sums of db: rows_per rows a workgroup of 64 lanes
-// (8 columns each) by 4 rows.  dz may be NULL (no activation: db alone).
-template <class T>
-__global__ __launch_bounds__(THREADS) void dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, const uint8_t *__restrict__ dcodes, int act,
-                                                     int64_t M, int64_t N, int64_t rows_per, T *__restrict__ dz, float *__restrict__ partial)
+// An operand for the direct kernel, [rows, cols] -> [rows, ldp] of 16-bit elements (FP32: three planes of BF16 parts),
+// zeros behind cols.  src: x itself, dy with z or its derivative codes (dz = dy f'(z); with `partial`, also the
+// partial column sums of dz in FP32), or an 8-bit checkpoint.  rows_per rows a workgroup of 64 lanes (8 columns each) by 4
+// rows.  out may be NULL (db alone).  FP32: flags[workgroup] = whether it met a magnitude of 2^127 or more.
+enum Made { COPY, DZ, EIGHT };
+struct PrepArgs {
+    const void *src, *pre;
+    const uint8_t *dcodes;
+    const int8_t *codes;
+    const uint8_t *scales;
+    int act;
+    int64_t rows, cols, ldp, rows_per, plane;
+    void *out;
+    float *partial;
+    uint32_t *flags;
+};
+
+template <class T, Made MADE>
+__global__ __launch_bounds__(THREADS) void prepare_kernel(PrepArgs a)
 {
-    __shared__ float lds[4][512];
+    typedef typename Part<T>::type P;
+    constexpr int PARTS = Mma<T>::PARTS;
+    __shared__ float lds[MADE == DZ ? 4 : 1][512];
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const int64_t col = ((int64_t)blockIdx.x * 64 + tx) * 8;
-    const int n = (int)(N - col < 8 ? N - col : 8);
-    const int64_t r0 = (int64_t)blockIdx.y * rows_per, r1 = r0 + rows_per < M ? r0 + rows_per : M;
-    float sum[8] = {};
-    if (n > 0)
-        with_act(act, [&](auto actc) {
-            constexpr int ACT = decltype(actc)::value;
-#pragma unroll 2
-            for (int64_t r = r0 + ty; r < r1; r += 4) {
-                const int64_t at = r * N + col;
-                const Pack<T, 8> v = load_some<T, 8>(dy + at, n);
-                float f[8];
-                if constexpr (ACT == AFIV_ACT_NONE) {
+    const int n = (int)(a.cols - col < 8 ? a.cols - col : 8);
+    const int64_t r0 = (int64_t)blockIdx.y * a.rows_per, r1 = r0 + a.rows_per < a.rows ? r0 + a.rows_per : a.rows;
+    float sum[8] = {}, amax = 0.0f;
+    auto rows = [&](auto full, auto act) {
+        constexpr bool FULL = decltype(full)::value;
+        constexpr int ACT = decltype(act)::value, U = FULL ? 4 : 1;
+        const int64_t nb = (a.cols + 31) / 32;
+        // U rows' loads together, the last ones again where fewer are left
+        for (int64_t r = r0 + ty; r < r1; r += 4 * U) {
+            Pack<T, 8> v[U], z[MADE == DZ ? U : 1];
+            Pack<uint8_t, 8> c[MADE == DZ ? U : 1];
+            Pack<int8_t, 8> q[MADE == EIGHT ? U : 1];
+            int e[MADE == EIGHT ? U : 1];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = (float)v.v[i];
-                } else if (pre) {
-                    const Pack<T, 8> z = load_some<T, 8>(pre + at, n);
+            for (int u = 0; u < U; ++u) {
+                const int64_t row = r + 4 * u < r1 ? r + 4 * u : r, at = row * a.cols + col;
+                if constexpr (MADE == EIGHT) {
+                    q[u] = FULL ? load_pack<int8_t, 8>(a.codes + at) : load_some<int8_t, 8>(a.codes + at, n);
+                    e[u] = a.scales[row * nb + col / 32];
+                } else v[u] = FULL ? load_pack<T, 8>((const T *)a.src + at) : load_some<T, 8>((const T *)a.src + at, n);
+            }
+            if constexpr (MADE == DZ && ACT != AFIV_ACT_NONE) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float y, d;
-                        act_both<ACT>((float)z.v[i], y, d);
-                        f[i] = (float)v.v[i] * d;
-                    }
-                } else {
-                    const Pack<uint8_t, 8> c = load_some<uint8_t, 8>(dcodes + at, n);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = (float)v.v[i] * derivative_of_code<ACT>(c.v[i]);
+                for (int u = 0; u < U; ++u) {
+                    const int64_t row = r + 4 * u < r1 ? r + 4 * u : r, at = row * a.cols + col;
+                    if (a.pre) z[u] = FULL ? load_pack<T, 8>((const T *)a.pre + at) : load_some<T, 8>((const T *)a.pre + at, n);
+                    else c[u] = FULL ? load_pack<uint8_t, 8>(a.dcodes + at) : load_some<uint8_t, 8>(a.dcodes + at, n);
                 }
-                Pack<T, 8> o;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (u > 0 && r + 4 * u >= r1) break;
+                float f[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    sum[i] += f[i];
-                    o.v[i] = (T)f[i];
+                    if constexpr (MADE == EIGHT) f[i] = eight_value(q[u].v[i], e[u]);
+                    else f[i] = (float)v[u].v[i];
+                    if constexpr (MADE == DZ && ACT != AFIV_ACT_NONE) {
+                        float y, d;
+                        if (a.pre) act_both<ACT>((float)z[u].v[i], y, d);
+                        else d = derivative_of_code<ACT>(c[u].v[i]);
+                        f[i] *= d;
+                    }
+                    if (!FULL && i >= n) f[i] = 0.0f;
+                    if constexpr (MADE == DZ) sum[i] += f[i];
+                    if constexpr (PARTS == 3) amax = fmaxf(amax, fabsf(f[i]));        // NaN splits into NaNs
                 }
-                if (ACT != AFIV_ACT_NONE && dz) store_some<T, 8>(dz + at, o, n);
-            }
-        });
-    if (!partial) return;
+                if (MADE == DZ && !a.out) continue;
+                P *o = (P *)a.out + (r + 4 * u) * a.ldp + col;
+                if constexpr (PARTS == 3) {
+                    float w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lds[ty][tx * 8 + i] = sum[i];
-    __syncthreads();
-    for (int c = threadIdx.x; c < 512; c += THREADS)
-        if ((int64_t)blockIdx.x * 512 + c < N)
-            partial[(int64_t)blockIdx.y * N + (int64_t)blockIdx.x * 512 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
+                    for (int i = 0; i < 8; ++i) w[i] = f[i];
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        Pack<P, 8> b;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            b.v[i] = (P)w[i];
+                            w[i] -= (float)b.v[i];
+                        }
+                        store_pack<P, 8>(o + p * a.plane, b);
+                    }
+                } else {
+                    Pack<P, 8> b;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b.v[i] = (P)f[i];
+                    store_pack<P, 8>(o, b);
+                }
+            }
+        }
+    };
+    auto with = [&](auto act) {
+        if (n >= 8) rows(std::true_type(), act);
+        else if (n > 0) rows(std::false_type(), act);
+    };
+    if constexpr (MADE == DZ) with_act(a.act, with);
+    else with(std::integral_constant<int, AFIV_ACT_NONE>());
+    if constexpr (PARTS == 3) {
+        const int any = __syncthreads_or(!(amax < 0x1p127f));
+        if (threadIdx.x == 0 && a.flags) a.flags[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = any;
+    }
+    if constexpr (MADE == DZ) {
+        if (!a.partial) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lds[ty][tx * 8 + i] = sum[i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < 512; c += THREADS)
+            if ((int64_t)blockIdx.x * 512 + c < a.cols)
+                a.partial[(int64_t)blockIdx.y * a.cols + (int64_t)blockIdx.x * 512 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
+    }
 }
 
 // db from the partial sums: 16 columns a workgroup, 16 threads each over the chunks
@@ -806,18 +925,51 @@ int product(LinArgs a, float *scratch, hipStream_t s)
     return ok();
 }
 
-template <class T, bool XA, bool XB>
-int direct(LinArgs a, float *scratch, hipStream_t s)
+template <class T, Kind KA, Kind KB>
+int direct(LinArgs a, const Source &sa, const Source &sb, float *scratch, hipStream_t s)
 {
-    const Plan p = direct_plan(a.R, a.C, a.L);
+    const Plan p = direct_plan(a.R, a.C, a.L, sizeof(T) == 4);
     a.splits = p.splits;
     a.l_per = p.l_per;
     a.partial = scratch;
+    a.db = nullptr;
     const dim3 grid((unsigned)(p.tiles * p.splits));
-    if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, XA, XB, 2, 4, 8, 4>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((direct_kernel<T, XA, XB, 2, 2, 4, 4>), grid, dim3(256), 0, s, a);
-    if (p.splits > 1) join<T, !XA && !XB>(a, s);
+    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 32, 2, 4, 4, 2>), grid, dim3(512), 0, s, a, sa, sb);
+    else if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 64, 2, 4, 8, 4>), grid, dim3(512), 0, s, a, sa, sb);
+    else hipLaunchKernelGGL((direct_kernel<T, KA, KB, 64, 2, 2, 4, 4>), grid, dim3(256), 0, s, a, sa, sb);
+    if (p.splits > 1) join<T, KA == ALONG && KB == ALONG>(a, s);
     return ok();
+}
+
+// writes an operand to `room`, and says how the direct kernel reads it
+template <class T, Made MADE>
+Source prepared(PrepArgs a, const Room &room, char *scratch, float *partial, bool write, hipStream_t s)
+{
+    const int64_t cb = (a.cols + 511) / 512, chunks = prep_chunks(a.rows, a.cols);
+    a.ldp = padded(a.cols);
+    a.plane = a.rows * a.ldp;
+    a.rows_per = (a.rows + chunks - 1) / chunks;
+    a.out = write ? scratch + room.at : nullptr;
+    a.partial = partial;
+    a.flags = sizeof(T) == 4 ? (uint32_t *)(scratch + room.flags) : nullptr;
+    hipLaunchKernelGGL((prepare_kernel<T, MADE>), dim3((unsigned)cb, (unsigned)chunks), dim3(THREADS), 0, s, a);
+    const Source o = {a.out, a.ldp, a.plane, a.flags, a.rows_per, chunks, cb};
+    return o;
+}
+
+// an operand that may be read where it stands
+Source standing(const void *p, int64_t ld)
+{
+    const Source o = {p, ld, 0, nullptr, 1, 0, 0};
+    return o;
+}
+template <class T>
+Source plain_source(const void *p, int64_t rows, int64_t cols, const Room &room, char *scratch, hipStream_t s)
+{
+    if (!room.bytes) return standing(p, cols);
+    PrepArgs q = {};
+    q.src = p; q.rows = rows; q.cols = cols;
+    return prepared<T, COPY>(q, room, scratch, nullptr, true, s);
 }
 
 template <class T>
@@ -830,8 +982,12 @@ int forward(const LinArgs &a, float *scratch, hipStream_t s)
         else hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, dim3(256), 0, s, a);
         return ok();
     }
-    if constexpr (sizeof(T) == 2)
-        if (direct_rows(a.L) && direct_pays(a.R, a.C, a.L) && aligned(a.A) && aligned(a.B)) return direct<T, false, false>(a, scratch, s);
+    const Places p = forward_places(a.R, a.C, a.L, sizeof(T) == 4);
+    if (p.direct && (p.x.bytes || aligned(a.A)) && (p.w.bytes || aligned(a.B)) && aligned(scratch)) {
+        char *at = (char *)scratch;
+        const Source x = plain_source<T>(a.A, a.R, a.L, p.x, at, s), w = plain_source<T>(a.B, a.C, a.L, p.w, at, s);
+        return direct<T, ALONG, ALONG>(a, x, w, scratch, s);
+    }
     return product<T, ALONG, ALONG>(a, scratch, s);
 }
 
@@ -839,49 +995,50 @@ template <class T>
 int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w, const void *pre,
              const uint8_t *dcodes, int act, int64_t M, int64_t N, int64_t K, void *dx, void *dw, void *db, float *scratch, hipStream_t s)
 {
+    if (act == AFIV_ACT_NONE) {
+        pre = nullptr;
+        dcodes = nullptr;
+    }
     LinArgs a = {};
-    a.A = dy; a.act = act;
-    if (act != AFIV_ACT_NONE) { a.pre = pre; a.dcodes = dcodes; }
-    LinArgs d = a;
+    a.A = dy; a.act = act; a.pre = pre; a.dcodes = dcodes;
+    LinArgs d = a, e = a;
     d.B = w; d.R = M; d.C = K; d.L = N; d.out = dx;
-    if constexpr (sizeof(T) == 2)
-        if (direct_backward(M, N, K) && aligned(dy) && aligned(w) && aligned(x) && aligned(scratch)) {
-            const Places p = places(M, N, K);
-            char *at = (char *)scratch;
-            T *dz = (T *)(at + p.dz);
-            float *partial = db ? (float *)(at + p.db) : nullptr;
-            if (act != AFIV_ACT_NONE || db) {
-                const int64_t cb = (N + 511) / 512, chunks = std::min(DB_CHUNKS, std::max<int64_t>(1, std::min((2048 + cb - 1) / cb, (M + 15) / 16)));
-                hipLaunchKernelGGL(dz_kernel<T>, dim3((unsigned)cb, (unsigned)chunks), dim3(THREADS), 0, s, (const T *)dy, (const T *)a.pre, a.dcodes,
-                                   act, M, N, (M + chunks - 1) / chunks, dz, partial);
-                if (db) hipLaunchKernelGGL(db_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(THREADS), 0, s, partial, chunks, N, (T *)db);
-            }
-            if (act != AFIV_ACT_NONE) d.A = dz;
-            d.pre = nullptr;
-            d.dcodes = nullptr;
-            int rc = ok();
-            if (!rc && dx) rc = direct<T, false, true>(d, scratch, s);
-            if (!rc && dw) {
-                d.B = x;
-                if (codes) {
-                    rc = afiv_launch_checkpoint8_restore(codes, scales, std::is_same<T, __bf16>::value ? AFIV_BF16 : AFIV_F16, M, K, at + p.x, s);
-                    d.B = at + p.x;
-                }
-                d.R = N; d.C = K; d.L = M; d.out = dw;
-                if (!rc) rc = direct<T, true, true>(d, scratch, s);
-            }
-            return rc;
+    e.B = x; e.codes = codes; e.scales = scales; e.R = N; e.C = K; e.L = M; e.out = dw; e.db = db;
+
+    const Places p = backward_places(M, N, K, sizeof(T) == 4);
+    const bool make_dz = p.dz.bytes && (sizeof(T) == 4 || act != AFIV_ACT_NONE || N % 8);
+    if (p.direct && (make_dz || aligned(dy)) && (p.w.bytes || aligned(w)) && (codes || (sizeof(T) == 4 || K % 8) || aligned(x)) && aligned(scratch)) {
+        char *at = (char *)scratch;
+        float *partial = db ? (float *)(at + p.db) : nullptr;
+        Source g = standing(dy, N);
+        if (make_dz || db) {
+            PrepArgs q = {};
+            q.src = dy; q.pre = pre; q.dcodes = dcodes; q.act = act; q.rows = M; q.cols = N;
+            const Source made = prepared<T, DZ>(q, p.dz, at, partial, make_dz, s);
+            if (make_dz) g = made;
+            if (db) hipLaunchKernelGGL(db_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(THREADS), 0, s, partial, prep_chunks(M, N), N, (T *)db);
         }
+        int rc = ok();
+        if (!rc && dx) rc = direct<T, ALONG_DZ, ACROSS>(d, g, plain_source<T>(w, N, K, p.w, at, s), scratch, s);
+        if (!rc && dw) {
+            if (codes) {
+                PrepArgs q = {};
+                q.codes = codes; q.scales = scales; q.rows = M; q.cols = K;
+                const Source xs = prepared<T, EIGHT>(q, p.x, at, nullptr, true, s);
+                if constexpr (sizeof(T) == 4) rc = direct<T, ACROSS_DZ, ACROSS_EIGHT>(e, g, xs, scratch, s);
+                else rc = direct<T, ACROSS_DZ, ACROSS>(e, g, xs, scratch, s);
+            } else {
+                const Room none = {};
+                rc = direct<T, ACROSS_DZ, ACROSS>(e, g, plain_source<T>(x, M, K, sizeof(T) == 4 || K % 8 ? p.x : none, at, s), scratch, s);
+            }
+        }
+        return rc;
+    }
     if (dx) {
         const int rc = product<T, ALONG_DZ, ACROSS>(d, scratch, s);
         if (rc) return rc;
     }
-    if (dw || db) {
-        LinArgs e = a;
-        e.B = x; e.codes = codes; e.scales = scales;
-        e.R = N; e.C = K; e.L = M; e.out = dw; e.db = db;
-        return codes ? product<T, ACROSS_DZ, ACROSS_EIGHT>(e, scratch, s) : product<T, ACROSS_DZ, ACROSS>(e, scratch, s);
-    }
+    if (dw || db) return codes ? product<T, ACROSS_DZ, ACROSS_EIGHT>(e, scratch, s) : product<T, ACROSS_DZ, ACROSS>(e, scratch, s);
     return AFIV_OK;
 }
 

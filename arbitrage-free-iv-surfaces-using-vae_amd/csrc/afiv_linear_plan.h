@@ -10,7 +10,6 @@
 namespace {
 
 constexpr int BK = 32;                    // steps of l in LDS, tile kernel
-constexpr int FK = 64;                    // and direct kernel
 constexpr int FEW = 16;                   // rows of the few-rows kernel
 
 int64_t tiles_of(int64_t R, int64_t C, int64_t t) { return ((R + t - 1) / t) * ((C + t - 1) / t); }
@@ -33,44 +32,76 @@ Plan cut(int64_t tiles, int64_t L, int64_t step, int64_t want, int64_t least)
 bool big_tiles(int64_t R, int64_t C) { return tiles_of(R, C, 128) >= 256; }
 Plan plan_for(int64_t R, int64_t C, int64_t L) { return cut(tiles_of(R, C, big_tiles(R, C) ? 128 : 64), L, BK, 512, 8); }
 
-// The direct kernel: 256 x 256 tiles where they fill the chip at least once, else 128 x 128 (cut like the above).
+// The direct kernel: 256 x 256 tiles where they fill the chip at least once, else 128 x 128 (FP32: always), cut
+// like the above.
 bool huge_tiles(int64_t R, int64_t C) { return tiles_of(R, C, 256) >= 256; }
-Plan direct_plan(int64_t R, int64_t C, int64_t L)
+Plan direct_plan(int64_t R, int64_t C, int64_t L, bool f32)
 {
-    return huge_tiles(R, C) ? cut(tiles_of(R, C, 256), L, FK, 0, 1) : cut(tiles_of(R, C, 128), L, FK, 512, 8);
+    if (f32) return cut(tiles_of(R, C, 128), L, 32, 512, 8);
+    return huge_tiles(R, C) ? cut(tiles_of(R, C, 256), L, 64, 0, 1) : cut(tiles_of(R, C, 128), L, 64, 512, 8);
 }
 
-// what the direct kernel takes: rows of whole 16-byte chunks within 2^31 bytes of a tile's corner, and enough
-// work that its tiles are not mostly padding
-bool direct_rows(int64_t len) { return len % 8 == 0 && len <= (1 << 21); }
-bool direct_pays(int64_t R, int64_t C, int64_t L) { return R >= 128 && C >= 128 && L >= 128 && R * C >= 128 * 128 * 32; }
+// what the direct kernel takes: rows within 2^31 bytes of a tile's corner, and enough work that its tiles are not
+// mostly padding and the operands' preparation is paid back
+bool direct_takes(int64_t R, int64_t C, int64_t L)
+{
+    return R >= 128 && C >= 128 && L >= 128 && R * C >= 128 * 128 * 32 && std::max(std::max(R, C), L) <= (int64_t)1 << 36;
+}
+bool direct_rows(int64_t len) { return len <= 1 << 21; }
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // floats that either kernel's split takes
-int64_t scratch_floats(int64_t R, int64_t C, int64_t L)
+int64_t scratch_floats(int64_t R, int64_t C, int64_t L, bool f32)
 {
-    const Plan p = plan_for(R, C, L), d = direct_plan(R, C, L);
+    const Plan p = plan_for(R, C, L), d = direct_plan(R, C, L, f32);
     return std::max(p.splits > 1 ? p.splits * (R * C + R) : 0, d.splits > 1 ? d.splits * R * C : 0);
 }
 
-// The backward pass by the direct kernel: dz and, from a checkpoint, x are written to memory first (they are read
-// by many tiles; the products are long), 16-byte aligned behind the splits' floats.
-int64_t align16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
-constexpr int64_t DB_CHUNKS = 256;
-bool direct_backward(int64_t M, int64_t N, int64_t K)
+// Scratch of a call: the splits' floats, then the operands written for the direct kernel, each with its flag words
+// (FP32), then the partial sums of db.
+int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
+constexpr int64_t PREP_CHUNKS = 256;
+int64_t prep_chunks(int64_t rows, int64_t cols)
 {
-    return direct_rows(N) && direct_rows(K) && direct_pays(M, K, N) && direct_pays(N, K, M);
+    const int64_t cb = (cols + 511) / 512;
+    return std::max<int64_t>(1, std::min(PREP_CHUNKS, std::min((2048 + cb - 1) / cb, (rows + 15) / 16)));
 }
-struct Places { int64_t floats, dz, x, db, bytes; };
-Places places(int64_t M, int64_t N, int64_t K)
+struct Room { int64_t at, flags, bytes; };
+struct Places { bool direct; Room x, w, dz; int64_t db, bytes; };
+
+Room place(int64_t &end, bool wanted, int64_t rows, int64_t cols, bool f32)
 {
-    Places p;
-    p.floats = 0;
-    p.dz = align16(std::max(scratch_floats(M, K, N), scratch_floats(N, K, M)) * 4);
-    const bool direct = direct_backward(M, N, K);
-    p.x = p.dz + (direct ? M * N * 2 : 0);              // N, K multiples of 8: aligned
-    p.db = p.x + (direct ? M * K * 2 : 0);
-    p.bytes = p.db + (direct ? DB_CHUNKS * N * 4 : 0);
+    Room r = {0, 0, 0};
+    if (!wanted) return r;
+    auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+    r.at = up(end);
+    r.flags = up(r.at + rows * padded(cols) * (f32 ? 6 : 2));
+    end = r.flags + (f32 ? (cols + 511) / 512 * prep_chunks(rows, cols) * 4 : 0);
+    r.bytes = end - r.at;
+    return r;
+}
+
+Places forward_places(int64_t M, int64_t N, int64_t K, bool f32)
+{
+    Places p = {};
+    p.bytes = M <= FEW ? 0 : scratch_floats(M, N, K, f32) * 4;
+    p.direct = M > FEW && direct_takes(M, N, K) && direct_rows(K);
+    const bool make = p.direct && (f32 || K % 8);
+    p.x = place(p.bytes, make, M, K, f32);
+    p.w = place(p.bytes, make, N, K, f32);
+    return p;
+}
+
+Places backward_places(int64_t M, int64_t N, int64_t K, bool f32)
+{
+    Places p = {};
+    p.bytes = std::max(scratch_floats(M, K, N, f32), scratch_floats(N, K, M, f32)) * 4;
+    p.direct = direct_takes(M, K, N) && direct_takes(N, K, M) && direct_rows(N) && direct_rows(K);
+    p.dz = place(p.bytes, p.direct, M, N, f32);
+    p.x = place(p.bytes, p.direct, M, K, f32);
+    p.w = place(p.bytes, p.direct && (f32 || K % 8), N, K, f32);
+    p.db = (p.bytes + 255) / 256 * 256;
+    if (p.direct) p.bytes = p.db + PREP_CHUNKS * N * 4;
     return p;
 }
 

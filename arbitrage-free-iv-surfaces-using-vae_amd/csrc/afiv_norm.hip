@@ -13,10 +13,11 @@
 // sums, added in chunk order by a second kernel, so results do not depend on scheduling.
 //
 // Statistics are summed in FP64 (plain sum and sum of squares: the squares are exact, and the
-// cancellation in var = E[x^2] - mu^2 costs 1e-16 mu^2/var), and h and the pre-activation are FP64
-// operations rounded to FP32 at their end: on this chip they cost what FP32 ones do, x - mu does not
-// cancel, and the sign of the pre-activation, where relu's derivative jumps, does not hang on an FP32
-// rounding.
+// cancellation in var = E[x^2] - mu^2 costs 1e-16 mu^2/var).  What follows is FP32 on mu split into two
+// parts, h = ((x - mu1) - mu2) rstd: x and mu1 are exact, so nothing is lost where they cancel, and h is within a few
+// roundings of its own size (all of it in FP64 took twice the registers and, with its conversions, twice
+// the time).  relu's derivative jumps at zero, so there a pre-activation within 2^-20 |beta| of zero, that is,
+// within reach of its rounding, is taken again in FP64, and its side is right to 1e-16.
 #include "afiv_layer.h"
 
 namespace {
@@ -41,6 +42,33 @@ struct NormArgs {
     uint8_t *scales;
     float *dgamma, *dbeta;
 };
+
+// Rows come in groups of four: their loads are issued together, so that a wave has several rows in flight (a row
+// at a time left HBM at 1.5 TB/s).  That needs loads that are not guarded one by one, so it is for lanes that have
+// all of their columns (FULL); the lane at a ragged edge goes row by row.
+
+template <bool FULL, class E, int V>
+__device__ __forceinline__ Pack<E, V> take(const E *p, int n)
+{
+    if constexpr (FULL) return load_pack<E, V>(p);
+    else return load_some<E, V>(p, n);
+}
+template <bool FULL, class E, int V>
+__device__ __forceinline__ void give(E *p, const Pack<E, V> &v, int n)
+{
+    if constexpr (FULL) store_pack<E, V>(p, v);
+    else store_some<E, V>(p, v, n);
+}
+
+// calls f(first row, rows) for the rows r0 + ty, + TY, ... below r1, four at a time and then one by one
+template <bool FULL, int TY, class F>
+__device__ __forceinline__ void each_group(int64_t r0, int64_t r1, int ty, F &&f)
+{
+    int64_t r = r0 + ty;
+    if constexpr (FULL)
+        for (; r + 3 * TY < r1; r += 4 * TY) f(r, std::integral_constant<int, 4>());
+    for (; r < r1; r += TY) f(r, std::integral_constant<int, 1>());
+}
 
 // Threads stand as TX lanes across columns (V elements each) by TY rows.  Sums of a column over the
 // TY rows of the workgroup: result at the threads of row 0, in row order.
@@ -69,7 +97,7 @@ __device__ __forceinline__ void reduce_rows(double (&a)[V], double (&b)[V], doub
     }
 }
 
-template <class T, int V, int TX>
+template <bool FULL, class T, int V, int TX>
 __device__ __forceinline__ void sum_x(const NormArgs &p, const T *__restrict__ x, int64_t r0, int64_t r1, int64_t col, int n,
                                       int ty, double (&s1)[V], double (&s2)[V])
 {
@@ -77,16 +105,20 @@ __device__ __forceinline__ void sum_x(const NormArgs &p, const T *__restrict__ x
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0;
     if (n <= 0) return;
-#pragma unroll 4
-    for (int64_t r = r0 + ty; r < r1; r += TY) {
-        const Pack<T, V> v = load_some<T, V>(x + r * p.N + col, n);
+    each_group<FULL, TY>(r0, r1, ty, [&](int64_t r, auto rows) {
+        constexpr int U = decltype(rows)::value;
+        Pack<T, V> v[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const double d = (double)(float)v.v[i];
-            s1[i] += d;
-            s2[i] = __builtin_fma(d, d, s2[i]);
-        }
-    }
+        for (int u = 0; u < U; ++u) v[u] = take<FULL, T, V>(x + (r + u * TY) * p.N + col, n);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double d = (double)(float)v[u].v[i];
+                s1[i] += d;
+                s2[i] = __builtin_fma(d, d, s2[i]);
+            }
+    });
 }
 
 // statistics of one column from its sums
@@ -105,69 +137,102 @@ __device__ __forceinline__ void finish_stats(const NormArgs &p, int64_t col, dou
     }
 }
 
-// outputs (and the checkpoint) of rows r0..r1 at columns col..col+n, a = gamma rstd
-template <class T, int V, int TX>
-__device__ __forceinline__ void apply_rows(const NormArgs &p, const T *__restrict__ x, T *__restrict__ y, int64_t r0, int64_t r1,
-                                           int64_t col, int n, int ty, const double (&mu)[V], const double (&a)[V], const float (&beta)[V])
+// what a thread holds of its V columns
+template <int V> struct Column { float mu1[V], mu2[V], rstd[V], gamma[V], beta[V]; };
+
+__device__ __forceinline__ void set_column(float &mu1, float &mu2, float &rstd, double mu, double r)
 {
-    constexpr int TY = THREADS / TX, LANES = 32 / V;        // lanes of a checkpoint block
-    const int64_t nb = (p.N + 31) / 32;
-#pragma unroll 2
-    for (int64_t r = r0 + ty; r < r1; r += TY) {
-        const int64_t at = r * p.N + col;
-        Pack<T, V> v = {};
-        if (n > 0) v = load_some<T, V>(x + at, n);
-        Pack<uint8_t, V> k;
-        if (p.keep && n > 0) k = load_some<uint8_t, V>(p.keep + at, n);
-        Pack<T, V> out;
-        float f[V], z[V];
+    mu1 = (float)mu;
+    mu2 = (float)(mu - (double)mu1);
+    rstd = (float)r;
+}
+
+template <int V>
+__device__ __forceinline__ void columns(const NormArgs &p, int64_t col, int n, Column<V> &k)
+{
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            f[i] = (float)v.v[i];
-            z[i] = (float)__builtin_fma((double)f[i] - mu[i], a[i], (double)beta[i]);
-        }
-        with_act(p.act, [&](auto act) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float o, d;
-                act_both<decltype(act)::value>(z[i], o, d);
-                z[i] = o;
-            }
-        });
-#pragma unroll
-        for (int i = 0; i < V; ++i) out.v[i] = (T)(p.keep ? (k.v[i] ? z[i] * p.scale : 0.0f) : z[i]);
-        if (n > 0) store_some<T, V>(y + at, out, n);
-        if (p.codes) {
-            float amax = 0.0f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) amax = fmaxf(amax, finite_abs(f[i]));
-#pragma unroll
-            for (int d = 1; d < LANES; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-            const int e = scale_byte(amax);
-            Pack<int8_t, V> q;
-#pragma unroll
-            for (int i = 0; i < V; ++i) q.v[i] = eight_code(f[i], e);
-            if (n > 0) {
-                store_some<int8_t, V>(p.codes + at, q, n);
-                if ((col & 31) == 0) p.scales[r * nb + col / 32] = (uint8_t)e;
-            }
+    for (int i = 0; i < V; ++i) {
+        k.mu1[i] = k.mu2[i] = k.rstd[i] = k.gamma[i] = k.beta[i] = 0.0f;
+        if (i < n) {
+            set_column(k.mu1[i], k.mu2[i], k.rstd[i], p.stats[col + i], p.stats[p.N + col + i]);
+            k.gamma[i] = p.gamma[col + i];
+            k.beta[i] = p.beta[col + i];
         }
     }
 }
 
+// h and the pre-activation z of V elements f.  sides: z's sign matters
 template <int V>
-__device__ __forceinline__ void column_affine(const NormArgs &p, int64_t col, int n, double (&mu)[V], double (&a)[V], float (&beta)[V])
+__device__ __forceinline__ void normalise(const NormArgs &p, const float (&f)[V], int64_t col, int n, const Column<V> &k, bool sides, float (&h)[V],
+                                          float (&z)[V])
 {
+    bool near = false;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        mu[i] = a[i] = 0.0;
-        beta[i] = 0.0f;
-        if (i < n) {
-            mu[i] = p.stats[col + i];
-            a[i] = (double)p.gamma[col + i] * p.stats[p.N + col + i];
-            beta[i] = p.beta[col + i];
-        }
+        h[i] = ((f[i] - k.mu1[i]) - k.mu2[i]) * k.rstd[i];
+        z[i] = __builtin_fmaf(h[i], k.gamma[i], k.beta[i]);
+        near |= fabsf(z[i]) <= 0x1p-20f * fabsf(k.beta[i]);
     }
+    if (sides && near) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) z[i] = (float)__builtin_fma(((double)f[i] - p.stats[col + i]) * p.stats[p.N + col + i], (double)k.gamma[i], (double)k.beta[i]);
+    }
+}
+
+// outputs (and the checkpoint) of rows r0..r1 at columns col..col+n
+template <bool FULL, class T, int V, int TX>
+__device__ __forceinline__ void apply_rows(const NormArgs &p, const T *__restrict__ x, T *__restrict__ y, int64_t r0, int64_t r1,
+                                           int64_t col, int n, int ty, const Column<V> &c)
+{
+    constexpr int TY = THREADS / TX, LANES = 32 / V;        // lanes of a checkpoint block
+    const int64_t nb = (p.N + 31) / 32;
+    with_act(p.act, [&](auto act) {
+        each_group<FULL, TY>(r0, r1, ty, [&](int64_t r, auto rows) {
+            constexpr int U = decltype(rows)::value;
+            Pack<T, V> v[U] = {};
+            Pack<uint8_t, V> k[U] = {};
+            if (FULL || n > 0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = take<FULL, T, V>(x + (r + u * TY) * p.N + col, n);
+                if (p.keep) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) k[u] = take<FULL, uint8_t, V>(p.keep + (r + u * TY) * p.N + col, n);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t at = (r + u * TY) * p.N + col;
+                Pack<T, V> out;
+                float f[V], h[V], z[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] = (float)v[u].v[i];
+                normalise<V>(p, f, col, n, c, false, h, z);             // f itself does not jump
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float o, d;
+                    act_both<decltype(act)::value>(z[i], o, d);
+                    out.v[i] = (T)(p.keep ? (k[u].v[i] ? o * p.scale : 0.0f) : o);
+                }
+                if (FULL || n > 0) give<FULL, T, V>(y + at, out, n);
+                if (p.codes) {
+                    float amax = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) amax = fmaxf(amax, finite_abs(f[i]));
+#pragma unroll
+                    for (int d = 1; d < LANES; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+                    const int e = scale_byte(amax);
+                    Pack<int8_t, V> q;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) q.v[i] = eight_code(f[i], e);
+                    if (FULL || n > 0) {
+                        give<FULL, int8_t, V>(p.codes + at, q, n);
+                        if ((col & 31) == 0) p.scales[(r + u * TY) * nb + col / 32] = (uint8_t)e;
+                    }
+                }
+            }
+        });
+    });
 }
 
 constexpr int WIDE = 16;       // TX of the chunked kernels
@@ -182,7 +247,8 @@ __global__ __launch_bounds__(THREADS) void stats_kernel(NormArgs p, const T *__r
     const int n = (int)(p.N - col < V ? p.N - col : V);
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
     double s1[V], s2[V];
-    sum_x<T, V, TX>(p, x, r0, r1, col, n, ty, s1, s2);
+    if (n >= V) sum_x<true, T, V, TX>(p, x, r0, r1, col, n, ty, s1, s2);
+    else sum_x<false, T, V, TX>(p, x, r0, r1, col, n, ty, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
     if (ty == 0) {
 #pragma unroll
@@ -236,10 +302,11 @@ __global__ __launch_bounds__(THREADS) void apply_kernel(NormArgs p, const T *__r
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
-    double mu[V], a[V];
-    float beta[V];
-    column_affine<V>(p, col, n, mu, a, beta);
-    apply_rows<T, V, TX>(p, x, y, r0, r1, col, n, ty, mu, a, beta);
+    Column<V> k;
+    columns<V>(p, col, n, k);
+    const bool whole = (int64_t)(blockIdx.x + 1) * TX * V <= p.N;       // the lanes of a checkpoint block stay together
+    if (whole) apply_rows<true, T, V, TX>(p, x, y, r0, r1, col, n, ty, k);
+    else apply_rows<false, T, V, TX>(p, x, y, r0, r1, col, n, ty, k);
 }
 
 // A batch of few rows: one workgroup does 32 columns from the sums to the outputs, in one launch.
@@ -252,7 +319,8 @@ __global__ __launch_bounds__(THREADS) void small_forward_kernel(NormArgs p, cons
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
     double s1[V], s2[V];
-    sum_x<T, V, TX>(p, x, 0, p.M, col, n, ty, s1, s2);
+    if (n >= V) sum_x<true, T, V, TX>(p, x, 0, p.M, col, n, ty, s1, s2);
+    else sum_x<false, T, V, TX>(p, x, 0, p.M, col, n, ty, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
     if (ty == 0) {
 #pragma unroll
@@ -261,125 +329,128 @@ __global__ __launch_bounds__(THREADS) void small_forward_kernel(NormArgs p, cons
                 double mu, rstd;
                 finish_stats(p, col + i, s1[i], s2[i], mu, rstd);
                 lds[(tx * V + i) * 2] = mu;
-                lds[(tx * V + i) * 2 + 1] = (double)p.gamma[col + i] * rstd;
+                lds[(tx * V + i) * 2 + 1] = rstd;
             }
     }
     __syncthreads();
-    double mu[V], a[V];
-    float beta[V];
+    Column<V> k;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        mu[i] = i < n ? lds[(tx * V + i) * 2] : 0.0;
-        a[i] = i < n ? lds[(tx * V + i) * 2 + 1] : 0.0;
-        beta[i] = i < n ? p.beta[col + i] : 0.0f;
-    }
-    apply_rows<T, V, TX>(p, x, y, 0, p.M, col, n, ty, mu, a, beta);
-}
-
-// ---- backward --------------------------------------------------------------------------------
-template <int V> struct Column { double mu[V], rstd[V]; float gamma[V], beta[V]; };
-
-template <int V>
-__device__ __forceinline__ void column_back(const NormArgs &p, int64_t col, int n, Column<V> &k)
-{
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        k.mu[i] = k.rstd[i] = 0.0;
-        k.gamma[i] = k.beta[i] = 0.0f;
+        k.mu1[i] = k.mu2[i] = k.rstd[i] = k.gamma[i] = k.beta[i] = 0.0f;
         if (i < n) {
-            k.mu[i] = p.stats[col + i];
-            k.rstd[i] = p.stats[p.N + col + i];
+            set_column(k.mu1[i], k.mu2[i], k.rstd[i], lds[(tx * V + i) * 2], lds[(tx * V + i) * 2 + 1]);
             k.gamma[i] = p.gamma[col + i];
             k.beta[i] = p.beta[col + i];
         }
     }
+    const bool whole = (int64_t)(blockIdx.x + 1) * TX * V <= p.N;
+    if (whole) apply_rows<true, T, V, TX>(p, x, y, 0, p.M, col, n, ty, k);
+    else apply_rows<false, T, V, TX>(p, x, y, 0, p.M, col, n, ty, k);
 }
 
-// g and h of V elements of a row
-template <class T, int V, bool EIGHT>
-__device__ __forceinline__ void g_and_h(const NormArgs &p, const T *__restrict__ x, const T *__restrict__ dy, int64_t r, int64_t nb,
-                                        int64_t col, int n, const Column<V> &k, float (&g)[V], float (&h)[V])
-{
-    const int64_t at = r * p.N + col;
-    const Pack<T, V> d = load_some<T, V>(dy + at, n);
-    Pack<uint8_t, V> m;
-    if (p.keep) m = load_some<uint8_t, V>(p.keep + at, n);
-    float f[V], z[V];
-    if (EIGHT) {
-        const Pack<int8_t, V> q = load_some<int8_t, V>(p.codes + at, n);
-        const int e = p.scales[r * nb + col / 32];
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = eight_value(q.v[i], e);
-    } else {
-        const Pack<T, V> v = load_some<T, V>(x + at, n);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = (float)v.v[i];
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const double hd = ((double)f[i] - k.mu[i]) * k.rstd[i];
-        h[i] = (float)hd;
-        g[i] = (float)d.v[i];
-        z[i] = (float)__builtin_fma(hd, (double)k.gamma[i], (double)k.beta[i]);
-    }
-    if (p.act != AFIV_ACT_NONE)
-        with_act(p.act, [&](auto act) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float f, d;
-                act_both<decltype(act)::value>(z[i], f, d);
-                g[i] *= d;
-            }
-        });
-    if (p.keep) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = m.v[i] ? g[i] * p.scale : 0.0f;
-    }
-}
+// ---- backward --------------------------------------------------------------------------------
+// what the backward pass reads of U rows, TY apart
+template <class T, int V, bool EIGHT, int U>
+struct BackRows {
+    Pack<T, V> d[U], x[EIGHT ? 1 : U];
+    Pack<uint8_t, V> k[U];
+    Pack<int8_t, V> q[EIGHT ? U : 1];
+    uint8_t e[U];
 
-template <class T, int V, int TX, bool EIGHT>
+    template <bool FULL>
+    __device__ __forceinline__ void load(const NormArgs &p, const T *__restrict__ xs, const T *__restrict__ dy, int64_t r, int ty_step, int64_t nb,
+                                         int64_t col, int n)
+    {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = r + u * ty_step, at = row * p.N + col;
+            d[u] = take<FULL, T, V>(dy + at, n);
+            if constexpr (EIGHT) {
+                q[u] = take<FULL, int8_t, V>(p.codes + at, n);
+                e[u] = p.scales[row * nb + col / 32];
+            } else x[u] = take<FULL, T, V>(xs + at, n);
+        }
+        if (p.keep) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[u] = take<FULL, uint8_t, V>(p.keep + (r + u * ty_step) * p.N + col, n);
+        }
+    }
+    // g and h of row u
+    template <int ACT>
+    __device__ __forceinline__ void g_and_h(const NormArgs &p, int u, int64_t col, int n, const Column<V> &c, float (&g)[V], float (&h)[V]) const
+    {
+        float f[V], z[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (EIGHT) f[i] = eight_value(q[u].v[i], e[u]);
+            else f[i] = (float)x[u].v[i];
+        }
+        normalise<V>(p, f, col, n, c, ACT == AFIV_ACT_RELU || ACT == AFIV_ACT_LEAKY_RELU, h, z);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float y, s;
+            act_both<ACT>(z[i], y, s);
+            g[i] = ACT == AFIV_ACT_NONE ? (float)d[u].v[i] : (float)d[u].v[i] * s;
+            if (p.keep) g[i] = k[u].v[i] ? g[i] * p.scale : 0.0f;
+        }
+    }
+};
+
+template <bool FULL, class T, int V, int TX, bool EIGHT>
 __device__ __forceinline__ void sum_g(const NormArgs &p, const T *__restrict__ x, const T *__restrict__ dy, int64_t r0, int64_t r1,
-                                      int64_t col, int n, int ty, const Column<V> &k, double (&s1)[V], double (&s2)[V])
+                                      int64_t col, int n, int ty, const Column<V> &c, double (&s1)[V], double (&s2)[V])
 {
     constexpr int TY = THREADS / TX;
     const int64_t nb = (p.N + 31) / 32;
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0;
     if (n <= 0) return;
-#pragma unroll 2
-    for (int64_t r = r0 + ty; r < r1; r += TY) {
-        float g[V], h[V];
-        g_and_h<T, V, EIGHT>(p, x, dy, r, nb, col, n, k, g, h);
+    with_act(p.act, [&](auto act) {
+        each_group<FULL, TY>(r0, r1, ty, [&](int64_t r, auto rows) {
+            BackRows<T, V, EIGHT, decltype(rows)::value> b;
+            b.template load<FULL>(p, x, dy, r, TY, nb, col, n);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            s1[i] += (double)g[i];
-            s2[i] = __builtin_fma((double)g[i], (double)h[i], s2[i]);
-        }
-    }
+            for (int u = 0; u < decltype(rows)::value; ++u) {
+                float g[V], h[V];
+                b.template g_and_h<decltype(act)::value>(p, u, col, n, c, g, h);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    s1[i] += (double)g[i];
+                    s2[i] = __builtin_fma((double)g[i], (double)h[i], s2[i]);
+                }
+            }
+        });
+    });
 }
 
 // mb = dbeta / M, mg = dgamma / M
-template <class T, int V, int TX, bool EIGHT>
+template <bool FULL, class T, int V, int TX, bool EIGHT>
 __device__ __forceinline__ void back_rows(const NormArgs &p, const T *__restrict__ x, const T *__restrict__ dy, T *__restrict__ dx,
-                                          int64_t r0, int64_t r1, int64_t col, int n, int ty, const Column<V> &k, const float (&mb)[V],
+                                          int64_t r0, int64_t r1, int64_t col, int n, int ty, const Column<V> &c, const float (&mb)[V],
                                           const float (&mg)[V])
 {
     constexpr int TY = THREADS / TX;
     const int64_t nb = (p.N + 31) / 32;
     if (n <= 0) return;
-#pragma unroll 2
-    for (int64_t r = r0 + ty; r < r1; r += TY) {
-        float g[V], h[V];
-        g_and_h<T, V, EIGHT>(p, x, dy, r, nb, col, n, k, g, h);
-        Pack<T, V> o;
+    with_act(p.act, [&](auto act) {
+        each_group<FULL, TY>(r0, r1, ty, [&](int64_t r, auto rows) {
+            BackRows<T, V, EIGHT, decltype(rows)::value> b;
+            b.template load<FULL>(p, x, dy, r, TY, nb, col, n);
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = (T)((float)(k.gamma[i] * k.rstd[i]) * (g[i] - mb[i] - h[i] * mg[i]));
-        store_some<T, V>(dx + r * p.N + col, o, n);
-    }
+            for (int u = 0; u < decltype(rows)::value; ++u) {
+                float g[V], h[V];
+                b.template g_and_h<decltype(act)::value>(p, u, col, n, c, g, h);
+                Pack<T, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.v[i] = (T)(c.gamma[i] * c.rstd[i] * (g[i] - mb[i] - h[i] * mg[i]));
+                give<FULL, T, V>(dx + (r + u * TY) * p.N + col, o, n);
+            }
+        });
+    });
 }
 
 template <class T, bool EIGHT>
-__global__ __launch_bounds__(THREADS) void back_sums_kernel(NormArgs p, const T *__restrict__ x, const T *__restrict__ dy)
+__global__ __launch_bounds__(THREADS, 2) void back_sums_kernel(NormArgs p, const T *__restrict__ x, const T *__restrict__ dy)
 {
     constexpr int V = Vec<T>::N, TX = WIDE;
     __shared__ double lds[THREADS / TX / 2 * TX * V * 2];
@@ -388,9 +459,10 @@ __global__ __launch_bounds__(THREADS) void back_sums_kernel(NormArgs p, const T 
     const int n = (int)(p.N - col < V ? p.N - col : V);
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
     Column<V> k;
-    column_back<V>(p, col, n, k);
+    columns<V>(p, col, n, k);
     double s1[V], s2[V];
-    sum_g<T, V, TX, EIGHT>(p, x, dy, r0, r1, col, n, ty, k, s1, s2);
+    if (n >= V) sum_g<true, T, V, TX, EIGHT>(p, x, dy, r0, r1, col, n, ty, k, s1, s2);
+    else sum_g<false, T, V, TX, EIGHT>(p, x, dy, r0, r1, col, n, ty, k, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
     if (ty == 0) {
 #pragma unroll
@@ -404,7 +476,7 @@ __global__ __launch_bounds__(THREADS) void back_sums_kernel(NormArgs p, const T 
 }
 
 template <class T, bool EIGHT>
-__global__ __launch_bounds__(THREADS) void back_dx_kernel(NormArgs p, const T *__restrict__ x, const T *__restrict__ dy, T *__restrict__ dx)
+__global__ __launch_bounds__(THREADS, 2) void back_dx_kernel(NormArgs p, const T *__restrict__ x, const T *__restrict__ dy, T *__restrict__ dx)
 {
     constexpr int V = Vec<T>::N, TX = WIDE;
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
@@ -412,18 +484,19 @@ __global__ __launch_bounds__(THREADS) void back_dx_kernel(NormArgs p, const T *_
     const int n = (int)(p.N - col < V ? p.N - col : V);
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
     Column<V> k;
-    column_back<V>(p, col, n, k);
+    columns<V>(p, col, n, k);
     float mb[V], mg[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         mb[i] = i < n ? (float)p.means[col + i] : 0.0f;
         mg[i] = i < n ? (float)p.means[p.N + col + i] : 0.0f;
     }
-    back_rows<T, V, TX, EIGHT>(p, x, dy, dx, r0, r1, col, n, ty, k, mb, mg);
+    if (n >= V) back_rows<true, T, V, TX, EIGHT>(p, x, dy, dx, r0, r1, col, n, ty, k, mb, mg);
+    else back_rows<false, T, V, TX, EIGHT>(p, x, dy, dx, r0, r1, col, n, ty, k, mb, mg);
 }
 
 template <class T, bool EIGHT>
-__global__ __launch_bounds__(THREADS) void small_backward_kernel(NormArgs p, const T *__restrict__ x, const T *__restrict__ dy,
+__global__ __launch_bounds__(THREADS, 2) void small_backward_kernel(NormArgs p, const T *__restrict__ x, const T *__restrict__ dy,
                                                                  T *__restrict__ dx)
 {
     constexpr int V = Vec<T>::N, TX = 32 / V;
@@ -432,9 +505,10 @@ __global__ __launch_bounds__(THREADS) void small_backward_kernel(NormArgs p, con
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
     Column<V> k;
-    column_back<V>(p, col, n, k);
+    columns<V>(p, col, n, k);
     double s1[V], s2[V];
-    sum_g<T, V, TX, EIGHT>(p, x, dy, 0, p.M, col, n, ty, k, s1, s2);
+    if (n >= V) sum_g<true, T, V, TX, EIGHT>(p, x, dy, 0, p.M, col, n, ty, k, s1, s2);
+    else sum_g<false, T, V, TX, EIGHT>(p, x, dy, 0, p.M, col, n, ty, k, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
     if (ty == 0) {
 #pragma unroll
@@ -454,7 +528,8 @@ __global__ __launch_bounds__(THREADS) void small_backward_kernel(NormArgs p, con
         mb[i] = i < n ? (float)lds[(tx * V + i) * 2] : 0.0f;
         mg[i] = i < n ? (float)lds[(tx * V + i) * 2 + 1] : 0.0f;
     }
-    back_rows<T, V, TX, EIGHT>(p, x, dy, dx, 0, p.M, col, n, ty, k, mb, mg);
+    if (n >= V) back_rows<true, T, V, TX, EIGHT>(p, x, dy, dx, 0, p.M, col, n, ty, k, mb, mg);
+    else back_rows<false, T, V, TX, EIGHT>(p, x, dy, dx, 0, p.M, col, n, ty, k, mb, mg);
 }
 
 // Rows up to which one launch of N/32 workgroups is taken instead of three.

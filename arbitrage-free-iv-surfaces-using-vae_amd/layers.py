@@ -15,11 +15,26 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .api import _ptr, _stream
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "tanh": 3, "gelu": 4, "silu": 5}
 NORM_SCRATCH_DOUBLES = 2 * 256 + 2      # afiv.h: AFIV_NORM_SCRATCH_DOUBLES, per column
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _run(name: str, device: torch.device, *args) -> None:
+    """One call of the library on the current stream of ``device``."""
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _act(name: str) -> int:
@@ -37,7 +52,13 @@ def _first(x, what: str) -> torch.Tensor:
         raise ValueError(f"{what} is on {x.device}: the layer kernels need a GPU (no CPU fallback)")
     if x.dtype not in DTYPES:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, got {x.dtype}")
-    return x.detach().contiguous()
+    return _plain(x)
+
+
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    if t.requires_grad:
+        t = t.detach()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = False) -> torch.Tensor:
@@ -46,13 +67,13 @@ def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = Fals
         raise TypeError(f"{what} must be a torch.Tensor")
     if t.device != x.device:
         raise ValueError(f"{what} is on {t.device}, expected {x.device}")
-    if t.dtype not in (dtypes or (x.dtype,)):
+    if (t.dtype != x.dtype) if dtypes is None else (t.dtype not in dtypes):
         raise TypeError(f"{what} must be {' or '.join(map(str, dtypes or (x.dtype,)))}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what} must be {list(shape)}, got {list(t.shape)}")
     if output and not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous: the kernels write into it in place")
-    return t.detach().contiguous()
+    return _plain(t)
 
 
 def _rows(x: torch.Tensor, what: str) -> int:
@@ -82,10 +103,8 @@ class Checkpoint8:
         """The tensor the codes stand for, in the type it was packed from."""
         out = torch.empty(self.codes.shape, dtype=self.dtype, device=self.codes.device)
         cols = self.codes.shape[-1]
-        with torch.cuda.device(out.device):
-            rc = _lib.lib().afiv_checkpoint8_restore(_ptr(self.codes), _ptr(self.scales), DTYPES[self.dtype],
-                                                     out.numel() // cols, cols, _ptr(out), _stream())
-        _lib.check(rc, "afiv_checkpoint8_restore")
+        _run("afiv_checkpoint8_restore", out.device, self.codes.data_ptr(), self.scales.data_ptr(), DTYPES[self.dtype],
+             out.numel() // cols, cols, out.data_ptr())
         return out
 
 
@@ -104,9 +123,7 @@ def checkpoint8(x: torch.Tensor) -> Checkpoint8:
 def _pack(v: torch.Tensor) -> Checkpoint8:
     rows, cols = _rows(v, "x"), v.shape[-1]
     out = _empty_checkpoint(v)
-    with torch.cuda.device(v.device):
-        rc = _lib.lib().afiv_checkpoint8_pack(_ptr(v), DTYPES[v.dtype], rows, cols, _ptr(out.codes), _ptr(out.scales), _stream())
-    _lib.check(rc, "afiv_checkpoint8_pack")
+    _run("afiv_checkpoint8_pack", v.device, v.data_ptr(), DTYPES[v.dtype], rows, cols, out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -150,13 +167,10 @@ def _linear(x, weight, bias, residual, act, want_pre: bool, want_codes: bool):
     y = torch.empty(shape, dtype=v.dtype, device=v.device)
     pre = torch.empty_like(y) if want_pre else None
     dcodes = torch.empty(shape, dtype=torch.uint8, device=v.device) if want_codes else None
-    L = _lib.lib()
-    nbytes = L.afiv_linear_act_scratch(m, n, k)
-    with torch.cuda.device(v.device):
-        scratch = _scratch(nbytes, v.device)
-        rc = L.afiv_linear_act(_ptr(v), _ptr(w), _ptr(b), _ptr(r), DTYPES[v.dtype], code, m, n, k, _ptr(y), _ptr(pre), _ptr(dcodes),
-                               _ptr(scratch), nbytes, _stream())
-    _lib.check(rc, "afiv_linear_act")
+    nbytes = _lib.lib().afiv_linear_act_scratch(m, n, k, DTYPES[v.dtype])
+    scratch = _scratch(nbytes, v.device)
+    _run("afiv_linear_act", v.device, v.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), DTYPES[v.dtype], code, m, n, k, y.data_ptr(), _ptr(pre),
+         _ptr(dcodes), _ptr(scratch), nbytes)
     return v, y, pre, dcodes
 
 
@@ -190,15 +204,11 @@ def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSav
     ran_on = (saved.x if saved.eight is None else saved.eight.codes).device
     if g.device != ran_on:
         raise ValueError(f"dy is on {g.device}, the forward pass ran on {ran_on}")
-    L = _lib.lib()
-    nbytes = L.afiv_linear_act_backward_scratch(m, n, k, DTYPES[g.dtype])
-    with torch.cuda.device(g.device):
-        scratch = _scratch(nbytes, g.device)
-        rc = L.afiv_linear_act_backward(_ptr(g), _ptr(saved.x), _ptr(saved.eight.codes if saved.eight else None),
-                                        _ptr(saved.eight.scales if saved.eight else None), _ptr(w), _ptr(saved.pre), _ptr(saved.dcodes),
-                                        DTYPES[g.dtype], _act(saved.act), m, n, k, _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), nbytes,
-                                        _stream())
-    _lib.check(rc, "afiv_linear_act_backward")
+    nbytes = _lib.lib().afiv_linear_act_backward_scratch(m, n, k, DTYPES[g.dtype])
+    scratch, eight = _scratch(nbytes, g.device), saved.eight
+    _run("afiv_linear_act_backward", g.device, g.data_ptr(), _ptr(saved.x), eight and eight.codes.data_ptr(), eight and eight.scales.data_ptr(),
+         w.data_ptr(), _ptr(saved.pre), _ptr(saved.dcodes), DTYPES[g.dtype], _act(saved.act), m, n, k, _ptr(dx), _ptr(dw), _ptr(db),
+         _ptr(scratch), nbytes)
     return dx, dw, db
 
 
@@ -275,12 +285,10 @@ def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     y = torch.empty_like(v)
     stats = torch.empty((2, n), dtype=torch.float64, device=v.device)
     eight = _empty_checkpoint(v) if checkpoint8 else None
-    with torch.cuda.device(v.device):
-        scratch = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=v.device)
-        rc = _lib.lib().afiv_norm_act(_ptr(v), _ptr(gamma), _ptr(beta), _ptr(keep), DTYPES[v.dtype], code, m, n, float(eps), float(momentum),
-                                      drop_p, _ptr(running_mean), _ptr(running_var), _ptr(y), _ptr(stats),
-                                      _ptr(eight.codes if eight else None), _ptr(eight.scales if eight else None), _ptr(scratch), _stream())
-    _lib.check(rc, "afiv_norm_act")
+    scratch = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=v.device)
+    _run("afiv_norm_act", v.device, v.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _ptr(keep), DTYPES[v.dtype], code, m, n, float(eps),
+         float(momentum), drop_p, _ptr(running_mean), _ptr(running_var), y.data_ptr(), stats.data_ptr(), eight and eight.codes.data_ptr(),
+         eight and eight.scales.data_ptr(), scratch.data_ptr())
     if running_mean is not None:         # written behind torch's back: caches keyed on versions must see it
         torch.autograd.graph.increment_version(running_mean)
         torch.autograd.graph.increment_version(running_var)
@@ -301,13 +309,10 @@ def batch_norm_act_backward(dy: torch.Tensor, weight: torch.Tensor, bias: torch.
     gamma, beta = _like(weight, g, (n,), "weight", f32), _like(bias, g, (n,), "bias", f32)
     dx = torch.empty_like(g) if need_dx else None
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
-    with torch.cuda.device(g.device):
-        scratch = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=g.device)
-        rc = _lib.lib().afiv_norm_act_backward(_ptr(g), _ptr(saved.x), _ptr(saved.eight.codes if saved.eight else None),
-                                               _ptr(saved.eight.scales if saved.eight else None), _ptr(gamma), _ptr(beta), _ptr(saved.keep),
-                                               _ptr(saved.stats), DTYPES[g.dtype], _act(saved.act), m, n, saved.drop_p, _ptr(dx),
-                                               _ptr(dgamma), _ptr(dbeta), _ptr(scratch), _stream())
-    _lib.check(rc, "afiv_norm_act_backward")
+    scratch, eight = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=g.device), saved.eight
+    _run("afiv_norm_act_backward", g.device, g.data_ptr(), _ptr(saved.x), eight and eight.codes.data_ptr(), eight and eight.scales.data_ptr(),
+         gamma.data_ptr(), beta.data_ptr(), _ptr(saved.keep), saved.stats.data_ptr(), DTYPES[g.dtype], _act(saved.act), m, n, saved.drop_p,
+         _ptr(dx), dgamma.data_ptr(), dbeta.data_ptr(), scratch.data_ptr())
     return dx, dgamma, dbeta
 
 

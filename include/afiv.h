@@ -279,8 +279,9 @@ int afiv_checkpoint8_restore(const int8_t *codes, const uint8_t *scales, int dty
  * For the backward pass one of these is kept, or both NULL: pre_out [M,N] T = the pre-activation, or
  * dcodes_out [M,N] = the activation's derivative in 8 bits (multiples of 1/200; relu and leaky_relu:
  * the sign; unused and may be NULL for AFIV_ACT_NONE).  M >= 0; 1 <= N, K <= 2^24.
- * scratch: device memory of at least afiv_linear_act_scratch(M, N, K) bytes (NULL where that is 0). */
-int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K);
+ * scratch: 16-byte aligned device memory of at least afiv_linear_act_scratch(M, N, K, dtype) bytes (NULL where that
+ * is 0). */
+int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K, int dtype);
 int afiv_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
                     int64_t K, void *y, void *pre_out, uint8_t *dcodes_out, void *scratch, int64_t scratch_bytes, void *stream);
 
@@ -289,8 +290,8 @@ int afiv_linear_act(const void *x, const void *w, const void *bias, const void *
  * its 8-bit checkpoint (codes, scales); the derivative from pre [M,N] T or, with pre == NULL, from
  * dcodes [M,N] (neither for AFIV_ACT_NONE).  w is needed for dx, the input for dw.  dy times the
  * derivative is rounded to T before the products (FP32: not rounded), db is summed before that rounding. */
-/* scratch: at least afiv_linear_act_backward_scratch(M, N, K, dtype) bytes; large products of 16-bit types keep dz
- * [M,N] and, from a checkpoint, x [M,K] there during the call. */
+/* scratch: 16-byte aligned, at least afiv_linear_act_backward_scratch(M, N, K, dtype) bytes (NULL where that is 0); large
+ * products keep dz [M,N] and, where they cannot read them in place, x [M,K] and w [N,K] there during the call. */
 int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype);
 int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w, const void *pre,
                              const uint8_t *dcodes, int dtype, int act, int64_t M, int64_t N, int64_t K, void *dx, void *dw, void *db,

@@ -123,7 +123,8 @@ def test_linear_forward_and_backward(afiv, typ, m, k, n):
 
 @pytest.mark.parametrize("typ,m,k,n", [("bf16", 2048, 1024, 2048), ("f16", 4096, 512, 1024), ("f32", 2048, 512, 2304), ("bf16", 2300, 1096, 2056),
                                        ("bf16", 40000, 64, 72), ("f32", 40000, 24, 40), ("bf16", 4104, 200, 4112), ("f16", 4104, 4120, 136),
-                                       ("bf16", 1000, 4096, 4200), ("f16", 136, 1288, 6008)])
+                                       ("bf16", 1000, 4096, 4200), ("f16", 136, 1288, 6008),
+                                       ("bf16", 1501, 777, 1029), ("f32", 1501, 777, 1029), ("f32", 4104, 200, 4112), ("f32", 300, 4096, 2100)])
 def test_linear_large_tiles(afiv, typ, m, k, n):
     x, w, b, r, dy = inputs(TYPES[typ], m, k, n, 5, residual=True)
     for act, eight in (("gelu", True), ("tanh", False)):
@@ -173,8 +174,8 @@ def test_linear_values_that_are_not_finite(afiv, typ):
     """An infinity or NaN of one row reaches that row of y and no other; in FP32 so do magnitudes that do
     not split into three parts."""
     t = TYPES[typ]
-    for m in (8, 200):                                     # the kernel for few rows, and the tiles
-        x, w, b, _, dy = inputs(t, m, 70, 30, 9)
+    for m, k, n in ((8, 70, 30), (200, 70, 30), (1500, 136, 520)):      # the kernels for few rows, small and large products
+        x, w, b, _, dy = inputs(t, m, k, n, 9)
         w = w.abs() + 0.01
         clean = afiv.linear_act(x, w, b)
         for bad in (float("inf"), float("-inf"), float("nan"), torch.finfo(t).max / 16):
@@ -185,18 +186,27 @@ def test_linear_values_that_are_not_finite(afiv, typ):
             assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
             assert torch.equal(y[3][torch.isinf(want[3])], want[3][torch.isinf(want[3])])
             rows = torch.arange(m, device="cuda") != 3
-            tol = 300 * U * (1 + clean.double().abs()) * 70 + half(t) * clean.double().abs()
+            tol = 300 * U * (1 + clean.double().abs()) * k + half(t) * clean.double().abs()
             within(y[rows], clean.double()[rows], 2 * tol[rows], "other rows")
             fin = torch.isfinite(want[3])
             assert torch.allclose(y[3][fin].double(), want[3][fin].double(), rtol=4 * half(t) + 1e-5)
-    # a gradient: row 3 of dy
-    x, w, b, _, dy = inputs(t, 200, 70, 30, 9)
-    y, saved = afiv.linear_act_forward(x, w, b, act="tanh")
-    dy = dy.clone()
-    dy[3] = float("inf")
-    dx, dw, db = afiv.linear_act_backward(dy, w, saved)
-    assert not torch.isfinite(dx[3]).any() and torch.isfinite(dx[torch.arange(200, device="cuda") != 3]).all()
-    assert not torch.isfinite(dw).any() and not torch.isfinite(db).any()
+    # a gradient: row 3 of dy, and a column of it
+    for m, k, n in ((200, 70, 30), (1500, 520, 1030)):
+        for eight in (False, True):
+            x, w, b, _, dy = inputs(t, m, k, n, 9)
+            y, saved = afiv.linear_act_forward(x, w, b, act="tanh", checkpoint8=eight)
+            row = dy.clone()
+            row[3] = float("inf")
+            dx, dw, db = afiv.linear_act_backward(row, w, saved)
+            assert not torch.isfinite(dx[3]).any() and torch.isfinite(dx[torch.arange(m, device="cuda") != 3]).all()
+            if not eight:                                   # a derivative of 0 in 8 bits makes NaN, which is not finite either
+                assert not torch.isfinite(dw).all(1).any() and not torch.isfinite(db).any()
+            clean = afiv.linear_act_backward(dy, w, saved)
+            dy[5, 7] = float("nan")
+            dx, dw, db = afiv.linear_act_backward(dy, w, saved)
+            rows, cols = torch.arange(m, device="cuda") != 5, torch.arange(n, device="cuda") != 7
+            assert torch.isnan(dx[5]).all() and torch.equal(dx[rows], clean[0][rows])
+            assert torch.isnan(dw[7]).all() and torch.equal(dw[cols], clean[1][cols]) and torch.isnan(db[7]) and torch.equal(db[cols], clean[2][cols])
 
 
 def test_linear_small_magnitudes(afiv):

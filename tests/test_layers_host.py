@@ -54,13 +54,13 @@ def test_linear_refusals(lib):
     assert fwd(m=1 << 35, n=1 << 20) == E_SHAPE                                  # more tiles than a launch has
     assert fwd(x=None) == E_NULL and fwd(w=None) == E_NULL and fwd(y=None) == E_NULL
     assert fwd(m=0, x=None, y=None) == 0
-    need = lib.afiv_linear_act_scratch(64, 64, 4096)
+    need = lib.afiv_linear_act_scratch(64, 64, 4096, 0)
     assert need > 0
     assert fwd(m=64, n=64, k=4096, scratch=None) == E_WORKSPACE
     assert fwd(m=64, n=64, k=4096, nbytes=need - 1) == E_WORKSPACE
-    assert lib.afiv_linear_act_scratch(-1, 4, 4) == E_SHAPE and lib.afiv_linear_act_backward_scratch(4, 4, 0, 0) == E_SHAPE
+    assert lib.afiv_linear_act_scratch(-1, 4, 4, 0) == E_SHAPE and lib.afiv_linear_act_backward_scratch(4, 4, 0, 0) == E_SHAPE
     assert lib.afiv_linear_act_backward_scratch(4, 4, 4, 3) == E_ARG
-    assert lib.afiv_linear_act_scratch(1 << 20, 1024, 1024) == 0                 # enough tiles: the sum is not cut
+    assert lib.afiv_linear_act_scratch(1 << 20, 1024, 1024, 1) == 0                 # enough tiles: the sum is not cut
 
     def bwd(dy=p, x=p, codes=None, scales=None, w=p, pre=None, dcodes=None, act=0, m=4, n=4, k=4, dx=p, dw=p, db=p, nbytes=1 << 40):
         return lib.afiv_linear_act_backward(dy, x, codes, scales, w, pre, dcodes, 0, act, m, n, k, dx, dw, db, p, nbytes, None)
