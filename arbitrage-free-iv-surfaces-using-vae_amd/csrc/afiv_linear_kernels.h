@@ -595,7 +595,7 @@ struct Direct {
 #if defined(__HIP_DEVICE_COMPILE__)             // buffer resources have no host type
         const P *corner = base + (XS ? l0 * ld + row0 : row0 * ld + l0);
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)corner, 0, 0x7fffffff, 0x00020000);
-        const int left = (int)(l_end - l0 < FK ? l_end - l0 : FK);
+        const int left = (int)(l_end - l0 < FK ? (l_end > l0 ? l_end - l0 : 0) : FK);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (wave * PER + i) * 1024), 16,
@@ -652,9 +652,13 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
     typedef typename Mma<T>::frag frag;
     typedef Direct<P, across(KA), FK, BR, W, TR> DA;
     typedef Direct<P, across(KB), FK, BC, W, TC> DB;
-    constexpr int STAGE = PARTS * (DA::BYTES + DB::BYTES);
-    __shared__ __align__(1024) char lds[2 * STAGE];
-    constexpr int SLAB = 16 * 16 * TC, FIT = 2 * STAGE / W / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
+    // each buffer an array of its own, named where it is used: the compiler then knows that loads into one do not
+    // touch reads of the other, and does not make those wait
+    __shared__ __align__(1024) char a0[PARTS * DA::BYTES];
+    __shared__ __align__(1024) char a1[PARTS * DA::BYTES];
+    __shared__ __align__(1024) char b0[PARTS * DB::BYTES];
+    __shared__ __align__(1024) char b1[PARTS * DB::BYTES];
+    constexpr int SLAB = 16 * 16 * TC, FIT = PARTS * DA::BYTES / W / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = (wave % WR) * 16 * TR, wc = (wave / WR) * 16 * TC;
     int64_t split, tr, tc;
@@ -667,57 +671,87 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
     db.init(a.C, sb.ld, col0, wc, wave, lane);
     f32x4 acc[TR][TC] = {};
 
-    auto load = [&](char *s, int64_t l0) {
-        if (l0 < l_end) {
+    auto load = [&](char *la, char *lb, int64_t l0) {                      // from l_end on: zeros
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                da.load((const P *)sa.p + p * sa.plane, sa.ld, row0, l0, l_end, s + p * DA::BYTES, wave);
-                db.load((const P *)sb.p + p * sb.plane, sb.ld, col0, l0, l_end, s + PARTS * DA::BYTES + p * DB::BYTES, wave);
-            }
+        for (int p = 0; p < PARTS; ++p) {
+            da.load((const P *)sa.p + p * sa.plane, sa.ld, row0, l0, l_end, la + p * DA::BYTES, wave);
+            db.load((const P *)sb.p + p * sb.plane, sb.ld, col0, l0, l_end, lb + p * DB::BYTES, wave);
         }
     };
-    auto multiply = [&](const char *s) {
+    // Fragments of one 32-step slice at a time: while row block i of this slice is multiplied, its registers take
+    // the next slice's (those of B, shared by the row blocks, have a second set), so the matrix units need not
+    // wait for LDS, nor the reads for a barrier that comes once a step.
+    frag fa[PARTS][TR], fb[2][PARTS][TC];
+    auto read_a = [&](const char *s, int i, int kk) {
 #pragma unroll
-        for (int kk = 0; kk < FK / 32; ++kk) {
-            frag fa[PARTS][TR], fb[PARTS][TC];
+        for (int p = 0; p < PARTS; ++p) fa[p][i] = da.read(s + p * DA::BYTES, i, kk);
+    };
+    auto read_b = [&](const char *s, int set, int j, int kk) {
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
+        for (int p = 0; p < PARTS; ++p) fb[set][p][j] = db.read(s + p * DB::BYTES, j, kk);
+    };
+    auto slice = [&](int set, const char *na, const char *nb, int next_kk) {
 #pragma unroll
-                for (int j = 0; j < TC; ++j) fb[p][j] = db.read(s + PARTS * DA::BYTES + p * DB::BYTES, j, kk);
-#pragma unroll
-                for (int i = 0; i < TR; ++i) fa[p][i] = da.read(s + p * DA::BYTES, i, kk);
-            }
+        for (int i = 0; i < TR; ++i) {
 #pragma unroll
             for (int p = PARTS - 1; p >= 0; --p)                  // small products first
 #pragma unroll
                 for (int q = 0; q <= p; ++q)
 #pragma unroll
-                    for (int i = 0; i < TR; ++i)
-#pragma unroll
-                        for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[q][j], fa[p - q][i], acc[i][j]);
+                    for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[set][q][j], fa[p - q][i], acc[i][j]);
+            read_a(na, i, next_kk);
+            if (i < TC) read_b(nb, set ^ 1, i, next_kk);
+            __builtin_amdgcn_sched_group_barrier(0x008, TC * PARTS * (PARTS + 1) / 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, PARTS * (across(KA) ? 2 : 1), 0);
+            if (i < TC) __builtin_amdgcn_sched_group_barrier(0x100, PARTS * (across(KB) ? 2 : 1), 0);
         }
     };
-    // every load of this wave has arrived (vmcnt 0) before any wave reads the tile, and every read of the
-    // other buffer is done before any wave loads into it
+    static_assert(TC <= TR, "a row block for every column block's reads");
+    // every load of this wave has arrived and its reads are done (vmcnt 0, lgkmcnt 0) before any wave reads the next
+    // tile or loads over this one
     auto meet = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __builtin_amdgcn_s_waitcnt(0x0070);
         __syncthreads();
     };
-    int here = 0;
-    load(lds, l_begin);
+    load(a0, b0, l_begin);
+    load(a1, b1, l_begin + FK);
+    meet();
+#pragma unroll
+    for (int i = 0; i < TR; ++i) read_a(a0, i, 0);
+#pragma unroll
+    for (int j = 0; j < TC; ++j) read_b(b0, 0, j, 0);
+    // (sched_barrier: loads are issued before the products, not among them)
 #pragma unroll 1
-    for (int64_t l0 = l_begin; l0 < l_end; l0 += FK) {
-        meet();
-        load(lds + (STAGE - here), l0 + FK);
-        multiply(lds + here);
-        here = STAGE - here;
+    for (int64_t l0 = l_begin; l0 < l_end; l0 += 2 * FK) {      // an odd last step is multiplied with zeros
+        if constexpr (FK == 64) {
+            slice(0, a0, b0, 1);
+            meet();
+            load(a0, b0, l0 + 2 * FK);
+            __builtin_amdgcn_sched_barrier(0);
+            slice(1, a1, b1, 0);
+            slice(0, a1, b1, 1);
+            meet();
+            load(a1, b1, l0 + 3 * FK);
+            __builtin_amdgcn_sched_barrier(0);
+            slice(1, a0, b0, 0);
+        } else {
+            meet();
+            load(a0, b0, l0 + 2 * FK);
+            __builtin_amdgcn_sched_barrier(0);
+            slice(0, a1, b1, 0);
+            meet();
+            load(a1, b1, l0 + 3 * FK);
+            __builtin_amdgcn_sched_barrier(0);
+            slice(1, a0, b0, 0);
+        }
     }
+    __builtin_amdgcn_s_waitcnt(0x0070);                         // the last loads and reads, before LDS is used again
     if constexpr (PARTS == 3) {
         if (__syncthreads_or(unsplittable<across(KA)>(sa, row0, BR) || unsplittable<across(KB)>(sb, col0, BC)))
             plain_sums<T, KA, KB, TR, TC>(a, acc, row0 + wr, col0 + wc, l_begin, l_end, lane);
     }
     __syncthreads();
-    write_out<T, EPI, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)lds + wave * SLABS * SLAB);
+    write_out<T, EPI, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)a0 + wave * SLABS * SLAB);
 }
 
 // An operand for the direct kernel, [rows, cols] -> [rows, ldp] of 16-bit elements (FP32: three planes of BF16 parts),
