@@ -327,12 +327,33 @@ __device__ __forceinline__ void finish(const LinArgs &a, int64_t i, int64_t j, f
 // each 16 x 16 block) by way of LDS, SLABS blocks of 16 rows at a time in the wave's own room: a lane then
 // has 8 neighbouring columns, the memory accesses are whole lines, and the epilogue's code stands once.
 // The 16-byte chunks of a row are permuted by the row so that a column of writes meets all banks.
+// Tiles inside the matrix take the forward epilogue four rows at a time, the residual's loads first: one by one they
+// were a fifth of a large layer's time.
 template <class T, bool EPI, int TR, int TC, int SLABS>
 __device__ __forceinline__ void write_out(const LinArgs &a, const f32x4 (&acc)[TR][TC], int64_t row0, int64_t col0, int64_t split, int lane,
                                           float *room)
 {
     constexpr int COLS = 16 * TC, CHUNKS = COLS / 4, UNITS = 16 * COLS / 8;      // of a slab
-    static_assert(TR % SLABS == 0 && UNITS % 64 == 0, "whole passes");
+    static_assert(TR % SLABS == 0 && UNITS % 64 == 0 && 64 % (COLS / 8) == 0, "whole passes, a lane's column stays");
+    const bool inside = row0 + 16 * TR <= a.R && col0 + COLS <= a.C && a.splits == 1;
+    const int c0 = lane % (COLS / 8) * 2;                                          // a lane's first chunk
+    const int64_t col = col0 + c0 * 4;
+    float bias[8] = {};
+    if (EPI && inside && a.bias) {
+        const Pack<T, 8> b = load_pack<T, 8>((const T *)a.bias + col);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) bias[q] = (float)b.v[q];
+    }
+    auto from_room = [&](int r, float (&z)[8]) {
+        const f32x4 lo = *(const f32x4 *)&room[r * COLS + ((c0 ^ (r & (CHUNKS - 1))) * 4)];
+        const f32x4 hi = *(const f32x4 *)&room[r * COLS + (((c0 + 1) ^ (r & (CHUNKS - 1))) * 4)];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            z[q] = lo[q];
+            z[4 + q] = hi[q];
+        }
+    };
+    constexpr int RSTEP = 64 / (COLS / 8), ROWS = SLABS * 16, G = ROWS / RSTEP < 4 ? ROWS / RSTEP : 4;   // rows from unit to unit
 #pragma unroll 1
     for (int phase = 0; phase < TR / SLABS; ++phase) {
 #pragma unroll
@@ -348,25 +369,54 @@ __device__ __forceinline__ void write_out(const LinArgs &a, const f32x4 (&acc)[T
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        const int64_t first = row0 + phase * ROWS;
+        if (EPI && inside) {
 #pragma unroll 1
-        for (int u = lane; u < SLABS * UNITS; u += 64) {
-            const int r = u / (COLS / 8), c = u % (COLS / 8) * 2;
-            const int64_t row = row0 + phase * SLABS * 16 + r, col = col0 + c * 4;
-            if (row < a.R && col < a.C) {
-                float z[8];
-                const f32x4 lo = *(const f32x4 *)&room[r * COLS + ((c ^ (r & (CHUNKS - 1))) * 4)];
-                const f32x4 hi = *(const f32x4 *)&room[r * COLS + (((c + 1) ^ (r & (CHUNKS - 1))) * 4)];
+            for (int r0 = lane / (COLS / 8); r0 < ROWS; r0 += G * RSTEP) {
+                Pack<T, 8> res[G];
+                if (a.residual) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    z[q] = lo[q];
-                    z[4 + q] = hi[q];
+                    for (int g = 0; g < G; ++g) res[g] = load_pack<T, 8>((const T *)a.residual + (first + r0 + g * RSTEP) * a.C + col);
                 }
-                if (a.splits > 1) {
-                    Pack<float, 8> o;
+                with_act(a.act_out, [&](auto act) {
+                    constexpr int ACT = decltype(act)::value;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) o.v[q] = z[q];
-                    store_some<float, 8>(a.partial + (split * a.R + row) * a.C + col, o, (int)(a.C - col < 8 ? a.C - col : 8));
-                } else finish<T, EPI, 8>(a, row, col, z);
+                    for (int g = 0; g < G; ++g) {
+                        const int64_t at = (first + r0 + g * RSTEP) * a.C + col;
+                        float z[8];
+                        from_room(r0 + g * RSTEP, z);
+                        Pack<T, 8> o, pre;
+                        Pack<uint8_t, 8> code;
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            z[q] += bias[q];
+                            float y, d;
+                            act_both<ACT>(z[q], y, d);
+                            pre.v[q] = (T)z[q];
+                            if (a.dcodes_out) code.v[q] = derivative_code<ACT>(z[q], d);
+                            if (a.residual) y += (float)res[g].v[q];
+                            o.v[q] = (T)y;
+                        }
+                        if (a.pre_out) store_pack<T, 8>((T *)a.pre_out + at, pre);
+                        if (a.dcodes_out) store_pack<uint8_t, 8>(a.dcodes_out + at, code);
+                        store_pack<T, 8>((T *)a.out + at, o);
+                    }
+                });
+            }
+        } else {
+#pragma unroll 1
+            for (int r = lane / (COLS / 8); r < ROWS; r += RSTEP) {
+                const int64_t row = first + r;
+                if (row < a.R && col < a.C) {
+                    float z[8];
+                    from_room(r, z);
+                    if (a.splits > 1) {
+                        Pack<float, 8> o;
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) o.v[q] = z[q];
+                        store_some<float, 8>(a.partial + (split * a.R + row) * a.C + col, o, (int)(a.C - col < 8 ? a.C - col : 8));
+                    } else finish<T, EPI, 8>(a, row, col, z);
+                }
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -658,7 +708,11 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
     __shared__ __align__(1024) char a1[PARTS * DA::BYTES];
     __shared__ __align__(1024) char b0[PARTS * DB::BYTES];
     __shared__ __align__(1024) char b1[PARTS * DB::BYTES];
-    constexpr int SLAB = 16 * 16 * TC, FIT = PARTS * DA::BYTES / W / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
+    __shared__ __align__(1024) char a2[PARTS == 3 ? PARTS * DA::BYTES : 16];
+    __shared__ __align__(1024) char b2[PARTS == 3 ? PARTS * DB::BYTES : 16];
+    // the epilogue's room of a wave: a quarter of the waves share an array
+    static_assert(W % 4 == 0 && DA::BYTES == DB::BYTES, "four arrays of one size");
+    constexpr int SLAB = 16 * 16 * TC, FIT = PARTS * DA::BYTES / (W / 4) / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = (wave % WR) * 16 * TR, wc = (wave / WR) * 16 * TC;
     int64_t split, tr, tc;
@@ -707,23 +761,31 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
         }
     };
     static_assert(TC <= TR, "a row block for every column block's reads");
-    // every load of this wave has arrived and its reads are done (vmcnt 0, lgkmcnt 0) before any wave reads the next
-    // tile or loads over this one
-    auto meet = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0070);
-        __syncthreads();
+    // all but this wave's last AHEAD loads have arrived and its reads are done, before any wave reads the next tile or
+    // loads over this one
+    constexpr int LOADS = PARTS * (DA::PER + DB::PER), AHEAD = PARTS == 3 ? LOADS : 0;
+    // (__syncthreads would wait for every load: the bare barrier, with nothing moved across it)
+    auto arrive = [&](auto left) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0070 | (decltype(left)::value & 15) | (decltype(left)::value >> 4 << 14));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
     };
+    auto meet = [&]() { arrive(std::integral_constant<int, AHEAD>()); };
     load(a0, b0, l_begin);
     load(a1, b1, l_begin + FK);
-    meet();
+    if constexpr (PARTS == 3) load(a2, b2, l_begin + 2 * FK);
+    arrive(std::integral_constant<int, 2 * AHEAD>());
 #pragma unroll
     for (int i = 0; i < TR; ++i) read_a(a0, i, 0);
 #pragma unroll
     for (int j = 0; j < TC; ++j) read_b(b0, 0, j, 0);
     // (sched_barrier: loads are issued before the products, not among them)
+    if constexpr (FK == 64) {
 #pragma unroll 1
-    for (int64_t l0 = l_begin; l0 < l_end; l0 += 2 * FK) {      // an odd last step is multiplied with zeros
-        if constexpr (FK == 64) {
+        for (int64_t l0 = l_begin; l0 < l_end; l0 += 2 * FK) {  // an odd last step is multiplied with zeros
             slice(0, a0, b0, 1);
             meet();
             load(a0, b0, l0 + 2 * FK);
@@ -734,15 +796,25 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
             load(a1, b1, l0 + 3 * FK);
             __builtin_amdgcn_sched_barrier(0);
             slice(1, a0, b0, 0);
-        } else {
-            meet();
-            load(a0, b0, l0 + 2 * FK);
-            __builtin_amdgcn_sched_barrier(0);
-            slice(0, a1, b1, 0);
-            meet();
-            load(a1, b1, l0 + 3 * FK);
-            __builtin_amdgcn_sched_barrier(0);
-            slice(1, a0, b0, 0);
+        }
+    } else {
+        // steps are short here (0.6 us of products), so loads run two steps ahead, in three buffers
+        auto step = [&](int64_t l0, char *la, char *lb, int set, const char *na, const char *nb) {
+            if (l0 < l_end) {
+                meet();
+                load(la, lb, l0 + 3 * FK);
+                __builtin_amdgcn_sched_barrier(0);
+                slice(set, na, nb, 0);
+            }
+        };
+#pragma unroll 1
+        for (int64_t l0 = l_begin; l0 < l_end; l0 += 6 * FK) {
+            step(l0, a0, b0, 0, a1, b1);
+            step(l0 + FK, a1, b1, 1, a2, b2);
+            step(l0 + 2 * FK, a2, b2, 0, a0, b0);
+            step(l0 + 3 * FK, a0, b0, 1, a1, b1);
+            step(l0 + 4 * FK, a1, b1, 0, a2, b2);
+            step(l0 + 5 * FK, a2, b2, 1, a0, b0);
         }
     }
     __builtin_amdgcn_s_waitcnt(0x0070);                         // the last loads and reads, before LDS is used again
@@ -751,7 +823,8 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
             plain_sums<T, KA, KB, TR, TC>(a, acc, row0 + wr, col0 + wc, l_begin, l_end, lane);
     }
     __syncthreads();
-    write_out<T, EPI, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)a0 + wave * SLABS * SLAB);
+    write_out<T, EPI, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane,
+                                        (float *)(wave % 4 == 0 ? a0 : wave % 4 == 1 ? a1 : wave % 4 == 2 ? b0 : b1) + wave / 4 * SLABS * SLAB);
 }
 
 // An operand for the direct kernel, [rows, cols] -> [rows, ldp] of 16-bit elements (FP32: three planes of BF16 parts),

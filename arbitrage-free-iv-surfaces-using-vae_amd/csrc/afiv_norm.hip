@@ -12,8 +12,9 @@
 // checkpoint, dy and keep twice.  Column sums go row chunk by row chunk: P chunks give P partial
 // sums, added in chunk order by a second kernel, so results do not depend on scheduling.
 //
-// Statistics are summed in FP64 (plain sum and sum of squares: the squares are exact, and the
-// cancellation in var = E[x^2] - mu^2 costs 1e-16 mu^2/var).  What follows is FP32 on mu split into two
+// Statistics are FP64 sums of d = x - x0 and d^2, x0 = the column's first element: var = E[d^2] - E[d]^2 then cancels
+// only as far as x0 lies from the mean (without the shift a column of mean 1e5 and variance 1 lost five
+// digits, and showed it in FP32 outputs).  What follows is FP32 on mu split into two
 // parts, h = ((x - mu1) - mu2) rstd: x and mu1 are exact, so nothing is lost where they cancel, and h is within a few
 // roundings of its own size (all of it in FP64 took twice the registers and, with its conversions, twice
 // the time).  relu's derivative jumps at zero, so there a pre-activation within 2^-20 |beta| of zero, that is,
@@ -105,6 +106,7 @@ __device__ __forceinline__ void sum_x(const NormArgs &p, const T *__restrict__ x
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0;
     if (n <= 0) return;
+    const Pack<T, V> x0 = take<FULL, T, V>(x + col, n);
     each_group<FULL, TY>(r0, r1, ty, [&](int64_t r, auto rows) {
         constexpr int U = decltype(rows)::value;
         Pack<T, V> v[U];
@@ -114,19 +116,19 @@ __device__ __forceinline__ void sum_x(const NormArgs &p, const T *__restrict__ x
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const double d = (double)(float)v[u].v[i];
+                const double d = (double)(float)v[u].v[i] - (double)(float)x0.v[i];
                 s1[i] += d;
                 s2[i] = __builtin_fma(d, d, s2[i]);
             }
     });
 }
 
-// statistics of one column from its sums
-__device__ __forceinline__ void finish_stats(const NormArgs &p, int64_t col, double s1, double s2, double &mu, double &rstd)
+// statistics of one column from its sums and first element
+__device__ __forceinline__ void finish_stats(const NormArgs &p, int64_t col, double s1, double s2, double x0, double &mu, double &rstd)
 {
-    const double m = (double)p.M;
-    mu = s1 / m;
-    const double d = s2 / m - mu * mu;
+    const double m = (double)p.M, e = s1 / m;
+    mu = x0 + e;
+    const double d = s2 / m - e * e;
     const double var = d < 0.0 ? 0.0 : d;                 // NaN stays NaN
     rstd = 1.0 / sqrt(var + p.eps);
     p.stats[col] = mu;
@@ -257,6 +259,7 @@ __global__ __launch_bounds__(THREADS) void stats_kernel(NormArgs p, const T *__r
                 double *o = p.partial + ((int64_t)blockIdx.y * p.N + col + i) * 2;
                 o[0] = s1[i];
                 o[1] = s2[i];
+                if (blockIdx.y == 0) p.stats[col + i] = (double)(float)x[col + i];      // for finish_kernel
             }
     }
 }
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(THREADS) void finish_kernel(NormArgs p)
         }
         if (FORWARD) {
             double mu, rstd;
-            finish_stats(p, col, a, b, mu, rstd);
+            finish_stats(p, col, a, b, p.stats[col], mu, rstd);
         } else {
             p.dbeta[col] = (float)a;
             p.dgamma[col] = (float)b;
@@ -327,7 +330,7 @@ __global__ __launch_bounds__(THREADS) void small_forward_kernel(NormArgs p, cons
         for (int i = 0; i < V; ++i)
             if (i < n) {
                 double mu, rstd;
-                finish_stats(p, col + i, s1[i], s2[i], mu, rstd);
+                finish_stats(p, col + i, s1[i], s2[i], (double)(float)x[col + i], mu, rstd);
                 lds[(tx * V + i) * 2] = mu;
                 lds[(tx * V + i) * 2 + 1] = rstd;
             }
