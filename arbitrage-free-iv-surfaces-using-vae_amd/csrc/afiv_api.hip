@@ -738,7 +738,7 @@ int afiv_norm_act(const void *x, const float *gamma, const float *beta, const ui
     if (bad_layer(dtype, act)) return AFIV_E_ARG;
     if (!(drop_p >= 0.0 && drop_p < 1.0) || (!keep && drop_p != 0.0) || !(eps >= 0.0) || !std::isfinite(momentum)) return AFIV_E_ARG;
     if (M < 2 || bad_sizes(M, N)) return AFIV_E_SHAPE;
-    if (!x || !gamma || !beta || !y || !stats_out || !scratch || !running_mean != !running_var || !codes_out != !scales_out)
+    if (!x || !gamma || !beta || !y || !stats_out || (!scratch && M > AFIV_NORM_SMALL_ROWS) || !running_mean != !running_var || !codes_out != !scales_out)
         return AFIV_E_NULL;
     return afiv_launch_norm_act(x, gamma, beta, keep, dtype, act, M, N, eps, momentum, drop_p, running_mean, running_var, y, stats_out,
                                 codes_out, scales_out, scratch, as_stream(stream));
@@ -751,7 +751,9 @@ int afiv_norm_act_backward(const void *dy, const void *x, const int8_t *codes, c
     if (bad_layer(dtype, act)) return AFIV_E_ARG;
     if (!(drop_p >= 0.0 && drop_p < 1.0) || (!keep && drop_p != 0.0)) return AFIV_E_ARG;
     if (M < 2 || bad_sizes(M, N)) return AFIV_E_SHAPE;
-    if (!dy || (!x && (!codes || !scales)) || !gamma || !beta || !stats || !dgamma || !dbeta || !scratch) return AFIV_E_NULL;
+    if (!dy || (!x && (!codes || !scales)) || !gamma || !beta || !stats || !dgamma || !dbeta ||
+        (!scratch && M > AFIV_NORM_SMALL_ROWS))
+        return AFIV_E_NULL;
     return afiv_launch_norm_act_backward(dy, x, x ? nullptr : codes, x ? nullptr : scales, gamma, beta, keep, stats, dtype, act, M, N,
                                          drop_p, dx, dgamma, dbeta, scratch, as_stream(stream));
 }

@@ -31,10 +31,18 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r)
 template <class T, int N>
 __device__ __forceinline__ Pack<T, N> load_some(const T *p, int n)
 {
-    if (n >= N) return load_pack<T, N>(p);
-    Pack<T, N> r;
+    static_assert(sizeof(T) * N % 4 == 0, "whole words");
+    // joined as words: a branch that yields elements would take them apart, and so wait for its load, before it ends
+    uint32_t w[sizeof(T) * N / 4];
+    if (n >= N) __builtin_memcpy(w, p, sizeof w);
+    else {
+        Pack<T, N> r;
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.v[i] = i < n ? p[i] : T(0);
+        for (int i = 0; i < N; ++i) r.v[i] = i < n ? p[i] : T(0);
+        __builtin_memcpy(w, &r, sizeof w);
+    }
+    Pack<T, N> r;
+    __builtin_memcpy(&r, w, sizeof r);
     return r;
 }
 template <class T, int N>

@@ -964,45 +964,75 @@ __global__ __launch_bounds__(THREADS) void db_kernel(const float *__restrict__ p
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
-// R <= 16 rows of A (stored along l) against 16 rows of B a workgroup: the matrix instruction's 16 columns
-// are the rows of A, its rows those of B, and both operands go from memory to registers 16 bytes a
-// lane.  The workgroup's waves take steps of l in turn and are summed in LDS, wave by wave.
-template <class T, int WAVES>
+// R <= 16 GROUPS rows of A (stored along l) against 16 rows of B a workgroup: the matrix instruction's 16 columns
+// are rows of A, its rows those of B, and both operands go from memory to registers 16 bytes a lane, four
+// steps' loads together (FP32 by its own matrix instruction: memory, not arithmetic, bounds this).  The workgroup's
+// waves take steps of l in turn and are summed in LDS, wave by wave.  Beyond 32 rows A, which every workgroup reads
+// whole, costs as much as B, and the tiles take over.
+template <class T, int WAVES, int GROUPS>
 __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinArgs a)
 {
-    __shared__ float part[WAVES][16][FEW + 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t col0 = (int64_t)blockIdx.x * 16, col = col0 + (lane & 15), row = lane & 15;
-    f32x4 acc = {};
-    constexpr int STEP = 32;
-    const T *pa = (const T *)a.A + row * a.L, *pb = (const T *)a.B + col * a.L;
-    const bool ina = row < a.R, inb = col < a.C;
-#pragma unroll 4
-    for (int64_t l = (int64_t)wave * STEP + (lane >> 4) * 8; l - (lane >> 4) * 8 < a.L; l += WAVES * STEP) {
-        const int n = (int)(a.L - l < 8 ? a.L - l : 8);
-        Pack<T, 8> va = {}, vb = {};
-        if (n > 0 && ina) va = load_some<T, 8>(pa + l, n);
-        if (n > 0 && inb) vb = load_some<T, 8>(pb + l, n);
+    constexpr int STEP = 32, U = 4;
+    __shared__ float part[WAVES][16][16 * GROUPS + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = (lane >> 4) * 8;
+    const int64_t col0 = (int64_t)blockIdx.x * 16, col = col0 + (lane & 15);
+    // lanes beyond the matrices read a row inside: what they multiply is not stored
+    const T *pb = (const T *)a.B + (col < a.C ? col : a.C - 1) * a.L, *pa[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        const int64_t row = g * 16 + (lane & 15);
+        pa[g] = (const T *)a.A + (row < a.R ? row : a.R - 1) * a.L;
+    }
+    f32x4 acc[GROUPS] = {};
+    auto multiply = [&](const Pack<T, 8> &vb, const Pack<T, 8> &va, f32x4 &c) {
         if constexpr (sizeof(T) == 2) {
             typename Mma<T>::frag fa, fb;
             __builtin_memcpy(&fa, &va, 16);
             __builtin_memcpy(&fb, &vb, 16);
-            acc = Mma<T>::mul(fb, fa, acc);
+            c = Mma<T>::mul(fb, fa, c);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(vb.v[i], va.v[i], acc, 0, 0, 0);
+            for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(vb.v[i], va.v[i], c, 0, 0, 0);
+        }
+    };
+    int64_t l = (int64_t)wave * STEP;                          // the same for the wave's lanes
+    for (; l + (U - 1) * WAVES * STEP + STEP <= a.L; l += U * WAVES * STEP) {
+        Pack<T, 8> vb[U], va[U][GROUPS];
+#pragma unroll
+        for (int u = 0; u < U; ++u) vb[u] = load_pack<T, 8>(pb + l + u * WAVES * STEP + sub);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) va[u][g] = load_pack<T, 8>(pa[g] + l + u * WAVES * STEP + sub);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) multiply(vb[u], va[u][g], acc[g]);
+    }
+    for (; l < a.L; l += WAVES * STEP) {
+        const int n = (int)(a.L - l - sub < 8 ? a.L - l - sub : 8);
+        Pack<T, 8> vb = {};
+        if (n > 0) vb = load_some<T, 8>(pb + l + sub, n);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            Pack<T, 8> va = {};
+            if (n > 0) va = load_some<T, 8>(pa[g] + l + sub, n);
+            multiply(vb, va, acc[g]);
         }
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) part[wave][(lane >> 4) * 4 + q][lane & 15] = acc[q];
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) part[wave][(lane >> 4) * 4 + q][g * 16 + (lane & 15)] = acc[g][q];
     __syncthreads();
-    if (tid < 64) {                                            // lane: row = lane & 15, four columns
+    if (wave < GROUPS) {                                       // a wave a group; lane: row = lane & 15, four columns
+        const int64_t row = wave * 16 + (lane & 15), j = col0 + (lane >> 4) * 4;
         float z[4] = {};
+#pragma unroll
         for (int w = 0; w < WAVES; ++w)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) z[q] += part[w][(lane >> 4) * 4 + q][lane & 15];
-        const int64_t j = col0 + (lane >> 4) * 4;
-        if (ina && j < a.C) finish<T, true, 4>(a, row, j, z);
+            for (int q = 0; q < 4; ++q) z[q] += part[w][(lane >> 4) * 4 + q][row];
+        if (row < a.R && j < a.C) finish<T, true, 4>(a, row, j, z);
     }
 }
 
@@ -1085,8 +1115,14 @@ int forward(const LinArgs &a, float *scratch, hipStream_t s)
     if (a.R <= FEW && a.R > 0 && a.C > 0) {
         const dim3 grid((unsigned)((a.C + 15) / 16));
         // 16 waves where the layer has few workgroups to fill the chip with
-        if (grid.x < 512 && a.L >= 512) hipLaunchKernelGGL((few_rows_kernel<T, 16>), grid, dim3(1024), 0, s, a);
-        else hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, dim3(256), 0, s, a);
+        const bool many = grid.x < 512 && a.L >= 512;
+        if (a.R <= 16) {
+            if (many) hipLaunchKernelGGL((few_rows_kernel<T, 16, 1>), grid, dim3(1024), 0, s, a);
+            else hipLaunchKernelGGL((few_rows_kernel<T, 4, 1>), grid, dim3(256), 0, s, a);
+        } else {
+            if (many) hipLaunchKernelGGL((few_rows_kernel<T, 16, 2>), grid, dim3(1024), 0, s, a);
+            else hipLaunchKernelGGL((few_rows_kernel<T, 4, 2>), grid, dim3(256), 0, s, a);
+        }
         return ok();
     }
     const Places p = forward_places(a.R, a.C, a.L, sizeof(T) == 4);

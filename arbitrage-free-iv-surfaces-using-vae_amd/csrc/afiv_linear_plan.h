@@ -10,7 +10,7 @@
 namespace {
 
 constexpr int BK = 32;                    // steps of l in LDS, tile kernel
-constexpr int FEW = 16;                   // rows of the few-rows kernel
+constexpr int FEW = 32;                   // most rows of the few-rows kernel
 
 int64_t tiles_of(int64_t R, int64_t C, int64_t t) { return ((R + t - 1) / t) * ((C + t - 1) / t); }
 

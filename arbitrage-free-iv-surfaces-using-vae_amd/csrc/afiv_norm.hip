@@ -535,9 +535,6 @@ __global__ __launch_bounds__(THREADS, 2) void small_backward_kernel(NormArgs p, 
     else back_rows<false, T, V, TX, EIGHT>(p, x, dy, dx, 0, p.M, col, n, ty, k, mb, mg);
 }
 
-// Rows up to which one launch of N/32 workgroups is taken instead of three.
-constexpr int64_t SMALL_ROWS = 1024;
-
 // row chunks of the chunked kernels: enough workgroups for eight waves a SIMD, at least 16 rows each
 int64_t chunks_for(int64_t M, int64_t col_blocks)
 {
@@ -554,7 +551,7 @@ int forward(NormArgs p, const void *xv, void *yv, hipStream_t s)
 {
     const T *x = (const T *)xv;
     T *y = (T *)yv;
-    if (p.M <= SMALL_ROWS) {
+    if (p.M <= AFIV_NORM_SMALL_ROWS) {
         hipLaunchKernelGGL(small_forward_kernel<T>, dim3((unsigned)((p.N + 31) / 32)), dim3(THREADS), 0, s, p, x, y);
         return ok();
     }
@@ -573,7 +570,7 @@ int backward(NormArgs p, const void *xv, const void *dyv, void *dxv, hipStream_t
 {
     const T *x = (const T *)xv, *dy = (const T *)dyv;
     T *dx = (T *)dxv;
-    if (p.M <= SMALL_ROWS) {
+    if (p.M <= AFIV_NORM_SMALL_ROWS) {
         hipLaunchKernelGGL((small_backward_kernel<T, EIGHT>), dim3((unsigned)((p.N + 31) / 32)), dim3(THREADS), 0, s, p, x, dy, dx);
         return ok();
     }

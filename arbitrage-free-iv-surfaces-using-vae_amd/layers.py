@@ -11,6 +11,7 @@ synchronise.  Inputs that are not contiguous are copied first.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -19,6 +20,7 @@ from . import _lib
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "tanh": 3, "gelu": 4, "silu": 5}
 NORM_SCRATCH_DOUBLES = 2 * 256 + 2      # afiv.h: AFIV_NORM_SCRATCH_DOUBLES, per column
+NORM_SMALL_ROWS = 1024                  # afiv.h: AFIV_NORM_SMALL_ROWS, up to which none is needed
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -147,9 +149,15 @@ class LinearSaved:
         return self.x.dtype if self.eight is None else self.eight.dtype
 
 
-def _scratch(nbytes: int, device) -> torch.Tensor | None:
+@lru_cache(maxsize=4096)
+def _scratch_bytes(query: str, m: int, n: int, k: int, dtype: int) -> int:
+    nbytes = getattr(_lib.lib(), query)(m, n, k, dtype)
     if nbytes < 0:
-        _lib.check(int(nbytes), "afiv_linear_act_scratch")
+        _lib.check(int(nbytes), query)
+    return nbytes
+
+
+def _scratch(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
@@ -167,7 +175,7 @@ def _linear(x, weight, bias, residual, act, want_pre: bool, want_codes: bool):
     y = torch.empty(shape, dtype=v.dtype, device=v.device)
     pre = torch.empty_like(y) if want_pre else None
     dcodes = torch.empty(shape, dtype=torch.uint8, device=v.device) if want_codes else None
-    nbytes = _lib.lib().afiv_linear_act_scratch(m, n, k, DTYPES[v.dtype])
+    nbytes = _scratch_bytes("afiv_linear_act_scratch", m, n, k, DTYPES[v.dtype])
     scratch = _scratch(nbytes, v.device)
     _run("afiv_linear_act", v.device, v.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), DTYPES[v.dtype], code, m, n, k, y.data_ptr(), _ptr(pre),
          _ptr(dcodes), _ptr(scratch), nbytes)
@@ -204,7 +212,7 @@ def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSav
     ran_on = (saved.x if saved.eight is None else saved.eight.codes).device
     if g.device != ran_on:
         raise ValueError(f"dy is on {g.device}, the forward pass ran on {ran_on}")
-    nbytes = _lib.lib().afiv_linear_act_backward_scratch(m, n, k, DTYPES[g.dtype])
+    nbytes = _scratch_bytes("afiv_linear_act_backward_scratch", m, n, k, DTYPES[g.dtype])
     scratch, eight = _scratch(nbytes, g.device), saved.eight
     _run("afiv_linear_act_backward", g.device, g.data_ptr(), _ptr(saved.x), eight and eight.codes.data_ptr(), eight and eight.scales.data_ptr(),
          w.data_ptr(), _ptr(saved.pre), _ptr(saved.dcodes), DTYPES[g.dtype], _act(saved.act), m, n, k, _ptr(dx), _ptr(dw), _ptr(db),
@@ -231,7 +239,11 @@ class _LinearAct(torch.autograd.Function):
 
 
 def _graph(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                return True
+    return False
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
@@ -252,6 +264,12 @@ class NormSaved:
     keep: torch.Tensor | None
     act: str
     drop_p: float
+
+
+def _norm_scratch(m: int, n: int, device) -> torch.Tensor | None:
+    if m <= NORM_SMALL_ROWS:
+        return None
+    return torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=device)
 
 
 def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, running_mean: torch.Tensor | None = None,
@@ -285,13 +303,12 @@ def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     y = torch.empty_like(v)
     stats = torch.empty((2, n), dtype=torch.float64, device=v.device)
     eight = _empty_checkpoint(v) if checkpoint8 else None
-    scratch = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=v.device)
+    scratch = _norm_scratch(m, n, v.device)
     _run("afiv_norm_act", v.device, v.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _ptr(keep), DTYPES[v.dtype], code, m, n, float(eps),
          float(momentum), drop_p, _ptr(running_mean), _ptr(running_var), y.data_ptr(), stats.data_ptr(), eight and eight.codes.data_ptr(),
-         eight and eight.scales.data_ptr(), scratch.data_ptr())
+         eight and eight.scales.data_ptr(), _ptr(scratch))
     if running_mean is not None:         # written behind torch's back: caches keyed on versions must see it
-        torch.autograd.graph.increment_version(running_mean)
-        torch.autograd.graph.increment_version(running_var)
+        torch.autograd.graph.increment_version((running_mean, running_var))
     return y, NormSaved(None if checkpoint8 else v, eight, stats, keep, act, drop_p)
 
 
@@ -309,10 +326,10 @@ def batch_norm_act_backward(dy: torch.Tensor, weight: torch.Tensor, bias: torch.
     gamma, beta = _like(weight, g, (n,), "weight", f32), _like(bias, g, (n,), "bias", f32)
     dx = torch.empty_like(g) if need_dx else None
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
-    scratch, eight = torch.empty(NORM_SCRATCH_DOUBLES * n, dtype=torch.float64, device=g.device), saved.eight
+    scratch, eight = _norm_scratch(m, n, g.device), saved.eight
     _run("afiv_norm_act_backward", g.device, g.data_ptr(), _ptr(saved.x), eight and eight.codes.data_ptr(), eight and eight.scales.data_ptr(),
          gamma.data_ptr(), beta.data_ptr(), _ptr(saved.keep), saved.stats.data_ptr(), DTYPES[g.dtype], _act(saved.act), m, n, saved.drop_p,
-         _ptr(dx), dgamma.data_ptr(), dbeta.data_ptr(), scratch.data_ptr())
+         _ptr(dx), dgamma.data_ptr(), dbeta.data_ptr(), _ptr(scratch))
     return dx, dgamma, dbeta
 
 

@@ -303,7 +303,9 @@ int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes,
  * was), or NULL for no dropout (drop_p = 0 then).  gamma, beta [N] float.  running_mean, running_var: both NULL, or
  * [N] float, updated in place with `momentum` and the unbiased variance.  stats_out: [2,N] doubles,
  * mean and 1/sqrt(var + eps), for the backward pass.  codes_out, scales_out: both NULL, or the 8-bit
- * checkpoint of x.  1 <= N <= 2^24.  scratch: AFIV_NORM_SCRATCH_DOUBLES * N doubles. */
+ * checkpoint of x.  1 <= N <= 2^24.  scratch: AFIV_NORM_SCRATCH_DOUBLES * N doubles; may be
+ * NULL up to AFIV_NORM_SMALL_ROWS rows, in both directions. */
+#define AFIV_NORM_SMALL_ROWS 1024
 #define AFIV_NORM_CHUNKS 256
 #define AFIV_NORM_SCRATCH_DOUBLES (2 * AFIV_NORM_CHUNKS + 2)
 int afiv_norm_act(const void *x, const float *gamma, const float *beta, const uint8_t *keep, int dtype, int act, int64_t M, int64_t N,

@@ -104,7 +104,7 @@ def check_backward(dy, w, saved, act, dx, dw, db):
 
 # one row to thousands; every residue of the tiles; lengths below, at and beyond a step of 32
 SHAPES = [(1, 1, 1), (1, 4096, 64), (2, 7, 3), (16, 33, 17), (17, 32, 16), (5, 1000, 1001), (31, 13, 128), (64, 13, 128), (100, 128, 64),
-          (33, 31, 65), (65, 64, 63), (129, 100, 127), (257, 8, 4), (1000, 77, 5), (3, 5000, 20), (130, 2048, 130), (2049, 257, 513)]
+          (33, 31, 65), (65, 64, 63), (129, 100, 127), (257, 8, 4), (1000, 77, 5), (3, 5000, 20), (130, 2048, 130), (2049, 257, 513), (32, 1056, 40), (24, 530, 9000)]
 
 
 @pytest.mark.parametrize("typ", TYPES)

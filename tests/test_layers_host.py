@@ -84,7 +84,7 @@ def test_norm_refusals(lib):
     assert fwd(keep=p, drop=1.0) == E_ARG and fwd(keep=p, drop=-0.1) == E_ARG and fwd(keep=p, drop=float("nan")) == E_ARG
     assert fwd(eps=-1.0) == E_ARG and fwd(momentum=float("inf")) == E_ARG
     assert fwd(m=1) == E_SHAPE and fwd(m=0) == E_SHAPE and fwd(n=0) == E_SHAPE
-    assert fwd(rm=p) == E_NULL and fwd(codes=p) == E_NULL and fwd(x=None) == E_NULL and fwd(stats=None) == E_NULL and fwd(scratch=None) == E_NULL
+    assert fwd(rm=p) == E_NULL and fwd(codes=p) == E_NULL and fwd(x=None) == E_NULL and fwd(stats=None) == E_NULL and fwd(m=2000, scratch=None) == E_NULL
 
     def bwd(dy=p, x=p, codes=None, scales=None, drop=0.0, m=4, dgamma=p):
         return lib.afiv_norm_act_backward(dy, x, codes, scales, p, p, None, p, 0, 0, m, 4, drop, p, dgamma, p, p, None)
@@ -113,6 +113,7 @@ def test_abi_limits_match_the_wrappers(afiv):
     text = open(os.path.join(os.path.dirname(__file__), "..", "include", "afiv.h")).read()
     chunks = int(re.search(r"#define AFIV_NORM_CHUNKS (\d+)", text).group(1))
     assert afiv.layers.NORM_SCRATCH_DOUBLES == 2 * chunks + 2
+    assert afiv.layers.NORM_SMALL_ROWS == int(re.search(r"#define AFIV_NORM_SMALL_ROWS (\d+)", text).group(1))
     for name, value in afiv.layers.ACTIVATIONS.items():
         assert re.search(r"AFIV_ACT_%s = %d\b" % (name.upper(), value), text)
     for name, value in (("F32", 0), ("BF16", 1), ("F16", 2)):
