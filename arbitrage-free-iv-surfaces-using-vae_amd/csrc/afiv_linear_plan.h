@@ -16,36 +16,39 @@ int64_t tiles_of(int64_t R, int64_t C, int64_t t) { return ((R + t - 1) / t) * (
 
 struct Plan { int64_t tiles, splits, l_per; };
 
-// runs of l: below `want` workgroups the sum is cut, into runs of at least `least` steps
-Plan cut(int64_t tiles, int64_t L, int64_t step, int64_t want, int64_t least)
+// runs of l: with fewer than `few` tiles the sum is cut, for `want` workgroups, into runs of at least `least` steps
+Plan cut(int64_t tiles, int64_t L, int64_t step, int64_t few, int64_t want, int64_t least)
 {
     Plan p = {tiles, 1, 1};
     const int64_t steps = (L + step - 1) / step;
-    if (tiles > 0 && tiles < want / 2 && steps >= 2 * least) p.splits = std::min((want + tiles - 1) / tiles, steps / least);
+    if (tiles > 0 && tiles < few && steps >= 2 * least) p.splits = std::min((want + tiles - 1) / tiles, steps / least);
     p.l_per = std::max<int64_t>(1, (steps + p.splits - 1) / p.splits) * step;
     p.splits = std::max<int64_t>(1, (L + p.l_per - 1) / p.l_per);
     return p;
 }
 
-// Tile and split of a product of R x C outputs and L steps.  128 x 128 tiles once they give every CU
-// one; below that 64 x 64, and below 512 workgroups the sum is cut into runs of at least 256 steps.
-bool big_tiles(int64_t R, int64_t C) { return tiles_of(R, C, 128) >= 256; }
-Plan plan_for(int64_t R, int64_t C, int64_t L) { return cut(tiles_of(R, C, big_tiles(R, C) ? 128 : 64), L, BK, 512, 8); }
+// Tile kernel: 64 x 64 tiles; below 256 workgroups the sum is cut into runs of at least 256 steps.
+Plan plan_for(int64_t R, int64_t C, int64_t L) { return cut(tiles_of(R, C, 64), L, BK, 256, 512, 8); }
 
-// The direct kernel: 256 x 256 tiles where they fill the chip at least once, else 128 x 128 (FP32: always), cut
-// like the above.
+// The direct kernel: 256 x 256 tiles where they fill the chip at least once, else 128 x 128 (FP32: always).  Below 96
+// tiles the sum is cut, for two workgroups a CU (FP32, whose buffers take a CU's LDS: one); above, the kernel
+// that joins the runs costs more than the idle CUs.
 bool huge_tiles(int64_t R, int64_t C) { return tiles_of(R, C, 256) >= 256; }
 Plan direct_plan(int64_t R, int64_t C, int64_t L, bool f32)
 {
-    if (f32) return cut(tiles_of(R, C, 128), L, 32, 512, 8);
-    return huge_tiles(R, C) ? cut(tiles_of(R, C, 256), L, 64, 0, 1) : cut(tiles_of(R, C, 128), L, 64, 512, 8);
+    if (f32) return cut(tiles_of(R, C, 128), L, 32, 96, 256, 8);
+    return huge_tiles(R, C) ? cut(tiles_of(R, C, 256), L, 64, 0, 0, 1) : cut(tiles_of(R, C, 128), L, 64, 96, 512, 8);
 }
 
-// what the direct kernel takes: rows within 2^31 bytes of a tile's corner, and enough work that its tiles are not
-// mostly padding and the operands' preparation is paid back
-bool direct_takes(int64_t R, int64_t C, int64_t L)
+// What the direct kernel takes: at least a tile each way, rows within 2^31 bytes of a tile's corner, and enough work that
+// its few, large tiles fill the chip (16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23 and 12).  FP32
+// operands are always written first, 10 bytes an element, which R C / (R + C) products per element have to pay back
+// (131072 x 512 x 512 backward 1.09 ms and 3.47 ms; 131072 x 128 x 128 0.36 and 0.27).
+bool direct_takes(int64_t R, int64_t C, int64_t L, bool f32)
 {
-    return R >= 128 && C >= 128 && L >= 128 && R * C >= 128 * 128 * 32 && std::max(std::max(R, C), L) <= (int64_t)1 << 36;
+    if (R < 128 || C < 128 || L < 128) return false;
+    const double work = (double)R * (double)C * (double)L;
+    return f32 ? work >= (1 << 28) && R * C >= 192 * (R + C) : work >= (1 << 27);
 }
 bool direct_rows(int64_t len) { return len <= 1 << 21; }
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -67,7 +70,7 @@ int64_t prep_chunks(int64_t rows, int64_t cols)
     return std::max<int64_t>(1, std::min(PREP_CHUNKS, std::min((2048 + cb - 1) / cb, (rows + 15) / 16)));
 }
 struct Room { int64_t at, flags, bytes; };
-struct Places { bool direct; Room x, w, dz; int64_t db, bytes; };
+struct Places { bool direct, direct_dw; Room x, w, dz; int64_t db, bytes; };      // direct: the forward product, or dx's
 
 Room place(int64_t &end, bool wanted, int64_t rows, int64_t cols, bool f32)
 {
@@ -85,7 +88,7 @@ Places forward_places(int64_t M, int64_t N, int64_t K, bool f32)
 {
     Places p = {};
     p.bytes = M <= FEW ? 0 : scratch_floats(M, N, K, f32) * 4;
-    p.direct = M > FEW && direct_takes(M, N, K) && direct_rows(K);
+    p.direct = M > FEW && direct_takes(M, N, K, f32) && direct_rows(K);
     const bool make = p.direct && (f32 || K % 8);
     p.x = place(p.bytes, make, M, K, f32);
     p.w = place(p.bytes, make, N, K, f32);
@@ -96,12 +99,13 @@ Places backward_places(int64_t M, int64_t N, int64_t K, bool f32)
 {
     Places p = {};
     p.bytes = std::max(scratch_floats(M, K, N, f32), scratch_floats(N, K, M, f32)) * 4;
-    p.direct = direct_takes(M, K, N) && direct_takes(N, K, M) && direct_rows(N) && direct_rows(K);
-    p.dz = place(p.bytes, p.direct, M, N, f32);
-    p.x = place(p.bytes, p.direct, M, K, f32);
+    p.direct = direct_takes(M, K, N, f32) && direct_rows(N) && direct_rows(K);
+    p.direct_dw = direct_takes(N, K, M, f32) && direct_rows(N) && direct_rows(K);
+    p.dz = place(p.bytes, p.direct || p.direct_dw, M, N, f32);
+    p.x = place(p.bytes, p.direct_dw, M, K, f32);
     p.w = place(p.bytes, p.direct && (f32 || K % 8), N, K, f32);
     p.db = (p.bytes + 255) / 256 * 256;
-    if (p.direct) p.bytes = p.db + PREP_CHUNKS * N * 4;
+    if (p.direct_dw) p.bytes = p.db + PREP_CHUNKS * N * 4;
     return p;
 }
 

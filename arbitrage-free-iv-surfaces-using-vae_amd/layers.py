@@ -78,6 +78,12 @@ def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = Fals
     return _plain(t)
 
 
+def _held(t, x: torch.Tensor, shape, what: str, dtype=None) -> None:
+    """A saved tensor, if there is one, is what the forward pass made for such an output gradient x."""
+    if t is not None and (t.device != x.device or t.shape != shape or not t.is_contiguous() or (dtype is not None and t.dtype != dtype)):
+        raise ValueError(f"{what} ({t.dtype} {list(t.shape)} on {t.device}) does not belong to dy {list(x.shape)} on {x.device}")
+
+
 def _rows(x: torch.Tensor, what: str) -> int:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what} must be [..., features] with at least one feature, got {list(x.shape)}")
@@ -92,6 +98,14 @@ class Checkpoint8:
     codes: torch.Tensor
     scales: torch.Tensor
     dtype: torch.dtype
+
+    def __post_init__(self):
+        c, s = self.codes, self.scales
+        if c.dtype != torch.int8 or s.dtype != torch.uint8 or self.dtype not in DTYPES:
+            raise TypeError("a checkpoint is int8 codes, uint8 scales and a float32, bfloat16 or float16 dtype")
+        if c.dim() < 1 or c.shape[-1] < 1 or s.shape != c.shape[:-1] + ((c.shape[-1] + 31) // 32,) or c.device != s.device \
+                or not (c.is_contiguous() and s.is_contiguous()):
+            raise ValueError(f"codes {list(c.shape)} and scales {list(s.shape)} are not one contiguous checkpoint")
 
     @property
     def shape(self) -> torch.Size:
@@ -209,9 +223,11 @@ def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSav
     dx = torch.empty(saved.shape, dtype=g.dtype, device=g.device) if need[0] else None
     dw = torch.empty((n, k), dtype=g.dtype, device=g.device) if need[1] else None
     db = torch.empty((n,), dtype=g.dtype, device=g.device) if need[2] else None
-    ran_on = (saved.x if saved.eight is None else saved.eight.codes).device
-    if g.device != ran_on:
-        raise ValueError(f"dy is on {g.device}, the forward pass ran on {ran_on}")
+    _held(saved.x if saved.eight is None else saved.eight.codes, g, saved.shape, "the saved input")
+    if saved.act != "none" and saved.pre is None and saved.dcodes is None:
+        raise ValueError(f"nothing is saved of the derivative of {saved.act}")
+    _held(saved.pre, g, g.shape, "the saved pre-activation", g.dtype)
+    _held(saved.dcodes, g, g.shape, "the saved derivative", torch.uint8)
     nbytes = _scratch_bytes("afiv_linear_act_backward_scratch", m, n, k, DTYPES[g.dtype])
     scratch, eight = _scratch(nbytes, g.device), saved.eight
     _run("afiv_linear_act_backward", g.device, g.data_ptr(), _ptr(saved.x), eight and eight.codes.data_ptr(), eight and eight.scales.data_ptr(),
@@ -318,10 +334,11 @@ def batch_norm_act_backward(dy: torch.Tensor, weight: torch.Tensor, bias: torch.
     held = saved.x if saved.eight is None else saved.eight
     if g.dtype != held.dtype:
         raise TypeError(f"dy must be {held.dtype}, got {g.dtype}")
-    if g.device != saved.stats.device:
-        raise ValueError(f"dy is on {g.device}, the forward pass ran on {saved.stats.device}")
     g = _like(g, g, held.shape, "dy")
     m, n = g.shape
+    _held(saved.x if saved.eight is None else saved.eight.codes, g, g.shape, "the saved input")
+    _held(saved.stats, g, (2, n), "the saved statistics", torch.float64)
+    _held(saved.keep, g, g.shape, "the saved mask")
     f32 = (torch.float32,)
     gamma, beta = _like(weight, g, (n,), "weight", f32), _like(bias, g, (n,), "bias", f32)
     dx = torch.empty_like(g) if need_dx else None

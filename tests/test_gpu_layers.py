@@ -318,6 +318,15 @@ def test_linear_refusals(afiv):
     _, saved = afiv.linear_act_forward(x, w, b, act="tanh")
     bad += [lambda: afiv.linear_act_backward(dy[:5], w, saved), lambda: afiv.linear_act_backward(dy.half(), w.half(), saved),
             lambda: afiv.linear_act_backward(dy, w[:, :4], saved), lambda: afiv.linear_act_backward(dy.cpu(), w, saved)]
+    # saved tensors of another call: another width, another batch, a derivative that is missing
+    import dataclasses
+    other = afiv.linear_act_forward(x, w[:3], b[:3], act="tanh", checkpoint8=True)[1]
+    bad += [lambda: afiv.linear_act_backward(dy, w, other), lambda: afiv.linear_act_backward(dy, w, dataclasses.replace(saved, pre=saved.pre[:5])),
+            lambda: afiv.linear_act_backward(dy, w, dataclasses.replace(saved, pre=None)),
+            lambda: afiv.linear_act_backward(dy, w, dataclasses.replace(saved, pre=saved.pre.half())),
+            lambda: afiv.Checkpoint8(other.eight.codes, other.eight.scales[:5], torch.float32),
+            lambda: afiv.Checkpoint8(other.eight.codes.T, other.eight.scales, torch.float32),
+            lambda: afiv.Checkpoint8(other.eight.codes, other.eight.scales, torch.float64)]
     for call in bad:
         with pytest.raises((ValueError, TypeError)):
             call()
@@ -536,6 +545,9 @@ def test_norm_refusals(afiv):
            lambda: afiv.batch_norm_act(x, gamma.cpu(), beta), lambda: afiv.batch_norm_act(x.double(), gamma, beta)]
     saved = afiv.batch_norm_act_forward(x, gamma, beta)[1]
     bad += [lambda: afiv.batch_norm_act_backward(dy[:4], gamma, beta, saved), lambda: afiv.batch_norm_act_backward(dy.half(), gamma, beta, saved)]
+    import dataclasses
+    bad += [lambda: afiv.batch_norm_act_backward(dy, gamma, beta, dataclasses.replace(saved, stats=saved.stats[:, :5])),
+            lambda: afiv.batch_norm_act_backward(dy, gamma, beta, dataclasses.replace(saved, keep=keep[:4]))]
     for call in bad:
         with pytest.raises((ValueError, TypeError)):
             call()
