@@ -865,14 +865,14 @@ struct PrepArgs {
     const int8_t *codes;
     const uint8_t *scales;
     int act;
-    int64_t rows, cols, ldp, rows_per, plane;
+    int64_t rows, cols, ldp, rows_per, plane, chunks, blocks;      // workgroups: chunks of rows by blocks of 512 columns
     void *out;
     float *partial;
     uint32_t *flags;
 };
 
 template <class T, Made MADE>
-__global__ __launch_bounds__(THREADS) void prepare_kernel(PrepArgs a)
+__device__ __forceinline__ void prepare(const PrepArgs &a)
 {
     typedef typename Part<T>::type P;
     constexpr int PARTS = Mma<T>::PARTS;
@@ -959,7 +959,7 @@ __global__ __launch_bounds__(THREADS) void prepare_kernel(PrepArgs a)
     else with(std::integral_constant<int, AFIV_ACT_NONE>());
     if constexpr (PARTS == 3) {
         const int any = __syncthreads_or(!(amax < 0x1p127f));
-        if (threadIdx.x == 0 && a.flags) a.flags[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = any;
+        if (threadIdx.x == 0 && a.flags) a.flags[(int64_t)blockIdx.y * a.blocks + blockIdx.x] = any;
     }
     if constexpr (MADE == DZ) {
         if (!a.partial) return;
@@ -970,6 +970,20 @@ __global__ __launch_bounds__(THREADS) void prepare_kernel(PrepArgs a)
             if ((int64_t)blockIdx.x * 512 + c < a.cols)
                 a.partial[(int64_t)blockIdx.y * a.cols + (int64_t)blockIdx.x * 512 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
     }
+}
+
+template <class T, Made MADE>
+__global__ __launch_bounds__(THREADS) void prepare_kernel(PrepArgs a)
+{
+    prepare<T, MADE>(a);
+}
+
+// both operands of a forward product in one launch
+template <class T>
+__global__ __launch_bounds__(THREADS) void prepare_two_kernel(PrepArgs a, PrepArgs b)
+{
+    const PrepArgs &p = blockIdx.z == 0 ? a : b;
+    if ((int64_t)blockIdx.x < p.blocks && (int64_t)blockIdx.y < p.chunks) prepare<T, COPY>(p);      // the same for the workgroup
 }
 
 // db from the partial sums: 16 columns a workgroup, 16 threads each over the chunks
@@ -1106,19 +1120,26 @@ int direct(LinArgs a, const Source &sa, const Source &sb, float *scratch, hipStr
     return ok();
 }
 
-// writes an operand to `room`, and says how the direct kernel reads it
-template <class T, Made MADE>
-Source prepared(PrepArgs a, const Room &room, char *scratch, float *partial, bool write, hipStream_t s)
+// how an operand is written to `room`, and how the direct kernel reads it
+template <class T>
+Source placed(PrepArgs &a, const Room &room, char *scratch, float *partial, bool write)
 {
-    const int64_t cb = (a.cols + 511) / 512, chunks = prep_chunks(a.rows, a.cols);
+    a.blocks = (a.cols + 511) / 512;
+    a.chunks = prep_chunks(a.rows, a.cols);
     a.ldp = padded(a.cols);
     a.plane = a.rows * a.ldp;
-    a.rows_per = (a.rows + chunks - 1) / chunks;
+    a.rows_per = (a.rows + a.chunks - 1) / a.chunks;
     a.out = write ? scratch + room.at : nullptr;
     a.partial = partial;
     a.flags = sizeof(T) == 4 ? (uint32_t *)(scratch + room.flags) : nullptr;
-    hipLaunchKernelGGL((prepare_kernel<T, MADE>), dim3((unsigned)cb, (unsigned)chunks), dim3(THREADS), 0, s, a);
-    const Source o = {a.out, a.ldp, a.plane, a.flags, a.rows_per, chunks, cb};
+    const Source o = {a.out, a.ldp, a.plane, a.flags, a.rows_per, a.chunks, a.blocks};
+    return o;
+}
+template <class T, Made MADE>
+Source prepared(PrepArgs a, const Room &room, char *scratch, float *partial, bool write, hipStream_t s)
+{
+    const Source o = placed<T>(a, room, scratch, partial, write);
+    hipLaunchKernelGGL((prepare_kernel<T, MADE>), dim3((unsigned)a.blocks, (unsigned)a.chunks), dim3(THREADS), 0, s, a);
     return o;
 }
 
@@ -1128,13 +1149,16 @@ Source standing(const void *p, int64_t ld)
     const Source o = {p, ld, 0, nullptr, 1, 0, 0};
     return o;
 }
+PrepArgs copy_of(const void *p, int64_t rows, int64_t cols)
+{
+    PrepArgs q = {};
+    q.src = p; q.rows = rows; q.cols = cols;
+    return q;
+}
 template <class T>
 Source plain_source(const void *p, int64_t rows, int64_t cols, const Room &room, char *scratch, hipStream_t s)
 {
-    if (!room.bytes) return standing(p, cols);
-    PrepArgs q = {};
-    q.src = p; q.rows = rows; q.cols = cols;
-    return prepared<T, COPY>(q, room, scratch, nullptr, true, s);
+    return room.bytes ? prepared<T, COPY>(copy_of(p, rows, cols), room, scratch, nullptr, true, s) : standing(p, cols);
 }
 
 template <class T>
@@ -1155,8 +1179,12 @@ int forward(const LinArgs &a, float *scratch, hipStream_t s)
     }
     const Places p = forward_places(a.R, a.C, a.L, sizeof(T) == 4);
     if (p.direct && (p.x.bytes || aligned(a.A)) && (p.w.bytes || aligned(a.B)) && aligned(scratch)) {
+        if (!p.x.bytes) return direct<T, ALONG, ALONG>(a, standing(a.A, a.L), standing(a.B, a.L), scratch, s);
         char *at = (char *)scratch;
-        const Source x = plain_source<T>(a.A, a.R, a.L, p.x, at, s), w = plain_source<T>(a.B, a.C, a.L, p.w, at, s);
+        PrepArgs qx = copy_of(a.A, a.R, a.L), qw = copy_of(a.B, a.C, a.L);
+        const Source x = placed<T>(qx, p.x, at, nullptr, true), w = placed<T>(qw, p.w, at, nullptr, true);
+        hipLaunchKernelGGL(prepare_two_kernel<T>, dim3((unsigned)std::max(qx.blocks, qw.blocks), (unsigned)std::max(qx.chunks, qw.chunks), 2),
+                           dim3(THREADS), 0, s, qx, qw);
         return direct<T, ALONG, ALONG>(a, x, w, scratch, s);
     }
     return product<T, ALONG, ALONG>(a, scratch, s);
