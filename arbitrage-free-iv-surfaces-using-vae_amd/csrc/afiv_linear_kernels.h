@@ -12,13 +12,12 @@
 // their way in.  dz is formed there too (dy, and z or its 8-bit derivative codes), and so is an 8-bit
 // x: neither ever exists in memory.
 //
-// 16-bit types go to v_mfma_f32_16x16x32.  FP32 operands are split into three BF16 parts,
-// a = a1 + a2 + a3 (8 bits each, every difference exact), and the six products a1 b1, a1 b2, a2 b1,
-// a1 b3, a2 b2, a3 b1 are summed in FP32: what is dropped is 2^-26 of the product, a quarter of an FP32
-// rounding, and six BF16 products cost 6/16 of one FP32 matrix instruction's time.  Magnitudes
-// of 2^127 and above (infinities too) do not split; a workgroup that has loaded one does its
-// tile again with FP32 multiply-adds.  Parts below 2^-133 are lost, that is, an element under 2^-110
-// keeps fewer than 24 bits.
+// 16-bit types go to v_mfma_f32_16x16x32.  FP32 operands are cut into three BF16 parts of 8 bits,
+// a = a1 + a2 + a3 exactly (each the upper half of what is left), and the six products a1 b1, a1 b2, a2 b1,
+// a1 b3, a2 b2, a3 b1 are summed in FP32: what is dropped is at most 2^-21 of a product (a2 b3 and a3 b2, 2^-22 each) and
+// 2^-25 in the mean, half an FP32 rounding, and six BF16 products cost 6/16 of one FP32 matrix instruction's time.
+// An infinity does not split (its rest is NaN); a workgroup that has met one does its tile again with FP32
+// multiply-adds.  Parts below 2^-133 are lost, that is, an element under 2^-110 keeps fewer than 24 bits.
 //
 // Few rows (up to 16) take another kernel: W is read once, straight from memory into the matrix
 // instruction, by as many waves as the layer has.
@@ -196,6 +195,23 @@ template <> struct Mma<float> : Mma<__bf16> { static constexpr int PARTS = 3; };
 template <class T> struct Part { typedef T type; };
 template <> struct Part<float> { typedef __bf16 type; };
 
+// The three parts of eight FP32 values, two to a word: the upper halves of a, of a - a1 and of a - a1 - a2
+__device__ __forceinline__ void split8(const float (&a)[8], uint32_t (&p1)[4], uint32_t (&p2)[4], uint32_t (&p3)[4])
+{
+    float b[8], c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        b[i] = a[i] - __uint_as_float(__float_as_uint(a[i]) & 0xffff0000u);
+        c[i] = b[i] - __uint_as_float(__float_as_uint(b[i]) & 0xffff0000u);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        p1[i] = __builtin_amdgcn_perm(__float_as_uint(a[2 * i + 1]), __float_as_uint(a[2 * i]), 0x07060302);
+        p2[i] = __builtin_amdgcn_perm(__float_as_uint(b[2 * i + 1]), __float_as_uint(b[2 * i]), 0x07060302);
+        p3[i] = __builtin_amdgcn_perm(__float_as_uint(c[2 * i + 1]), __float_as_uint(c[2 * i]), 0x07060302);
+    }
+}
+
 // N values to consecutive places of each part's plane
 template <class T, int N>
 __device__ __forceinline__ void put(typename Part<T>::type *lds, int plane, const float (&f)[N])
@@ -207,18 +223,13 @@ __device__ __forceinline__ void put(typename Part<T>::type *lds, int plane, cons
         for (int i = 0; i < N; ++i) o.v[i] = (P)f[i];
         __builtin_memcpy(__builtin_assume_aligned(lds, sizeof o), &o, sizeof o);
     } else {
-        Pack<P, N> o[3];
+        uint32_t o[3][4];
+        float v[8] = {};
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const P a = (P)f[i];
-            const float r = f[i] - (float)a;
-            const P b = (P)r;
-            o[0].v[i] = a;
-            o[1].v[i] = b;
-            o[2].v[i] = (P)(r - (float)b);
-        }
+        for (int i = 0; i < N; ++i) v[i] = f[i];
+        split8(v, o[0], o[1], o[2]);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + p * plane, sizeof o[0]), &o[p], sizeof o[0]);
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + p * plane, 2 * N), o[p], 2 * N);
     }
 }
 
@@ -535,7 +546,7 @@ __global__ __launch_bounds__(THREADS) void tile_kernel(LinArgs a)
     }
 
     if constexpr (PARTS == 3) {
-        if (__syncthreads_or(!(amax < 0x1p127f)))
+        if (__syncthreads_or(!(amax < __builtin_inff())))
             plain_sums<T, KA, KB, TR, TC>(a, acc, row0 + wr, col0 + wc, l_begin, l_end, lane);
     }
 
@@ -611,60 +622,60 @@ __global__ __launch_bounds__(THREADS) void join_kernel(LinArgs a)
 }
 
 // ---- large products -------------------------------------------------------------------------------
-// The same product from operands that go from memory to LDS as they are: 16-bit elements, rows of whole
-// 16-byte chunks.  Operands of that kind are read where they stand; others are written so first, by
-// prepare_kernel: rows of another length, dz, an 8-bit x, and FP32 as its three BF16 parts (a plane each; a
-// fragment of each part is then read once for the six products).
-// Steps of 64 (FP32: 32): a tile's rows are 128 (64) bytes along l, or its steps of l are rows of 2 BR bytes
+// The same product from operands that go from memory to LDS as they are: rows of whole 16-byte chunks.  Operands of that kind are read where they stand; others are written so first, by
+// prepare_kernel: rows of another length, dz, an 8-bit x.
+// Steps of 64 (FP32: 32): a tile's rows are 128 bytes along l, or its steps of l are rows of BR elements
 // (across), and lie in LDS as the loads leave them, 1024 consecutive bytes an instruction; what keeps the
 // reads off each other's banks is therefore a permutation of the global addresses: 16-byte chunk c of row r stands
-// at c ^ (r & 7) (64-byte rows: c ^ ((r >> 1) & 3)), 32-byte block c of step l at c ^ key(l).  Operands across l are
-// transposed by the LDS read itself (ds_read_b64_tr_b16).
+// at c ^ (r & 7), block c of 16 elements of step l at c ^ key(l).  16-bit operands across l are transposed by the LDS
+// read itself (ds_read_b64_tr_b16), FP32 ones are read an element at a time.
 // Two buffers; one barrier a step: the loads of the next step run behind this one's products.
-__device__ __forceinline__ int across_key(int l) { return (l & 3) | ((l >> 1) & 4); }
-
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
-// P: 16-bit element, FK: steps of l, ROWS: rows of the tile, TN: blocks of 16 rows of a wave
-template <class P, bool XS, int FK, int ROWS, int WAVES, int TN>
+// P: element, ROWS: rows of the tile, TN: blocks of 16 rows of a wave
+template <class P, bool XS, int ROWS, int WAVES, int TN>
 struct Direct {
-    typedef typename Mma<P>::frag frag;
-    static constexpr int BYTES = ROWS * FK * 2, PER = BYTES / 1024 / WAVES;      // loads of a wave
+    static constexpr int ES = sizeof(P), FK = 128 / ES;           // steps of l
+    static constexpr int BYTES = ROWS * 128, PER = BYTES / 1024 / WAVES;      // loads of a wave
     static_assert(PER * WAVES * 1024 == BYTES, "whole loads");
-    static constexpr int LSTEP = XS ? 1024 / (2 * ROWS) : 0;      // steps of l from one load of a wave to the next
-    static constexpr int BASES = XS ? TN : FK / 32;
+    static constexpr int LSTEP = XS ? 1024 / (ES * ROWS) : 0;     // steps of l from one load of a wave to the next
+    static constexpr int BASES = XS ? TN : 2;
     uint32_t off[PER];                    // byte offset from the tile's corner; beyond the matrix: out of range
     uint32_t l_first;                     // step of l of the first load
     uint32_t at[BASES];                   // where a lane's reads start
 
-    static __device__ __forceinline__ int chunk_key(int r) { return FK == 64 ? r & 7 : (r >> 1) & 3; }
+    // across: blocks of 16 elements stand at block ^ key(l)
+    static __device__ __forceinline__ int key(int l) { return ES == 2 ? (l & 3) | ((l >> 1) & 4) : (l >> 3) & 3; }
 
     // w0: first of the wave's 16 TN rows
     __device__ __forceinline__ void init(int64_t R, int64_t ld, int64_t row0, int w0, int wave, int lane)
     {
-        constexpr int ROWB = FK * 2, CH = ROWB / 16;              // bytes and chunks of a row along l
+        constexpr int CB = 16 * ES / 16;                          // 16-byte chunks of a block of 16 elements
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int byte = (wave * PER + i) * 1024 + lane * 16;
             if (!XS) {
-                const int r = byte / ROWB, c = (lane & (CH - 1)) ^ chunk_key(lane / CH);
-                off[i] = row0 + r < R ? (uint32_t)(r * ld * 2 + c * 16) : 0x80000000u;
+                const int r = byte / 128, c = (lane & 7) ^ (lane >> 3);
+                off[i] = row0 + r < R ? (uint32_t)(r * ld * ES + c * 16) : 0x80000000u;
             } else {
-                const int l = byte / (2 * ROWS), pos = byte % (2 * ROWS) / 16;
-                const int col = ((pos >> 1) ^ across_key(l)) * 16 + (pos & 1) * 8;
-                off[i] = row0 + col < R ? (uint32_t)((l * ld + col) * 2) : 0x80000000u;
+                const int l = byte / (ES * ROWS), pos = byte % (ES * ROWS) / 16;
+                const int col = ((pos / CB) ^ key(l)) * 16 + pos % CB * (16 / ES);
+                off[i] = row0 + col < R ? (uint32_t)((l * ld + col) * ES) : 0x80000000u;
             }
         }
         if (!XS) {
-            l_first = ((lane & (CH - 1)) ^ chunk_key(lane / CH)) * 8;
+            l_first = ((lane & 7) ^ (lane >> 3)) * (16 / ES);
+            // 16 bit: chunk 4 kk + (lane >> 4) for slice kk; FP32: chunks 2 (lane >> 4) and the next
 #pragma unroll
-            for (int kk = 0; kk < FK / 32; ++kk) at[kk] = (w0 + (lane & 15)) * ROWB + (((kk * 4 + (lane >> 4)) ^ chunk_key(lane & 15)) << 4);
+            for (int k = 0; k < 2; ++k)
+                at[k] = (w0 + (lane & 15)) * 128 + (((ES == 2 ? k * 4 + (lane >> 4) : (lane >> 4) * 2 + k) ^ (lane & 7)) << 4);
         } else {
-            l_first = (wave * PER * 1024 + lane * 16) / (2 * ROWS);
-            // 16 lanes read 4 steps x 16 rows, 8 bytes each, and get 4 steps of a row each
-            const int l = (lane >> 4) * 8 + ((lane >> 2) & 3);
+            l_first = (wave * PER * 1024 + lane * 16) / (ES * ROWS);
+            // 16 bit: 16 lanes read 4 steps x 16 rows, 8 bytes each, and get 4 steps of a row each; FP32: a lane reads its own
+            const int l = ES == 2 ? (lane >> 4) * 8 + ((lane >> 2) & 3) : (lane >> 4) * 8;
 #pragma unroll
-            for (int i = 0; i < TN; ++i) at[i] = l * (2 * ROWS) + ((((w0 >> 4) + i) ^ across_key(l)) << 5) + (lane & 3) * 8;
+            for (int i = 0; i < TN; ++i)
+                at[i] = l * (ES * ROWS) + (((w0 >> 4) + i) ^ key(l)) * (16 * ES) + (ES == 2 ? (lane & 3) * 8 : (lane & 15) * 4);
         }
     }
     __device__ __forceinline__ void load(const P *base, int64_t ld, int64_t row0, int64_t l0, int64_t l_end, char *lds, int wave) const
@@ -679,11 +690,11 @@ struct Direct {
                                                      (int)l_first < left - i * LSTEP ? off[i] : 0x80000000u, 0, 0, 0);
 #endif
     }
-    // rows 16 i + (lane & 15) of the wave's, steps 32 kk + 8 (lane >> 4) ..+7
-    __device__ __forceinline__ frag read(const char *lds, int i, int kk) const
+    // 16 bit: rows 16 i + (lane & 15) of the wave's, steps 32 kk + 8 (lane >> 4) ..+7
+    __device__ __forceinline__ typename Mma<P>::frag read(const char *lds, int i, int kk) const
     {
-        frag f;
-        if constexpr (!XS) f = *(const frag *)(lds + at[kk] + i * (32 * FK));
+        typename Mma<P>::frag f;
+        if constexpr (!XS) f = *(const typename Mma<P>::frag *)(lds + at[kk] + i * 2048);
         else {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             s16x4 h[2];
@@ -694,52 +705,59 @@ struct Direct {
         }
         return f;
     }
-};
-
-// what the direct kernel reads of an operand
-struct Source {
-    const void *p;                        // 16-bit elements, plane after plane
-    int64_t ld, plane;                    // elements from row to row (of l across), and from plane to plane
-    // FP32: words [chunks, blocks]: whether rows_per rows by 512 columns hold values that do not split
-    const uint32_t *flags;
-    int64_t rows_per, chunks, blocks;
-};
-
-// whether a tile of `rows` rows from row0 on has such values in its operand
-template <bool XS>
-__device__ __forceinline__ bool unsplittable(const Source &s, int64_t row0, int rows)
-{
-    const int64_t first = row0 / (XS ? 512 : s.rows_per), most = XS ? s.blocks : s.chunks;
-    const int64_t end = std::min<int64_t>(most, (row0 + rows - 1) / (XS ? 512 : s.rows_per) + 1), other = XS ? s.chunks : s.blocks;
-    uint32_t any = 0;
-    for (int64_t i = threadIdx.x; i < (end - first) * other; i += blockDim.x) {
-        const int64_t a = first + i / other, b = i % other;
-        any |= XS ? s.flags[b * s.blocks + a] : s.flags[a * s.blocks + b];
+    // FP32: the same rows, steps 8 (lane >> 4) ..+7
+    __device__ __forceinline__ void read(const char *lds, int i, float (&f)[8]) const
+    {
+        if constexpr (!XS) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const f32x4 v = *(const f32x4 *)(lds + at[k] + i * 2048);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) f[4 * k + q] = v[q];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = *(const float *)(lds + at[i] + e * (4 * ROWS));
+        }
     }
-    return any != 0;
+};
+
+// what the direct kernels read of an operand
+struct Source {
+    const void *p;
+    int64_t ld;                           // elements from row to row (of l across)
+};
+
+// nothing of memory or LDS moves across; all but this wave's last LEFT loads have arrived and its LDS reads are done
+// (__syncthreads would wait for every load)
+template <int LEFT>
+__device__ __forceinline__ void arrive()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (LEFT & 15) | (LEFT >> 4 << 14));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
 }
 
-// WR x WC waves of 16 TR x 16 TC outputs.  `a` describes the operands as they came, sa and sb as they are read.
-template <class T, Kind KA, Kind KB, int FK, int WR, int WC, int TR, int TC>
+// 16-bit types.  WR x WC waves of 16 TR x 16 TC outputs.
+template <class T, Kind KA, Kind KB, int WR, int WC, int TR, int TC>
 __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source sa, Source sb)
 {
-    constexpr int W = WR * WC, BR = 16 * TR * WR, BC = 16 * TC * WC, PARTS = Mma<T>::PARTS;
-    constexpr bool EPI = KA == ALONG && KB == ALONG;
-    typedef typename Part<T>::type P;
+    constexpr int W = WR * WC, BR = 16 * TR * WR, BC = 16 * TC * WC, FK = 64;
     typedef typename Mma<T>::frag frag;
-    typedef Direct<P, across(KA), FK, BR, W, TR> DA;
-    typedef Direct<P, across(KB), FK, BC, W, TC> DB;
+    typedef Direct<T, across(KA), BR, W, TR> DA;
+    typedef Direct<T, across(KB), BC, W, TC> DB;
     // each buffer an array of its own, named where it is used: the compiler then knows that loads into one do not
     // touch reads of the other, and does not make those wait
-    __shared__ __align__(1024) char a0[PARTS * DA::BYTES];
-    __shared__ __align__(1024) char a1[PARTS * DA::BYTES];
-    __shared__ __align__(1024) char b0[PARTS * DB::BYTES];
-    __shared__ __align__(1024) char b1[PARTS * DB::BYTES];
-    __shared__ __align__(1024) char a2[PARTS == 3 ? PARTS * DA::BYTES : 16];
-    __shared__ __align__(1024) char b2[PARTS == 3 ? PARTS * DB::BYTES : 16];
+    __shared__ __align__(1024) char a0[DA::BYTES];
+    __shared__ __align__(1024) char a1[DA::BYTES];
+    __shared__ __align__(1024) char b0[DB::BYTES];
+    __shared__ __align__(1024) char b1[DB::BYTES];
     // the epilogue's room of a wave: a quarter of the waves share an array
     static_assert(W % 4 == 0 && DA::BYTES == DB::BYTES, "four arrays of one size");
-    constexpr int SLAB = 16 * 16 * TC, FIT = PARTS * DA::BYTES / (W / 4) / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
+    constexpr int SLAB = 16 * 16 * TC, FIT = DA::BYTES / (W / 4) / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = (wave % WR) * 16 * TR, wc = (wave / WR) * 16 * TC;
     int64_t split, tr, tc;
@@ -752,112 +770,165 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
     db.init(a.C, sb.ld, col0, wc, wave, lane);
     f32x4 acc[TR][TC] = {};
 
-    auto load = [&](char *la, char *lb, int64_t l0) {                      // from l_end on: zeros
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            da.load((const P *)sa.p + p * sa.plane, sa.ld, row0, l0, l_end, la + p * DA::BYTES, wave);
-            db.load((const P *)sb.p + p * sb.plane, sb.ld, col0, l0, l_end, lb + p * DB::BYTES, wave);
-        }
+    auto load = [&](char *la, char *lb, int64_t l0) {           // from l_end on: zeros
+        da.load((const T *)sa.p, sa.ld, row0, l0, l_end, la, wave);
+        db.load((const T *)sb.p, sb.ld, col0, l0, l_end, lb, wave);
     };
     // Fragments of one 32-step slice at a time: while row block i of this slice is multiplied, its registers take
     // the next slice's (those of B, shared by the row blocks, have a second set), so the matrix units need not
     // wait for LDS, nor the reads for a barrier that comes once a step.
-    frag fa[PARTS][TR], fb[2][PARTS][TC];
-    auto read_a = [&](const char *s, int i, int kk) {
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) fa[p][i] = da.read(s + p * DA::BYTES, i, kk);
-    };
-    auto read_b = [&](const char *s, int set, int j, int kk) {
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) fb[set][p][j] = db.read(s + p * DB::BYTES, j, kk);
-    };
+    frag fa[TR], fb[2][TC];
     auto slice = [&](int set, const char *na, const char *nb, int next_kk) {
 #pragma unroll
         for (int i = 0; i < TR; ++i) {
 #pragma unroll
-            for (int p = PARTS - 1; p >= 0; --p)                  // small products first
-#pragma unroll
-                for (int q = 0; q <= p; ++q)
-#pragma unroll
-                    for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[set][q][j], fa[p - q][i], acc[i][j]);
-            read_a(na, i, next_kk);
-            if (i < TC) read_b(nb, set ^ 1, i, next_kk);
-            __builtin_amdgcn_sched_group_barrier(0x008, TC * PARTS * (PARTS + 1) / 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, PARTS * (across(KA) ? 2 : 1), 0);
-            if (i < TC) __builtin_amdgcn_sched_group_barrier(0x100, PARTS * (across(KB) ? 2 : 1), 0);
+            for (int j = 0; j < TC; ++j) acc[i][j] = Mma<T>::mul(fb[set][j], fa[i], acc[i][j]);
+            fa[i] = da.read(na, i, next_kk);
+            if (i < TC) fb[set ^ 1][i] = db.read(nb, i, next_kk);
+            __builtin_amdgcn_sched_group_barrier(0x008, TC, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, across(KA) ? 2 : 1, 0);
+            if (i < TC) __builtin_amdgcn_sched_group_barrier(0x100, across(KB) ? 2 : 1, 0);
         }
     };
     static_assert(TC <= TR, "a row block for every column block's reads");
-    // all but this wave's last AHEAD loads have arrived and its reads are done, before any wave reads the next tile or
-    // loads over this one
-    constexpr int LOADS = PARTS * (DA::PER + DB::PER), AHEAD = PARTS == 3 ? LOADS : 0;
-    // (__syncthreads would wait for every load: the bare barrier, with nothing moved across it)
-    auto arrive = [&](auto left) {
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0x0070 | (decltype(left)::value & 15) | (decltype(left)::value >> 4 << 14));
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("" ::: "memory");
-    };
-    auto meet = [&]() { arrive(std::integral_constant<int, AHEAD>()); };
     load(a0, b0, l_begin);
     load(a1, b1, l_begin + FK);
-    if constexpr (PARTS == 3) load(a2, b2, l_begin + 2 * FK);
-    arrive(std::integral_constant<int, 2 * AHEAD>());
+    arrive<0>();
 #pragma unroll
-    for (int i = 0; i < TR; ++i) read_a(a0, i, 0);
+    for (int i = 0; i < TR; ++i) fa[i] = da.read(a0, i, 0);
 #pragma unroll
-    for (int j = 0; j < TC; ++j) read_b(b0, 0, j, 0);
-    // (sched_barrier: loads are issued before the products, not among them)
-    if constexpr (FK == 64) {
+    for (int j = 0; j < TC; ++j) fb[0][j] = db.read(b0, j, 0);
+    // every load of this wave has arrived and its reads are done before any wave reads the next tile or loads over this
+    // one; loads are issued before the products, not among them
 #pragma unroll 1
-        for (int64_t l0 = l_begin; l0 < l_end; l0 += 2 * FK) {  // an odd last step is multiplied with zeros
-            slice(0, a0, b0, 1);
-            meet();
-            load(a0, b0, l0 + 2 * FK);
-            __builtin_amdgcn_sched_barrier(0);
-            slice(1, a1, b1, 0);
-            slice(0, a1, b1, 1);
-            meet();
-            load(a1, b1, l0 + 3 * FK);
-            __builtin_amdgcn_sched_barrier(0);
-            slice(1, a0, b0, 0);
-        }
-    } else {
-        // steps are short here (0.6 us of products), so loads run two steps ahead, in three buffers
-        auto step = [&](int64_t l0, char *la, char *lb, int set, const char *na, const char *nb) {
-            if (l0 < l_end) {
-                meet();
-                load(la, lb, l0 + 3 * FK);
-                __builtin_amdgcn_sched_barrier(0);
-                slice(set, na, nb, 0);
-            }
-        };
-#pragma unroll 1
-        for (int64_t l0 = l_begin; l0 < l_end; l0 += 6 * FK) {
-            step(l0, a0, b0, 0, a1, b1);
-            step(l0 + FK, a1, b1, 1, a2, b2);
-            step(l0 + 2 * FK, a2, b2, 0, a0, b0);
-            step(l0 + 3 * FK, a0, b0, 1, a1, b1);
-            step(l0 + 4 * FK, a1, b1, 0, a2, b2);
-            step(l0 + 5 * FK, a2, b2, 1, a0, b0);
-        }
+    for (int64_t l0 = l_begin; l0 < l_end; l0 += 2 * FK) {      // an odd last step is multiplied with zeros
+        slice(0, a0, b0, 1);
+        arrive<0>();
+        load(a0, b0, l0 + 2 * FK);
+        __builtin_amdgcn_sched_barrier(0);
+        slice(1, a1, b1, 0);
+        slice(0, a1, b1, 1);
+        arrive<0>();
+        load(a1, b1, l0 + 3 * FK);
+        __builtin_amdgcn_sched_barrier(0);
+        slice(1, a0, b0, 0);
     }
     __builtin_amdgcn_s_waitcnt(0x0070);                         // the last loads and reads, before LDS is used again
-    if constexpr (PARTS == 3) {
-        if (__syncthreads_or(unsplittable<across(KA)>(sa, row0, BR) || unsplittable<across(KB)>(sb, col0, BC)))
-            plain_sums<T, KA, KB, TR, TC>(a, acc, row0 + wr, col0 + wc, l_begin, l_end, lane);
-    }
     __syncthreads();
-    write_out<T, EPI, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane,
-                                        (float *)(wave % 4 == 0 ? a0 : wave % 4 == 1 ? a1 : wave % 4 == 2 ? b0 : b1) + wave / 4 * SLABS * SLAB);
+    write_out<T, KA == ALONG && KB == ALONG, TR, TC, SLABS>(a, acc, row0 + wr, col0 + wc, split, lane,
+                                                            (float *)(wave % 4 == 0 ? a0 : wave % 4 == 1 ? a1 : wave % 4 == 2 ? b0 : b1) + wave / 4 * SLABS * SLAB);
 }
 
-// An operand for the direct kernel, [rows, cols] -> [rows, ldp] of 16-bit elements (FP32: three planes of BF16 parts),
-// zeros behind cols.  src: x itself, dy with z or its derivative codes (dz = dy f'(z); with `partial`, also the
-// partial column sums of dz in FP32), or an 8-bit checkpoint.  rows_per rows a workgroup of 64 lanes (8 columns each) by 4
-// rows.  out may be NULL (db alone).  FP32: flags[workgroup] = whether it met a magnitude of 2^127 or more.
+// whether rows row0..row0 + 127 of an operand hold an infinity in l_begin..l_end (the whole workgroup asks)
+template <bool XS>
+__device__ __forceinline__ bool infinities(const Source &s, int64_t R, int64_t row0, int64_t l_begin, int64_t l_end)
+{
+    bool any = false;
+    const int64_t run = XS ? 128 : l_end - l_begin, all = 128 * (l_end - l_begin);
+    for (int64_t i = threadIdx.x; i < all; i += blockDim.x) {
+        const int64_t outer = i / run, inner = i % run, row = row0 + (XS ? inner : outer), l = l_begin + (XS ? outer : inner);
+        if (row < R) any |= fabsf(((const float *)s.p)[XS ? l * s.ld + row : row * s.ld + l]) == __builtin_inff();
+    }
+    return any;
+}
+
+// FP32: 128 x 128 tiles, four waves of 64 x 64, two workgroups a CU.  The operands lie in LDS as they are, 32 steps to a
+// row of 128 bytes, and each wave splits its fragments on the way to the matrix units: 44 vector instructions a fragment
+// beside the 12 matrix instructions it feeds, which the two units of a SIMD run side by side.  (Parts written to memory
+// as three planes first were 10 bytes an element of extra traffic and half again as many through L2: forward and backward
+// of 8192 x 1024 x 512 took 221 us.)  `a` describes the operands as they came, sa and sb as they are read.
+template <Kind KA, Kind KB>
+__global__ __launch_bounds__(256, 2) void direct32_kernel(LinArgs a, Source sa, Source sb)
+{
+    constexpr int TR = 4, TC = 4, FK = 32;
+    typedef Direct<float, across(KA), 128, 4, TR> DA;
+    typedef Direct<float, across(KB), 128, 4, TC> DB;
+    __shared__ __align__(1024) char a0[DA::BYTES];
+    __shared__ __align__(1024) char a1[DA::BYTES];
+    __shared__ __align__(1024) char b0[DB::BYTES];
+    __shared__ __align__(1024) char b1[DB::BYTES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = (wave & 1) * 64, wc = (wave >> 1) * 64;
+    int64_t split, tr, tc;
+    place_tile(a, 128, 128, split, tr, tc);
+    const int64_t row0 = tr * 128, col0 = tc * 128;
+    const int64_t l_begin = split * a.l_per, l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
+    DA da;
+    DB db;
+    da.init(a.R, sa.ld, row0, wr, wave, lane);
+    db.init(a.C, sb.ld, col0, wc, wave, lane);
+    f32x4 acc[TR][TC] = {};
+
+    auto load = [&](char *la, char *lb, int64_t l0) {           // from l_end on: zeros
+        da.load((const float *)sa.p, sa.ld, row0, l0, l_end, la, wave);
+        db.load((const float *)sb.p, sb.ld, col0, l0, l_end, lb, wave);
+    };
+    auto parts = [](const float (&f)[8], bf16x8 (&p)[3]) {
+        uint32_t w[3][4];
+        split8(f, w[0], w[1], w[2]);
+        __builtin_memcpy(p, w, sizeof w);
+    };
+    float fa[TR][8], fb[TC][8];
+    bf16x8 pb[TC][3];
+    // one step of 32: its fragments are in fa and fb, whose registers take the next step's as they are split
+    auto step = [&](const char *na, const char *nb) {
+#pragma unroll
+        for (int j = 0; j < TC; ++j) {
+            parts(fb[j], pb[j]);
+            db.read(nb, j, fb[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < TR; ++i) {
+            bf16x8 pa[3];
+            parts(fa[i], pa);
+            da.read(na, i, fa[i]);
+#pragma unroll
+            for (int p = 2; p >= 0; --p)                          // small products first
+#pragma unroll
+                for (int q = 0; q <= p; ++q)
+#pragma unroll
+                    for (int j = 0; j < TC; ++j) acc[i][j] = Mma<float>::mul(pb[j][q], pa[p - q], acc[i][j]);
+        }
+    };
+    load(a0, b0, l_begin);
+    load(a1, b1, l_begin + FK);
+    arrive<0>();
+#pragma unroll
+    for (int i = 0; i < TR; ++i) da.read(a0, i, fa[i]);
+#pragma unroll
+    for (int j = 0; j < TC; ++j) db.read(b0, j, fb[j]);
+#pragma unroll 1
+    for (int64_t l0 = l_begin; l0 < l_end; l0 += 2 * FK) {
+        arrive<0>();
+        load(a0, b0, l0 + 2 * FK);
+        __builtin_amdgcn_sched_barrier(0);
+        step(a1, b1);
+        arrive<0>();
+        load(a1, b1, l0 + 3 * FK);
+        __builtin_amdgcn_sched_barrier(0);
+        step(a0, b0);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);                         // the last loads and reads, before LDS is used again
+    // an infinity's parts are infinity and NaN: a tile with NaNs is looked over for infinities
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < TR; ++i)
+#pragma unroll
+        for (int j = 0; j < TC; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) nan |= acc[i][j][q] != acc[i][j][q];
+    if (__syncthreads_or(nan)) {
+        const bool any = infinities<across(KA)>(sa, a.R, row0, l_begin, l_end) || infinities<across(KB)>(sb, a.C, col0, l_begin, l_end);
+        if (__syncthreads_or(any)) plain_sums<float, KA, KB, TR, TC>(a, acc, row0 + wr, col0 + wc, l_begin, l_end, lane);
+    }
+    __syncthreads();
+    write_out<float, KA == ALONG && KB == ALONG, TR, TC, 4>(a, acc, row0 + wr, col0 + wc, split, lane,
+                                                            (float *)(wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1));
+}
+
+// An operand for the direct kernels, [rows, cols] -> [rows, ldp], zeros behind cols.  src: x itself, dy with z or its
+// derivative codes (dz = dy f'(z); with `partial`, also the partial column sums of dz in FP32), or an 8-bit checkpoint.
+// rows_per rows a workgroup of 64 lanes (8 columns each) by 4 rows.  out may be NULL (db alone).
 enum Made { COPY, DZ, EIGHT };
 struct PrepArgs {
     const void *src, *pre;
@@ -865,23 +936,20 @@ struct PrepArgs {
     const int8_t *codes;
     const uint8_t *scales;
     int act;
-    int64_t rows, cols, ldp, rows_per, plane, chunks, blocks;      // workgroups: chunks of rows by blocks of 512 columns
+    int64_t rows, cols, ldp, rows_per, chunks, blocks;      // workgroups: chunks of rows by blocks of 512 columns
     void *out;
     float *partial;
-    uint32_t *flags;
 };
 
 template <class T, Made MADE>
 __device__ __forceinline__ void prepare(const PrepArgs &a)
 {
-    typedef typename Part<T>::type P;
-    constexpr int PARTS = Mma<T>::PARTS;
     __shared__ float lds[MADE == DZ ? 4 : 1][512];
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const int64_t col = ((int64_t)blockIdx.x * 64 + tx) * 8;
     const int n = (int)(a.cols - col < 8 ? a.cols - col : 8);
     const int64_t r0 = (int64_t)blockIdx.y * a.rows_per, r1 = r0 + a.rows_per < a.rows ? r0 + a.rows_per : a.rows;
-    float sum[8] = {}, amax = 0.0f;
+    float sum[8] = {};
     auto rows = [&](auto full, auto act) {
         constexpr bool FULL = decltype(full)::value;
         constexpr int ACT = decltype(act)::value, U = FULL ? 4 : 1;
@@ -924,30 +992,12 @@ __device__ __forceinline__ void prepare(const PrepArgs &a)
                     }
                     if (!FULL && i >= n) f[i] = 0.0f;
                     if constexpr (MADE == DZ) sum[i] += f[i];
-                    if constexpr (PARTS == 3) amax = fmaxf(amax, fabsf(f[i]));        // NaN splits into NaNs
                 }
                 if (MADE == DZ && !a.out) continue;
-                P *o = (P *)a.out + (r + 4 * u) * a.ldp + col;
-                if constexpr (PARTS == 3) {
-                    float w[8];
+                Pack<T, 8> b;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = f[i];
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        Pack<P, 8> b;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            b.v[i] = (P)w[i];
-                            w[i] -= (float)b.v[i];
-                        }
-                        store_pack<P, 8>(o + p * a.plane, b);
-                    }
-                } else {
-                    Pack<P, 8> b;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) b.v[i] = (P)f[i];
-                    store_pack<P, 8>(o, b);
-                }
+                for (int i = 0; i < 8; ++i) b.v[i] = (T)f[i];
+                store_pack<T, 8>((T *)a.out + (r + 4 * u) * a.ldp + col, b);
             }
         }
     };
@@ -957,10 +1007,6 @@ __device__ __forceinline__ void prepare(const PrepArgs &a)
     };
     if constexpr (MADE == DZ) with_act(a.act, with);
     else with(std::integral_constant<int, AFIV_ACT_NONE>());
-    if constexpr (PARTS == 3) {
-        const int any = __syncthreads_or(!(amax < 0x1p127f));
-        if (threadIdx.x == 0 && a.flags) a.flags[(int64_t)blockIdx.y * a.blocks + blockIdx.x] = any;
-    }
     if constexpr (MADE == DZ) {
         if (!a.partial) return;
 #pragma unroll
@@ -1113,9 +1159,9 @@ int direct(LinArgs a, const Source &sa, const Source &sb, float *scratch, hipStr
     a.partial = scratch;
     a.db = nullptr;
     const dim3 grid((unsigned)(p.tiles * p.splits));
-    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 32, 2, 4, 4, 2>), grid, dim3(512), 0, s, a, sa, sb);
-    else if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 64, 2, 4, 8, 4>), grid, dim3(512), 0, s, a, sa, sb);
-    else hipLaunchKernelGGL((direct_kernel<T, KA, KB, 64, 2, 2, 4, 4>), grid, dim3(256), 0, s, a, sa, sb);
+    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((direct32_kernel<KA, KB>), grid, dim3(256), 0, s, a, sa, sb);
+    else if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 8, 4>), grid, dim3(512), 0, s, a, sa, sb);
+    else hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 2, 4, 4>), grid, dim3(256), 0, s, a, sa, sb);
     if (p.splits > 1) join<T, KA == ALONG && KB == ALONG>(a, s);
     return ok();
 }
@@ -1127,12 +1173,10 @@ Source placed(PrepArgs &a, const Room &room, char *scratch, float *partial, bool
     a.blocks = (a.cols + 511) / 512;
     a.chunks = prep_chunks(a.rows, a.cols);
     a.ldp = padded(a.cols);
-    a.plane = a.rows * a.ldp;
     a.rows_per = (a.rows + a.chunks - 1) / a.chunks;
     a.out = write ? scratch + room.at : nullptr;
     a.partial = partial;
-    a.flags = sizeof(T) == 4 ? (uint32_t *)(scratch + room.flags) : nullptr;
-    const Source o = {a.out, a.ldp, a.plane, a.flags, a.rows_per, a.chunks, a.blocks};
+    const Source o = {a.out, a.ldp};
     return o;
 }
 template <class T, Made MADE>
@@ -1146,7 +1190,7 @@ Source prepared(PrepArgs a, const Room &room, char *scratch, float *partial, boo
 // an operand that may be read where it stands
 Source standing(const void *p, int64_t ld)
 {
-    const Source o = {p, ld, 0, nullptr, 1, 0, 0};
+    const Source o = {p, ld};
     return o;
 }
 PrepArgs copy_of(const void *p, int64_t rows, int64_t cols)
@@ -1206,9 +1250,10 @@ int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *
 
     // operands that the direct kernel cannot read in place are written first; a misaligned one of a kind that it
     // could sends the product to the tile kernel
+    constexpr int WHOLE = 16 / sizeof(T);
     const Places p = backward_places(M, N, K, sizeof(T) == 4);
     char *const at = (char *)scratch;
-    const bool make_dz = sizeof(T) == 4 || act != AFIV_ACT_NONE || N % 8, make_x = codes || sizeof(T) == 4 || K % 8;
+    const bool make_dz = act != AFIV_ACT_NONE || N % WHOLE, make_x = codes || K % WHOLE;
     const bool ready = aligned(scratch) && (make_dz || aligned(dy));
     const bool direct_dx = dx && p.direct && ready && (p.w.bytes || aligned(w));
     const bool direct_dw = dw && p.direct_dw && ready && (make_x || aligned(x));

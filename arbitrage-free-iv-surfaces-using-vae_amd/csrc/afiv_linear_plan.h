@@ -31,26 +31,21 @@ Plan cut(int64_t tiles, int64_t L, int64_t step, int64_t few, int64_t want, int6
 Plan plan_for(int64_t R, int64_t C, int64_t L) { return cut(tiles_of(R, C, 64), L, BK, 256, 512, 8); }
 
 // The direct kernel: 256 x 256 tiles where they fill the chip at least once, else 128 x 128 (FP32: always).  Below 96
-// tiles the sum is cut, for two workgroups a CU (FP32, whose buffers take a CU's LDS: one); above, the kernel
-// that joins the runs costs more than the idle CUs.
+// tiles the sum is cut, for two workgroups a CU; above, the kernel that joins the runs costs more than the idle CUs.
 bool huge_tiles(int64_t R, int64_t C) { return tiles_of(R, C, 256) >= 256; }
 Plan direct_plan(int64_t R, int64_t C, int64_t L, bool f32)
 {
-    if (f32) return cut(tiles_of(R, C, 128), L, 32, 96, 256, 8);
+    if (f32) return cut(tiles_of(R, C, 128), L, 32, 96, 512, 8);
     return huge_tiles(R, C) ? cut(tiles_of(R, C, 256), L, 64, 0, 0, 1) : cut(tiles_of(R, C, 128), L, 64, 96, 512, 8);
 }
 
 // What the direct kernel takes: at least a tile each way, rows within 2^31 bytes of a tile's corner, and enough work that
-// its few, large tiles fill the chip (16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23 and 12).  FP32
-// operands are always written first, 10 bytes an element, which R C / (R + C) products per element have to pay back
-// (131072 x 512 x 512 backward 1.09 ms and 3.47 ms; 131072 x 128 x 128 0.36 and 0.27).
-bool direct_takes(int64_t R, int64_t C, int64_t L, bool f32)
+// its few, large tiles fill the chip (16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23 and 12).
+bool direct_takes(int64_t R, int64_t C, int64_t L)
 {
-    if (R < 128 || C < 128 || L < 128) return false;
-    const double work = (double)R * (double)C * (double)L;
-    return f32 ? work >= (1 << 28) && R * C >= 192 * (R + C) : work >= (1 << 27);
+    return R >= 128 && C >= 128 && L >= 128 && (double)R * (double)C * (double)L >= (1 << 27);
 }
-bool direct_rows(int64_t len) { return len <= 1 << 21; }
+bool direct_rows(int64_t len) { return len <= 1 << 20; }
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // floats that either kernel's split takes
@@ -60,8 +55,7 @@ int64_t scratch_floats(int64_t R, int64_t C, int64_t L, bool f32)
     return std::max(p.splits > 1 ? p.splits * (R * C + R) : 0, d.splits > 1 ? d.splits * R * C : 0);
 }
 
-// Scratch of a call: the splits' floats, then the operands written for the direct kernel, each with its flag words
-// (FP32), then the partial sums of db.
+// Scratch of a call: the splits' floats, then the operands written for the direct kernel, then the partial sums of db.
 int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
 constexpr int64_t PREP_CHUNKS = 256;
 int64_t prep_chunks(int64_t rows, int64_t cols)
@@ -69,18 +63,16 @@ int64_t prep_chunks(int64_t rows, int64_t cols)
     const int64_t cb = (cols + 511) / 512;
     return std::max<int64_t>(1, std::min(PREP_CHUNKS, std::min((2048 + cb - 1) / cb, (rows + 15) / 16)));
 }
-struct Room { int64_t at, flags, bytes; };
+struct Room { int64_t at, bytes; };
 struct Places { bool direct, direct_dw; Room x, w, dz; int64_t db, bytes; };      // direct: the forward product, or dx's
 
 Room place(int64_t &end, bool wanted, int64_t rows, int64_t cols, bool f32)
 {
-    Room r = {0, 0, 0};
+    Room r = {0, 0};
     if (!wanted) return r;
-    auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
-    r.at = up(end);
-    r.flags = up(r.at + rows * padded(cols) * (f32 ? 6 : 2));
-    end = r.flags + (f32 ? (cols + 511) / 512 * prep_chunks(rows, cols) * 4 : 0);
-    r.bytes = end - r.at;
+    r.at = (end + 255) / 256 * 256;
+    r.bytes = rows * padded(cols) * (f32 ? 4 : 2);
+    end = r.at + r.bytes;
     return r;
 }
 
@@ -88,8 +80,8 @@ Places forward_places(int64_t M, int64_t N, int64_t K, bool f32)
 {
     Places p = {};
     p.bytes = M <= FEW ? 0 : scratch_floats(M, N, K, f32) * 4;
-    p.direct = M > FEW && direct_takes(M, N, K, f32) && direct_rows(K);
-    const bool make = p.direct && (f32 || K % 8);
+    p.direct = M > FEW && direct_takes(M, N, K) && direct_rows(K);
+    const bool make = p.direct && K % (f32 ? 4 : 8);
     p.x = place(p.bytes, make, M, K, f32);
     p.w = place(p.bytes, make, N, K, f32);
     return p;
@@ -99,11 +91,11 @@ Places backward_places(int64_t M, int64_t N, int64_t K, bool f32)
 {
     Places p = {};
     p.bytes = std::max(scratch_floats(M, K, N, f32), scratch_floats(N, K, M, f32)) * 4;
-    p.direct = direct_takes(M, K, N, f32) && direct_rows(N) && direct_rows(K);
-    p.direct_dw = direct_takes(N, K, M, f32) && direct_rows(N) && direct_rows(K);
+    p.direct = direct_takes(M, K, N) && direct_rows(N) && direct_rows(K);
+    p.direct_dw = direct_takes(N, K, M) && direct_rows(N) && direct_rows(K);
     p.dz = place(p.bytes, p.direct || p.direct_dw, M, N, f32);
     p.x = place(p.bytes, p.direct_dw, M, K, f32);
-    p.w = place(p.bytes, p.direct && (f32 || K % 8), N, K, f32);
+    p.w = place(p.bytes, p.direct && K % (f32 ? 4 : 8), N, K, f32);
     p.db = (p.bytes + 255) / 256 * 256;
     if (p.direct_dw) p.bytes = p.db + PREP_CHUNKS * N * 4;
     return p;
