@@ -870,24 +870,39 @@ __global__ __launch_bounds__(256, 2) void direct32_kernel(LinArgs a, Source sa, 
     };
     float fa[TR][8], fb[TC][8];
     bf16x8 pb[TC][3];
-    // one step of 32: its fragments are in fa and fb, whose registers take the next step's as they are split
+    // One step of 32: its fragments are in fa and fb, whose registers take the next step's as they are split.  The split of
+    // row block i + 1 stands among the products of block i.
     auto step = [&](const char *na, const char *nb) {
+        constexpr int READS_A = across(KA) ? 8 : 2, READS_B = across(KB) ? 8 : 2;
 #pragma unroll
         for (int j = 0; j < TC; ++j) {
             parts(fb[j], pb[j]);
             db.read(nb, j, fb[j]);
+            __builtin_amdgcn_sched_group_barrier(0x002, 44, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, READS_B, 0);
         }
+        bf16x8 pa[2][3];
+        parts(fa[0], pa[0]);
+        da.read(na, 0, fa[0]);
+        __builtin_amdgcn_sched_group_barrier(0x002, 44, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS_A, 0);
 #pragma unroll
         for (int i = 0; i < TR; ++i) {
-            bf16x8 pa[3];
-            parts(fa[i], pa);
-            da.read(na, i, fa[i]);
+            if (i + 1 < TR) {
+                parts(fa[i + 1], pa[(i + 1) & 1]);
+                da.read(na, i + 1, fa[i + 1]);
+            }
 #pragma unroll
             for (int p = 2; p >= 0; --p)                          // small products first
 #pragma unroll
                 for (int q = 0; q <= p; ++q)
 #pragma unroll
-                    for (int j = 0; j < TC; ++j) acc[i][j] = Mma<float>::mul(pb[j][q], pa[p - q], acc[i][j]);
+                    for (int j = 0; j < TC; ++j) {
+                        acc[i][j] = Mma<float>::mul(pb[j][q], pa[i & 1][p - q], acc[i][j]);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        if (i + 1 < TR) __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+                    }
+            if (i + 1 < TR) __builtin_amdgcn_sched_group_barrier(0x100, READS_A, 0);
         }
     };
     load(a0, b0, l_begin);

@@ -40,10 +40,11 @@ Plan direct_plan(int64_t R, int64_t C, int64_t L, bool f32)
 }
 
 // What the direct kernel takes: at least a tile each way, rows within 2^31 bytes of a tile's corner, and enough work that
-// its few, large tiles fill the chip (16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23 and 12).
-bool direct_takes(int64_t R, int64_t C, int64_t L)
+// its few, large tiles fill the chip (16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23 and 12; FP32:
+// 512^3 24 and 16, 4096 x 256 x 256 25 and 29).
+bool direct_takes(int64_t R, int64_t C, int64_t L, bool f32)
 {
-    return R >= 128 && C >= 128 && L >= 128 && (double)R * (double)C * (double)L >= (1 << 27);
+    return R >= 128 && C >= 128 && L >= 128 && (double)R * (double)C * (double)L >= (f32 ? 1 << 28 : 1 << 27);
 }
 bool direct_rows(int64_t len) { return len <= 1 << 20; }
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -80,7 +81,7 @@ Places forward_places(int64_t M, int64_t N, int64_t K, bool f32)
 {
     Places p = {};
     p.bytes = M <= FEW ? 0 : scratch_floats(M, N, K, f32) * 4;
-    p.direct = M > FEW && direct_takes(M, N, K) && direct_rows(K);
+    p.direct = M > FEW && direct_takes(M, N, K, f32) && direct_rows(K);
     const bool make = p.direct && K % (f32 ? 4 : 8);
     p.x = place(p.bytes, make, M, K, f32);
     p.w = place(p.bytes, make, N, K, f32);
@@ -91,8 +92,8 @@ Places backward_places(int64_t M, int64_t N, int64_t K, bool f32)
 {
     Places p = {};
     p.bytes = std::max(scratch_floats(M, K, N, f32), scratch_floats(N, K, M, f32)) * 4;
-    p.direct = direct_takes(M, K, N) && direct_rows(N) && direct_rows(K);
-    p.direct_dw = direct_takes(N, K, M) && direct_rows(N) && direct_rows(K);
+    p.direct = direct_takes(M, K, N, f32) && direct_rows(N) && direct_rows(K);
+    p.direct_dw = direct_takes(N, K, M, f32) && direct_rows(N) && direct_rows(K);
     p.dz = place(p.bytes, p.direct || p.direct_dw, M, N, f32);
     p.x = place(p.bytes, p.direct_dw, M, K, f32);
     p.w = place(p.bytes, p.direct && K % (f32 ? 4 : 8), N, K, f32);
