@@ -645,7 +645,7 @@ struct Direct {
     uint32_t at[BASES];                   // where a lane's reads start
 
     // across: blocks of 16 elements stand at block ^ key(l)
-    static __device__ __forceinline__ int key(int l) { return ES == 2 ? (l & 3) | ((l >> 1) & 4) : (l >> 3) & 3; }
+    static __device__ __forceinline__ int key(int l) { return ES == 2 ? (l & 3) | ((l >> 1) & 4) : (l >> 2) & 3; }
 
     // w0: first of the wave's 16 TN rows
     __device__ __forceinline__ void init(int64_t R, int64_t ld, int64_t row0, int w0, int wave, int lane)
@@ -665,14 +665,13 @@ struct Direct {
         }
         if (!XS) {
             l_first = ((lane & 7) ^ (lane >> 3)) * (16 / ES);
-            // 16 bit: chunk 4 kk + (lane >> 4) for slice kk; FP32: chunks 2 (lane >> 4) and the next
+            // chunks (lane >> 4) and 4 + (lane >> 4): a slice each in 16 bit, together one fragment in FP32
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-                at[k] = (w0 + (lane & 15)) * 128 + (((ES == 2 ? k * 4 + (lane >> 4) : (lane >> 4) * 2 + k) ^ (lane & 7)) << 4);
+            for (int k = 0; k < 2; ++k) at[k] = (w0 + (lane & 15)) * 128 + (((k * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
         } else {
             l_first = (wave * PER * 1024 + lane * 16) / (ES * ROWS);
             // 16 bit: 16 lanes read 4 steps x 16 rows, 8 bytes each, and get 4 steps of a row each; FP32: a lane reads its own
-            const int l = ES == 2 ? (lane >> 4) * 8 + ((lane >> 2) & 3) : (lane >> 4) * 8;
+            const int l = ES == 2 ? (lane >> 4) * 8 + ((lane >> 2) & 3) : (lane >> 4) * 4;
 #pragma unroll
             for (int i = 0; i < TN; ++i)
                 at[i] = l * (ES * ROWS) + (((w0 >> 4) + i) ^ key(l)) * (16 * ES) + (ES == 2 ? (lane & 3) * 8 : (lane & 15) * 4);
@@ -705,7 +704,8 @@ struct Direct {
         }
         return f;
     }
-    // FP32: the same rows, steps 8 (lane >> 4) ..+7
+    // FP32: the same rows, steps 4 (lane >> 4) ..+3 and 16 + 4 (lane >> 4) ..+3: any order of the steps will do that both
+    // operands share, and this one reads the chunks that 16-bit fragments do
     __device__ __forceinline__ void read(const char *lds, int i, float (&f)[8]) const
     {
         if constexpr (!XS) {
@@ -717,7 +717,7 @@ struct Direct {
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = *(const float *)(lds + at[i] + e * (4 * ROWS));
+            for (int e = 0; e < 8; ++e) f[e] = *(const float *)(lds + at[i] + (e < 4 ? e : 12 + e) * (4 * ROWS));
         }
     }
 };
