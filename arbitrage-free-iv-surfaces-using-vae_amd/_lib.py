@@ -62,7 +62,7 @@ SIGNATURES = {
     "afiv_checkpoint8_restore": (c_int, [c_void_p, c_void_p, c_int, c_i64, c_i64, c_void_p, c_void_p]),
     "afiv_linear_act_scratch": (c_i64, [c_i64, c_i64, c_i64, c_int]),
     "afiv_linear_act": (c_int, [c_void_p] * 4 + [c_int, c_int, c_i64, c_i64, c_i64] + [c_void_p] * 4 + [c_i64, c_void_p]),
-    "afiv_linear_act_backward_scratch": (c_i64, [c_i64, c_i64, c_i64, c_int]),
+    "afiv_linear_act_backward_scratch": (c_i64, [c_i64, c_i64, c_i64, c_int, c_int, c_int]),
     "afiv_linear_act_backward": (c_int, [c_void_p] * 7 + [c_int, c_int, c_i64, c_i64, c_i64] + [c_void_p] * 4 + [c_i64, c_void_p]),
     "afiv_norm_act": (c_int, [c_void_p] * 4 + [c_int, c_int, c_i64, c_i64, c_double, c_double, c_double] + [c_void_p] * 8),
     "afiv_norm_act_backward": (c_int, [c_void_p] * 8 + [c_int, c_int, c_i64, c_i64, c_double] + [c_void_p] * 5),

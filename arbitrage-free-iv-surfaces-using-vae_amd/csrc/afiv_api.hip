@@ -662,10 +662,10 @@ static bool bad_layer(int dtype, int act)
 static const int64_t MAX_WIDTH = (int64_t)1 << 24, MAX_ROWS = (int64_t)1 << 36;
 
 // rows and columns whose element offsets stay in range; a launch has fewer than 2^32 work items, so the
-// 128 x 128 tiles of 256 threads number less than 2^24
+// 64 x 64 tiles of 256 threads number less than 2^24
 static bool bad_sizes(int64_t rows, int64_t cols)
 {
-    return rows < 0 || rows > MAX_ROWS || cols < 1 || cols > MAX_WIDTH || (rows + 127) / 128 * ((cols + 127) / 128) >= (1 << 24);
+    return rows < 0 || rows > MAX_ROWS || cols < 1 || cols > MAX_WIDTH || (rows + 63) / 64 * ((cols + 63) / 64) >= (1 << 24);
 }
 
 int afiv_checkpoint8_pack(const void *x, int dtype, int64_t rows, int64_t cols, int8_t *codes, uint8_t *scales, void *stream)
@@ -697,10 +697,10 @@ int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K, int dtype)
     return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_forward_scratch(M, N, K, dtype);
 }
 
-int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype)
+int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype, int act, int from_checkpoint)
 {
-    if (bad_layer(dtype, 0)) return AFIV_E_ARG;
-    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_backward_scratch(M, N, K, dtype);
+    if (bad_layer(dtype, act)) return AFIV_E_ARG;
+    return bad_linear(M, N, K) ? AFIV_E_SHAPE : afiv_linear_backward_scratch(M, N, K, dtype, act, from_checkpoint != 0);
 }
 
 int afiv_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
@@ -725,7 +725,7 @@ int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes,
         if (!dy || (dx && !w) || (dw && !x && (!codes || !scales))) return AFIV_E_NULL;
         if (act != AFIV_ACT_NONE && !pre && !dcodes) return AFIV_E_NULL;
     }
-    const int64_t need = afiv_linear_backward_scratch(M, N, K, dtype);
+    const int64_t need = afiv_linear_backward_scratch(M, N, K, dtype, act, !x);
     if (need > 0 && (!scratch || scratch_bytes < need)) return AFIV_E_WORKSPACE;
     return afiv_launch_linear_act_backward(dy, x, x ? nullptr : codes, x ? nullptr : scales, w, pre, pre ? nullptr : dcodes, dtype, act, M,
                                            N, K, dx, dw, db, (float *)scratch, as_stream(stream));

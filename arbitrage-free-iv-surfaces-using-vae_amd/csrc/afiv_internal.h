@@ -131,7 +131,7 @@ int afiv_launch_checkpoint8_pack(const void *x, int dtype, int64_t rows, int64_t
 int afiv_launch_checkpoint8_restore(const int8_t *codes, const uint8_t *scales, int dtype, int64_t rows, int64_t cols, void *x,
                                     hipStream_t s);
 int64_t afiv_linear_forward_scratch(int64_t M, int64_t N, int64_t K, int dtype);      // bytes
-int64_t afiv_linear_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype);
+int64_t afiv_linear_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype, int act, bool from_checkpoint);
 int afiv_launch_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
                            int64_t K, void *y, void *pre, uint8_t *dcodes, float *scratch, hipStream_t s);
 int afiv_launch_linear_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w,

@@ -12,7 +12,10 @@ DECLARE(bf16)
 DECLARE(f16)
 
 int64_t afiv_linear_forward_scratch(int64_t M, int64_t N, int64_t K, int dtype) { return forward_places(M, N, K, dtype == AFIV_F32).bytes; }
-int64_t afiv_linear_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype) { return backward_places(M, N, K, dtype == AFIV_F32).bytes; }
+int64_t afiv_linear_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype, int act, bool from_checkpoint)
+{
+    return backward_places(M, N, K, dtype == AFIV_F32, act != AFIV_ACT_NONE, from_checkpoint).bytes;
+}
 
 int afiv_launch_linear_act(const void *x, const void *w, const void *bias, const void *residual, int dtype, int act, int64_t M, int64_t N,
                            int64_t K, void *y, void *pre, uint8_t *dcodes, float *scratch, hipStream_t s)

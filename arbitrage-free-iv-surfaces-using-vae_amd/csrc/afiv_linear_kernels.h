@@ -1266,7 +1266,7 @@ int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *
     // operands that the direct kernel cannot read in place are written first; a misaligned one of a kind that it
     // could sends the product to the tile kernel
     constexpr int WHOLE = 16 / sizeof(T);
-    const Places p = backward_places(M, N, K, sizeof(T) == 4);
+    const Places p = backward_places(M, N, K, sizeof(T) == 4, act != AFIV_ACT_NONE, !x);
     char *const at = (char *)scratch;
     const bool make_dz = act != AFIV_ACT_NONE || N % WHOLE, make_x = codes || K % WHOLE;
     const bool ready = aligned(scratch) && (make_dz || aligned(dy));

@@ -88,15 +88,17 @@ Places forward_places(int64_t M, int64_t N, int64_t K, bool f32)
     return p;
 }
 
-Places backward_places(int64_t M, int64_t N, int64_t K, bool f32)
+// act: dz differs from dy; eight: x is a checkpoint
+Places backward_places(int64_t M, int64_t N, int64_t K, bool f32, bool act, bool eight)
 {
+    const int64_t whole = f32 ? 4 : 8;                   // elements of 16 bytes
     Places p = {};
     p.bytes = std::max(scratch_floats(M, K, N, f32), scratch_floats(N, K, M, f32)) * 4;
     p.direct = direct_takes(M, K, N, f32) && direct_rows(N) && direct_rows(K);
     p.direct_dw = direct_takes(N, K, M, f32) && direct_rows(N) && direct_rows(K);
-    p.dz = place(p.bytes, p.direct || p.direct_dw, M, N, f32);
-    p.x = place(p.bytes, p.direct_dw, M, K, f32);
-    p.w = place(p.bytes, p.direct && K % (f32 ? 4 : 8), N, K, f32);
+    p.dz = place(p.bytes, (p.direct || p.direct_dw) && (act || N % whole), M, N, f32);
+    p.x = place(p.bytes, p.direct_dw && (eight || K % whole), M, K, f32);
+    p.w = place(p.bytes, p.direct && K % whole, N, K, f32);
     p.db = (p.bytes + 255) / 256 * 256;
     if (p.direct_dw) p.bytes = p.db + PREP_CHUNKS * N * 4;
     return p;

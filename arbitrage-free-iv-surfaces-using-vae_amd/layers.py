@@ -164,8 +164,8 @@ class LinearSaved:
 
 
 @lru_cache(maxsize=4096)
-def _scratch_bytes(query: str, m: int, n: int, k: int, dtype: int) -> int:
-    nbytes = getattr(_lib.lib(), query)(m, n, k, dtype)
+def _scratch_bytes(query: str, m: int, n: int, k: int, *how: int) -> int:
+    nbytes = getattr(_lib.lib(), query)(m, n, k, *how)
     if nbytes < 0:
         _lib.check(int(nbytes), query)
     return nbytes
@@ -228,10 +228,11 @@ def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSav
         raise ValueError(f"nothing is saved of the derivative of {saved.act}")
     _held(saved.pre, g, g.shape, "the saved pre-activation", g.dtype)
     _held(saved.dcodes, g, g.shape, "the saved derivative", torch.uint8)
-    nbytes = _scratch_bytes("afiv_linear_act_backward_scratch", m, n, k, DTYPES[g.dtype])
-    scratch, eight = _scratch(nbytes, g.device), saved.eight
+    act, eight = _act(saved.act), saved.eight
+    nbytes = _scratch_bytes("afiv_linear_act_backward_scratch", m, n, k, DTYPES[g.dtype], act, int(eight is not None))
+    scratch = _scratch(nbytes, g.device)
     _run("afiv_linear_act_backward", g.device, g.data_ptr(), _ptr(saved.x), eight and eight.codes.data_ptr(), eight and eight.scales.data_ptr(),
-         w.data_ptr(), _ptr(saved.pre), _ptr(saved.dcodes), DTYPES[g.dtype], _act(saved.act), m, n, k, _ptr(dx), _ptr(dw), _ptr(db),
+         w.data_ptr(), _ptr(saved.pre), _ptr(saved.dcodes), DTYPES[g.dtype], act, m, n, k, _ptr(dx), _ptr(dw), _ptr(db),
          _ptr(scratch), nbytes)
     return dx, dw, db
 
@@ -323,7 +324,8 @@ def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     _run("afiv_norm_act", v.device, v.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _ptr(keep), DTYPES[v.dtype], code, m, n, float(eps),
          float(momentum), drop_p, _ptr(running_mean), _ptr(running_var), y.data_ptr(), stats.data_ptr(), eight and eight.codes.data_ptr(),
          eight and eight.scales.data_ptr(), _ptr(scratch))
-    if running_mean is not None:         # written behind torch's back: caches keyed on versions must see it
+    # written behind torch's back: caches keyed on versions must see it (inference tensors have none)
+    if running_mean is not None and not running_mean.is_inference() and not running_var.is_inference():
         torch.autograd.graph.increment_version((running_mean, running_var))
     return y, NormSaved(None if checkpoint8 else v, eight, stats, keep, act, drop_p)
 

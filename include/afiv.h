@@ -290,9 +290,10 @@ int afiv_linear_act(const void *x, const void *w, const void *bias, const void *
  * its 8-bit checkpoint (codes, scales); the derivative from pre [M,N] T or, with pre == NULL, from
  * dcodes [M,N] (neither for AFIV_ACT_NONE).  w is needed for dx, the input for dw.  dy times the
  * derivative is rounded to T before the products (FP32: not rounded), db is summed before that rounding. */
-/* scratch: 16-byte aligned, at least afiv_linear_act_backward_scratch(M, N, K, dtype) bytes (NULL where that is 0); large
- * products keep dz [M,N] and, where they cannot read them in place, x [M,K] and w [N,K] there during the call. */
-int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype);
+/* scratch: 16-byte aligned, at least afiv_linear_act_backward_scratch(M, N, K, dtype, act, from_checkpoint) bytes (NULL where
+ * that is 0; from_checkpoint: x will be NULL).  Large products keep there, during the call, what they cannot read in
+ * place: dz [M,N], the restored x [M,K], rows that are not whole 16-byte chunks. */
+int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype, int act, int from_checkpoint);
 int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w, const void *pre,
                              const uint8_t *dcodes, int dtype, int act, int64_t M, int64_t N, int64_t K, void *dx, void *dw, void *db,
                              void *scratch, int64_t scratch_bytes, void *stream);

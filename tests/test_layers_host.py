@@ -58,8 +58,9 @@ def test_linear_refusals(lib):
     assert need > 0
     assert fwd(m=64, n=64, k=4096, scratch=None) == E_WORKSPACE
     assert fwd(m=64, n=64, k=4096, nbytes=need - 1) == E_WORKSPACE
-    assert lib.afiv_linear_act_scratch(-1, 4, 4, 0) == E_SHAPE and lib.afiv_linear_act_backward_scratch(4, 4, 0, 0) == E_SHAPE
-    assert lib.afiv_linear_act_backward_scratch(4, 4, 4, 3) == E_ARG
+    assert lib.afiv_linear_act_scratch(-1, 4, 4, 0) == E_SHAPE and lib.afiv_linear_act_backward_scratch(4, 4, 0, 0, 0, 0) == E_SHAPE
+    assert lib.afiv_linear_act_backward_scratch(4, 4, 4, 3, 0, 0) == E_ARG
+    assert lib.afiv_linear_act_backward_scratch(4, 4, 4, 0, 6, 0) == E_ARG
     assert lib.afiv_linear_act_scratch(1 << 20, 1024, 1024, 1) == 0                 # enough tiles: the sum is not cut
 
     def bwd(dy=p, x=p, codes=None, scales=None, w=p, pre=None, dcodes=None, act=0, m=4, n=4, k=4, dx=p, dw=p, db=p, nbytes=1 << 40):
@@ -68,8 +69,12 @@ def test_linear_refusals(lib):
     assert bwd(dy=None) == E_NULL and bwd(w=None) == E_NULL and bwd(x=None) == E_NULL and bwd(x=None, codes=p) == E_NULL
     assert bwd(act=3) == E_NULL                                                  # no derivative
     assert bwd(act=7) == E_ARG and bwd(k=0) == E_SHAPE
-    need = lib.afiv_linear_act_backward_scratch(1 << 16, 64, 64, 0)
+    need = lib.afiv_linear_act_backward_scratch(1 << 16, 64, 64, 0, 0, 0)
     assert need > 0 and bwd(m=1 << 16, n=64, k=64, nbytes=need - 1) == E_WORKSPACE
+    # room for dz and a restored x only where they are made
+    size = [lib.afiv_linear_act_backward_scratch(1 << 14, 4096, 4096, 1, act, eight) for act, eight in ((0, 0), (4, 0), (0, 1), (4, 1))]
+    assert size[0] < 1 << 23 and size[1] - size[0] >= 1 << 27 and size[2] - size[0] >= 1 << 27 and size[3] - size[0] >= 1 << 28
+    assert fwd(m=1 << 30, n=64) == E_SHAPE                                       # a launch's limit of work items
 
 
 def test_norm_refusals(lib):
