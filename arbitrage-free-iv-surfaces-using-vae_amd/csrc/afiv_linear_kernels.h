@@ -446,11 +446,11 @@ __device__ __forceinline__ void write_out(const LinArgs &a, const f32x4 (&acc)[T
 // workgroup -> split and tile: tile columns run fastest within a band of 8 tile rows, so that workgroups at work
 // together share both operands' tiles; consecutive workgroups go round the 8 XCDs, each with an L2 of its own, so
 // each XCD is given a run of consecutive tiles
-__device__ __forceinline__ void place_tile(const LinArgs &a, int br, int bc, int64_t &split, int64_t &tr, int64_t &tc)
+__device__ __forceinline__ void place_tile(const LinArgs &a, int br, int bc, int64_t block, int64_t all, int64_t &split, int64_t &tr, int64_t &tc)
 {
     const int64_t tiles_r = (a.R + br - 1) / br, tiles_c = (a.C + bc - 1) / bc, tiles = tiles_r * tiles_c;
-    const int64_t all = gridDim.x, each = all / 8, spare = all % 8, xcd = blockIdx.x % 8;
-    int64_t b = xcd * each + (xcd < spare ? xcd : spare) + blockIdx.x / 8;
+    const int64_t each = all / 8, spare = all % 8, xcd = block % 8;
+    int64_t b = xcd * each + (xcd < spare ? xcd : spare) + block / 8;
     split = b / tiles;
     b -= split * tiles;
     const int64_t band = b / (8 * tiles_c), in = b - band * 8 * tiles_c;
@@ -488,7 +488,7 @@ __device__ __forceinline__ void plain_sums(const LinArgs &a, f32x4 (&acc)[TR][TC
 // Tile of 32 TR x 32 TC outputs, four waves of 16 TR x 16 TC.  The matrix instruction gets B as its
 // first operand: a lane then holds four neighbouring columns of one row of C.
 template <class T, Kind KA, Kind KB, int TR, int TC>
-__global__ __launch_bounds__(THREADS) void tile_kernel(LinArgs a)
+__device__ __forceinline__ void tile(const LinArgs &a, int64_t block, int64_t blocks)
 {
     constexpr int BR = 32 * TR, BC = 32 * TC, PARTS = Mma<T>::PARTS;
     typedef typename Part<T>::type P;
@@ -503,7 +503,7 @@ __global__ __launch_bounds__(THREADS) void tile_kernel(LinArgs a)
     const int wr = (wave & 1) * 16 * TR, wc = (wave >> 1) * 16 * TC;
 
     int64_t split, tr, tc;
-    place_tile(a, BR, BC, split, tr, tc);
+    place_tile(a, BR, BC, block, blocks, split, tr, tc);
     const int64_t row0 = tr * BR, col0 = tc * BC;
     const int64_t l_begin = split * a.l_per, l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
 
@@ -575,6 +575,22 @@ __global__ __launch_bounds__(THREADS) void tile_kernel(LinArgs a)
 
     __syncthreads();
     write_out<T, KA == ALONG, TR, TC, 1>(a, acc, row0 + wr, col0 + wc, split, lane, (float *)lds + wave * ROOM);
+}
+
+template <class T, Kind KA, Kind KB>
+__global__ __launch_bounds__(THREADS) void tile_kernel(LinArgs a)
+{
+    tile<T, KA, KB, 2, 2>(a, blockIdx.x, gridDim.x);
+}
+
+// dx and dW in one launch: the first dx_blocks workgroups are dx's.  Neither fills the chip where the tile kernel takes
+// both, and neither waits for the other.
+template <class T, Kind KX>
+__global__ __launch_bounds__(THREADS) void both_kernel(LinArgs dx, LinArgs dw, int64_t dx_blocks)
+{
+    const int64_t block = blockIdx.x;
+    if (block < dx_blocks) tile<T, ALONG_DZ, ACROSS, 2, 2>(dx, block, dx_blocks);
+    else tile<T, ACROSS_DZ, KX, 2, 2>(dw, block - dx_blocks, gridDim.x - dx_blocks);
 }
 
 // The splits' sums, in a fixed order, and the epilogue: SLICES threads an output of four columns, each over every
@@ -761,7 +777,7 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = (wave % WR) * 16 * TR, wc = (wave / WR) * 16 * TC;
     int64_t split, tr, tc;
-    place_tile(a, BR, BC, split, tr, tc);
+    place_tile(a, BR, BC, blockIdx.x, gridDim.x, split, tr, tc);
     const int64_t row0 = tr * BR, col0 = tc * BC;
     const int64_t l_begin = split * a.l_per, l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
     DA da;
@@ -850,7 +866,7 @@ __global__ __launch_bounds__(256, 2) void direct32_kernel(LinArgs a, Source sa, 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = (wave & 1) * 64, wc = (wave >> 1) * 64;
     int64_t split, tr, tc;
-    place_tile(a, 128, 128, split, tr, tc);
+    place_tile(a, 128, 128, blockIdx.x, gridDim.x, split, tr, tc);
     const int64_t row0 = tr * 128, col0 = tc * 128;
     const int64_t l_begin = split * a.l_per, l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
     DA da;
@@ -1066,23 +1082,24 @@ __global__ __launch_bounds__(THREADS) void db_kernel(const float *__restrict__ p
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
-// R <= 16 GROUPS rows of A (stored along l) against 16 rows of B a workgroup: the matrix instruction's 16 columns
+// 16 GROUPS rows of A (stored along l) against 16 rows of B a workgroup: the matrix instruction's 16 columns
 // are rows of A, its rows those of B, and both operands go from memory to registers 16 bytes a lane, four
 // steps' loads together (FP32 by its own matrix instruction: memory, not arithmetic, bounds this).  The workgroup's
-// waves take steps of l in turn and are summed in LDS, wave by wave.  Beyond 32 rows A, which every workgroup reads
-// whole, costs as much as B, and the tiles take over.
+// waves take steps of l in turn and are summed in LDS, wave by wave.  It reads A again for every 16 columns and B for
+// every 32 rows, so beyond 32 rows only products too small for that to matter take it: one round of loads, where
+// a tile waits for one after the other.
 template <class T, int WAVES, int GROUPS>
 __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinArgs a)
 {
     constexpr int STEP = 32, U = 4;
     __shared__ float part[WAVES][16][16 * GROUPS + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = (lane >> 4) * 8;
-    const int64_t col0 = (int64_t)blockIdx.x * 16, col = col0 + (lane & 15);
+    const int64_t col0 = (int64_t)blockIdx.x * 16, col = col0 + (lane & 15), row0 = (int64_t)blockIdx.y * 16 * GROUPS;
     // lanes beyond the matrices read a row inside: what they multiply is not stored
     const T *pb = (const T *)a.B + (col < a.C ? col : a.C - 1) * a.L, *pa[GROUPS];
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-        const int64_t row = g * 16 + (lane & 15);
+        const int64_t row = row0 + g * 16 + (lane & 15);
         pa[g] = (const T *)a.A + (row < a.R ? row : a.R - 1) * a.L;
     }
     f32x4 acc[GROUPS] = {};
@@ -1128,12 +1145,12 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinArgs a)
         for (int q = 0; q < 4; ++q) part[wave][(lane >> 4) * 4 + q][g * 16 + (lane & 15)] = acc[g][q];
     __syncthreads();
     if (wave < GROUPS) {                                       // a wave a group; lane: row = lane & 15, four columns
-        const int64_t row = wave * 16 + (lane & 15), j = col0 + (lane >> 4) * 4;
+        const int64_t row = row0 + wave * 16 + (lane & 15), j = col0 + (lane >> 4) * 4;
         float z[4] = {};
 #pragma unroll
         for (int w = 0; w < WAVES; ++w)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) z[q] += part[w][(lane >> 4) * 4 + q][row];
+            for (int q = 0; q < 4; ++q) z[q] += part[w][(lane >> 4) * 4 + q][wave * 16 + (lane & 15)];
         if (row < a.R && j < a.C) finish<T, true, 4>(a, row, j, z);
     }
 }
@@ -1150,18 +1167,35 @@ void join(const LinArgs &a, hipStream_t s)
     else hipLaunchKernelGGL((join_kernel<T, EPI, 1>), blocks(THREADS), dim3(THREADS), 0, s, a);
 }
 
-template <class T, Kind KA, Kind KB>
-int product(LinArgs a, float *scratch, hipStream_t s)
+// the tile kernel's part of a product's arguments; returns its workgroups
+int64_t tiled(LinArgs &a, float *scratch)
 {
     const Plan p = plan_for(a.R, a.C, a.L);
-    if (p.tiles == 0) return AFIV_OK;
     a.splits = p.splits;
     a.l_per = p.l_per;
     a.partial = scratch;
     a.db_partial = scratch + p.splits * a.R * a.C;
-    const dim3 grid((unsigned)(p.tiles * p.splits));
-    hipLaunchKernelGGL((tile_kernel<T, KA, KB, 2, 2>), grid, dim3(THREADS), 0, s, a);
-    if (p.splits > 1) join<T, KA == ALONG>(a, s);
+    return p.tiles * p.splits;
+}
+
+template <class T, Kind KA, Kind KB>
+int product(LinArgs a, float *scratch, hipStream_t s)
+{
+    const int64_t blocks = tiled(a, scratch);
+    if (blocks == 0) return AFIV_OK;
+    hipLaunchKernelGGL((tile_kernel<T, KA, KB>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a);
+    if (a.splits > 1) join<T, KA == ALONG>(a, s);
+    return ok();
+}
+
+// both backward products (d: dx, e: dW), neither empty
+template <class T, Kind KX>
+int products(LinArgs d, LinArgs e, float *scratch, hipStream_t s)
+{
+    const int64_t blocks = tiled(d, scratch), more = tiled(e, scratch + tile_floats(d.R, d.C, d.L));
+    hipLaunchKernelGGL((both_kernel<T, KX>), dim3((unsigned)(blocks + more)), dim3(THREADS), 0, s, d, e, blocks);
+    if (d.splits > 1) join<T, false>(d, s);
+    if (e.splits > 1) join<T, false>(e, s);
     return ok();
 }
 
@@ -1176,7 +1210,7 @@ int direct(LinArgs a, const Source &sa, const Source &sb, float *scratch, hipStr
     const dim3 grid((unsigned)(p.tiles * p.splits));
     if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((direct32_kernel<KA, KB>), grid, dim3(256), 0, s, a, sa, sb);
     else if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 8, 4>), grid, dim3(512), 0, s, a, sa, sb);
-    else hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 2, 4, 4>), grid, dim3(256), 0, s, a, sa, sb);
+    else hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 4, 2>), grid, dim3(512), 0, s, a, sa, sb);
     if (p.splits > 1) join<T, KA == ALONG && KB == ALONG>(a, s);
     return ok();
 }
@@ -1223,10 +1257,10 @@ Source plain_source(const void *p, int64_t rows, int64_t cols, const Room &room,
 template <class T>
 int forward(const LinArgs &a, float *scratch, hipStream_t s)
 {
-    if (a.R <= FEW && a.R > 0 && a.C > 0) {
-        const dim3 grid((unsigned)((a.C + 15) / 16));
+    if (few_rows(a.R, a.C, a.L)) {
+        const dim3 grid((unsigned)((a.C + 15) / 16), (unsigned)((a.R + 31) / 32));
         // 16 waves where the layer has few workgroups to fill the chip with
-        const bool many = grid.x < 512 && a.L >= 512;
+        const bool many = grid.x * grid.y < 512 && a.L >= 512;
         if (a.R <= 16) {
             if (many) hipLaunchKernelGGL((few_rows_kernel<T, 16, 1>), grid, dim3(1024), 0, s, a);
             else hipLaunchKernelGGL((few_rows_kernel<T, 4, 1>), grid, dim3(256), 0, s, a);
@@ -1282,6 +1316,8 @@ int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *
         if (partial) hipLaunchKernelGGL(db_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(THREADS), 0, s, partial, prep_chunks(M, N), N, (T *)db);
     }
     int rc = ok();
+    if (!rc && dx && M > 0 && (dw || db) && !direct_dx && !direct_dw)
+        return codes ? products<T, ACROSS_EIGHT>(d, e, scratch, s) : products<T, ACROSS>(d, e, scratch, s);
     if (!rc && dx) {
         if (direct_dx) rc = direct<T, ALONG_DZ, ACROSS>(d, g, plain_source<T>(w, N, K, p.w, at, s), scratch, s);
         else rc = product<T, ALONG_DZ, ACROSS>(d, scratch, s);

@@ -10,7 +10,12 @@
 namespace {
 
 constexpr int BK = 32;                    // steps of l in LDS, tile kernel
-constexpr int FEW = 32;                   // most rows of the few-rows kernel
+
+// the few-rows kernel's products
+bool few_rows(int64_t R, int64_t C, int64_t L)
+{
+    return R > 0 && (R <= 32 || (R <= 4096 && (double)R * (double)C * (double)L <= 1 << 21));
+}
 
 int64_t tiles_of(int64_t R, int64_t C, int64_t t) { return ((R + t - 1) / t) * ((C + t - 1) / t); }
 
@@ -49,11 +54,16 @@ bool direct_takes(int64_t R, int64_t C, int64_t L, bool f32)
 bool direct_rows(int64_t len) { return len <= 1 << 20; }
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// floats that either kernel's split takes
+// floats that the tile kernel's split takes, and either kernel's
+int64_t tile_floats(int64_t R, int64_t C, int64_t L)
+{
+    const Plan p = plan_for(R, C, L);
+    return p.splits > 1 ? p.splits * (R * C + R) : 0;
+}
 int64_t scratch_floats(int64_t R, int64_t C, int64_t L, bool f32)
 {
-    const Plan p = plan_for(R, C, L), d = direct_plan(R, C, L, f32);
-    return std::max(p.splits > 1 ? p.splits * (R * C + R) : 0, d.splits > 1 ? d.splits * R * C : 0);
+    const Plan d = direct_plan(R, C, L, f32);
+    return std::max(tile_floats(R, C, L), d.splits > 1 ? d.splits * R * C : 0);
 }
 
 // Scratch of a call: the splits' floats, then the operands written for the direct kernel, then the partial sums of db.
@@ -80,8 +90,9 @@ Room place(int64_t &end, bool wanted, int64_t rows, int64_t cols, bool f32)
 Places forward_places(int64_t M, int64_t N, int64_t K, bool f32)
 {
     Places p = {};
-    p.bytes = M <= FEW ? 0 : scratch_floats(M, N, K, f32) * 4;
-    p.direct = M > FEW && direct_takes(M, N, K, f32) && direct_rows(K);
+    if (few_rows(M, N, K)) return p;
+    p.bytes = scratch_floats(M, N, K, f32) * 4;
+    p.direct = direct_takes(M, N, K, f32) && direct_rows(K);
     const bool make = p.direct && K % (f32 ? 4 : 8);
     p.x = place(p.bytes, make, M, K, f32);
     p.w = place(p.bytes, make, N, K, f32);
@@ -93,7 +104,7 @@ Places backward_places(int64_t M, int64_t N, int64_t K, bool f32, bool act, bool
 {
     const int64_t whole = f32 ? 4 : 8;                   // elements of 16 bytes
     Places p = {};
-    p.bytes = std::max(scratch_floats(M, K, N, f32), scratch_floats(N, K, M, f32)) * 4;
+    p.bytes = std::max(std::max(scratch_floats(M, K, N, f32), scratch_floats(N, K, M, f32)), tile_floats(M, K, N) + tile_floats(N, K, M)) * 4;
     p.direct = direct_takes(M, K, N, f32) && direct_rows(N) && direct_rows(K);
     p.direct_dw = direct_takes(N, K, M, f32) && direct_rows(N) && direct_rows(K);
     p.dz = place(p.bytes, (p.direct || p.direct_dw) && (act || N % whole), M, N, f32);

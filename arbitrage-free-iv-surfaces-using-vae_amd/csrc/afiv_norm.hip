@@ -71,31 +71,41 @@ __device__ __forceinline__ void each_group(int64_t r0, int64_t r1, int ty, F &&f
     for (; r < r1; r += TY) f(r, std::integral_constant<int, 1>());
 }
 
-// Threads stand as TX lanes across columns (V elements each) by TY rows.  Sums of a column over the
-// TY rows of the workgroup: result at the threads of row 0, in row order.
+// Threads stand as TX lanes across columns (V elements each) by TY rows.  Sums of a column over the TY rows of the
+// workgroup, in a fixed order: among a wave's rows by exchanges, then over the waves in LDS.  Result at the threads
+// of row 0.
+constexpr int SUMS_LDS = THREADS / 64;                 // doubles of LDS for each of a column's two sums
+
 template <int V, int TX>
 __device__ __forceinline__ void reduce_rows(double (&a)[V], double (&b)[V], double *lds, int tx, int ty)
 {
-    constexpr int TY = THREADS / TX, W = TX * V;
+    constexpr int WAVES = THREADS / 64, W = TX * V;
 #pragma unroll
-    for (int half = TY / 2; half >= 1; half /= 2) {
-        if (ty >= half && ty < 2 * half) {
+    for (int d = TX; d < 64; d *= 2)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                lds[((ty - half) * W + tx * V + i) * 2] = a[i];
-                lds[((ty - half) * W + tx * V + i) * 2 + 1] = b[i];
-            }
+        for (int i = 0; i < V; ++i) {
+            a[i] += __shfl_xor(a[i], d);
+            b[i] += __shfl_xor(b[i], d);
         }
-        __syncthreads();
-        if (ty < half) {
+    const int wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 < TX) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                a[i] += lds[(ty * W + tx * V + i) * 2];
-                b[i] += lds[(ty * W + tx * V + i) * 2 + 1];
-            }
+        for (int i = 0; i < V; ++i) {
+            lds[(wave * W + tx * V + i) * 2] = a[i];
+            lds[(wave * W + tx * V + i) * 2 + 1] = b[i];
         }
-        __syncthreads();
     }
+    __syncthreads();
+    if (ty == 0) {
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                a[i] += lds[(w * W + tx * V + i) * 2];
+                b[i] += lds[(w * W + tx * V + i) * 2 + 1];
+            }
+    }
+    __syncthreads();
 }
 
 template <bool FULL, class T, int V, int TX>
@@ -243,7 +253,7 @@ template <class T>
 __global__ __launch_bounds__(THREADS) void stats_kernel(NormArgs p, const T *__restrict__ x)
 {
     constexpr int V = Vec<T>::N, TX = WIDE;
-    __shared__ double lds[THREADS / TX / 2 * TX * V * 2];
+    __shared__ double lds[SUMS_LDS * TX * V * 2];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
@@ -317,7 +327,7 @@ template <class T>
 __global__ __launch_bounds__(THREADS) void small_forward_kernel(NormArgs p, const T *__restrict__ x, T *__restrict__ y)
 {
     constexpr int V = Vec<T>::N, TX = 32 / V;
-    __shared__ double lds[THREADS / TX / 2 * TX * V * 2];
+    __shared__ double lds[SUMS_LDS * TX * V * 2];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
@@ -456,7 +466,7 @@ template <class T, bool EIGHT>
 __global__ __launch_bounds__(THREADS, 2) void back_sums_kernel(NormArgs p, const T *__restrict__ x, const T *__restrict__ dy)
 {
     constexpr int V = Vec<T>::N, TX = WIDE;
-    __shared__ double lds[THREADS / TX / 2 * TX * V * 2];
+    __shared__ double lds[SUMS_LDS * TX * V * 2];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
@@ -503,7 +513,7 @@ __global__ __launch_bounds__(THREADS, 2) void small_backward_kernel(NormArgs p, 
                                                                  T *__restrict__ dx)
 {
     constexpr int V = Vec<T>::N, TX = 32 / V;
-    __shared__ double lds[THREADS / TX / 2 * TX * V * 2];
+    __shared__ double lds[SUMS_LDS * TX * V * 2];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);

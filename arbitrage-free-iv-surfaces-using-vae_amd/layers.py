@@ -29,12 +29,12 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _run(name: str, device: torch.device, *args) -> None:
     """One call of the library on the current stream of ``device``."""
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    fn, index = getattr(_lib.lib(), name), device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -67,7 +67,7 @@ def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = Fals
     """Another operand: on x's device, of x's type (or one of ``dtypes``), of the given shape."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a torch.Tensor")
-    if t.device != x.device:
+    if t.get_device() != x.get_device():
         raise ValueError(f"{what} is on {t.device}, expected {x.device}")
     if (t.dtype != x.dtype) if dtypes is None else (t.dtype not in dtypes):
         raise TypeError(f"{what} must be {' or '.join(map(str, dtypes or (x.dtype,)))}, got {t.dtype}")
@@ -80,7 +80,7 @@ def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = Fals
 
 def _held(t, x: torch.Tensor, shape, what: str, dtype=None) -> None:
     """A saved tensor, if there is one, is what the forward pass made for such an output gradient x."""
-    if t is not None and (t.device != x.device or t.shape != shape or not t.is_contiguous() or (dtype is not None and t.dtype != dtype)):
+    if t is not None and (t.get_device() != x.get_device() or t.shape != shape or not t.is_contiguous() or (dtype is not None and t.dtype != dtype)):
         raise ValueError(f"{what} ({t.dtype} {list(t.shape)} on {t.device}) does not belong to dy {list(x.shape)} on {x.device}")
 
 
