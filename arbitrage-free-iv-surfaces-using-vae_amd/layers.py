@@ -84,6 +84,13 @@ def _held(t, x: torch.Tensor, shape, what: str, dtype=None) -> None:
         raise ValueError(f"{what} ({t.dtype} {list(t.shape)} on {t.device}) does not belong to dy {list(x.shape)} on {x.device}")
 
 
+def _made(cls, **fields):
+    """A frozen record of tensors that were made here: its checks, and a setattr a field, are for callers'."""
+    record = object.__new__(cls)
+    record.__dict__.update(fields)
+    return record
+
+
 def _rows(x: torch.Tensor, what: str) -> int:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what} must be [..., features] with at least one feature, got {list(x.shape)}")
@@ -117,17 +124,17 @@ class Checkpoint8:
 
     def restore(self) -> torch.Tensor:
         """The tensor the codes stand for, in the type it was packed from."""
-        out = torch.empty(self.codes.shape, dtype=self.dtype, device=self.codes.device)
-        cols = self.codes.shape[-1]
+        out = self.codes.new_empty(self.codes.shape, dtype=self.dtype)
+        cols = out.shape[-1]
         _run("afiv_checkpoint8_restore", out.device, self.codes.data_ptr(), self.scales.data_ptr(), DTYPES[self.dtype],
              out.numel() // cols, cols, out.data_ptr())
         return out
 
 
 def _empty_checkpoint(x: torch.Tensor) -> Checkpoint8:
-    cols = x.shape[-1]
-    return Checkpoint8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
-                       torch.empty(tuple(x.shape[:-1]) + ((cols + 31) // 32,), dtype=torch.uint8, device=x.device), x.dtype)
+    shape = x.shape
+    return _made(Checkpoint8, codes=x.new_empty(shape, dtype=torch.int8),
+                 scales=x.new_empty((*shape[:-1], (shape[-1] + 31) // 32), dtype=torch.uint8), dtype=x.dtype)
 
 
 def checkpoint8(x: torch.Tensor) -> Checkpoint8:
@@ -183,12 +190,12 @@ def _linear(x, weight, bias, residual, act, want_pre: bool, want_codes: bool):
         raise ValueError("weight must be [out features, in features] with at least one of each")
     n = weight.shape[0]
     w = _like(weight, v, (n, k), "weight")
-    shape = tuple(v.shape[:-1]) + (n,)
+    shape = (*v.shape[:-1], n)
     b = None if bias is None else _like(bias, v, (n,), "bias")
     r = None if residual is None else _like(residual, v, shape, "residual")
-    y = torch.empty(shape, dtype=v.dtype, device=v.device)
-    pre = torch.empty_like(y) if want_pre else None
-    dcodes = torch.empty(shape, dtype=torch.uint8, device=v.device) if want_codes else None
+    y = v.new_empty(shape)
+    pre = v.new_empty(shape) if want_pre else None
+    dcodes = v.new_empty(shape, dtype=torch.uint8) if want_codes else None
     nbytes = _scratch_bytes("afiv_linear_act_scratch", m, n, k, DTYPES[v.dtype])
     scratch = _scratch(nbytes, v.device)
     _run("afiv_linear_act", v.device, v.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), DTYPES[v.dtype], code, m, n, k, y.data_ptr(), _ptr(pre),
@@ -207,7 +214,7 @@ def linear_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     want_codes = signs or (checkpoint8 and act != "none")
     v, y, pre, dcodes = _linear(x, weight, bias, residual, act, act != "none" and not want_codes, want_codes)
     eight = _pack(v) if checkpoint8 else None
-    return y, LinearSaved(None if checkpoint8 else v, eight, pre, dcodes, act)
+    return y, _made(LinearSaved, x=None if checkpoint8 else v, eight=eight, pre=pre, dcodes=dcodes, act=act)
 
 
 def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSaved, need=(True, True, True)):
@@ -217,12 +224,12 @@ def linear_act_backward(dy: torch.Tensor, weight: torch.Tensor, saved: LinearSav
     k, n = saved.shape[-1], weight.shape[0]
     if g.dtype != saved.dtype:
         raise TypeError(f"dy must be {saved.dtype}, got {g.dtype}")
-    g = _like(g, g, tuple(saved.shape[:-1]) + (n,), "dy")
+    g = _like(g, g, (*saved.shape[:-1], n), "dy")
     w = _like(weight, g, (n, k), "weight")
     m = g.numel() // n
-    dx = torch.empty(saved.shape, dtype=g.dtype, device=g.device) if need[0] else None
-    dw = torch.empty((n, k), dtype=g.dtype, device=g.device) if need[1] else None
-    db = torch.empty((n,), dtype=g.dtype, device=g.device) if need[2] else None
+    dx = g.new_empty(saved.shape) if need[0] else None
+    dw = g.new_empty((n, k)) if need[1] else None
+    db = g.new_empty((n,)) if need[2] else None
     _held(saved.x if saved.eight is None else saved.eight.codes, g, saved.shape, "the saved input")
     if saved.act != "none" and saved.pre is None and saved.dcodes is None:
         raise ValueError(f"nothing is saved of the derivative of {saved.act}")
@@ -249,7 +256,8 @@ class _LinearAct(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         weight, x, pre, dcodes, codes, scales = ctx.saved_tensors
-        saved = LinearSaved(x, None if codes is None else Checkpoint8(codes, scales, ctx.dtype), pre, dcodes, ctx.act)
+        eight = None if codes is None else _made(Checkpoint8, codes=codes, scales=scales, dtype=ctx.dtype)
+        saved = _made(LinearSaved, x=x, eight=eight, pre=pre, dcodes=dcodes, act=ctx.act)
         need = ctx.needs_input_grad
         grads = linear_act_backward(dy, weight, saved, need[:3]) if any(need[:3]) else (None, None, None)
         return (*grads, dy if need[3] else None, None, None)
@@ -318,7 +326,7 @@ def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     if keep is not None:
         keep = _like(keep, v, (m, n), "keep", (torch.bool, torch.uint8))
     y = torch.empty_like(v)
-    stats = torch.empty((2, n), dtype=torch.float64, device=v.device)
+    stats = v.new_empty((2, n), dtype=torch.float64)
     eight = _empty_checkpoint(v) if checkpoint8 else None
     scratch = _norm_scratch(m, n, v.device)
     _run("afiv_norm_act", v.device, v.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _ptr(keep), DTYPES[v.dtype], code, m, n, float(eps),
@@ -327,7 +335,7 @@ def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     # written behind torch's back: caches keyed on versions must see it (inference tensors have none)
     if running_mean is not None and not running_mean.is_inference() and not running_var.is_inference():
         torch.autograd.graph.increment_version((running_mean, running_var))
-    return y, NormSaved(None if checkpoint8 else v, eight, stats, keep, act, drop_p)
+    return y, _made(NormSaved, x=None if checkpoint8 else v, eight=eight, stats=stats, keep=keep, act=act, drop_p=drop_p)
 
 
 def batch_norm_act_backward(dy: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, saved: NormSaved, need_dx: bool = True):
@@ -364,7 +372,8 @@ class _BatchNormAct(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         weight, bias, x, stats, keep, codes, scales = ctx.saved_tensors
-        saved = NormSaved(x, None if codes is None else Checkpoint8(codes, scales, ctx.dtype), stats, keep, ctx.act, ctx.drop_p)
+        eight = None if codes is None else _made(Checkpoint8, codes=codes, scales=scales, dtype=ctx.dtype)
+        saved = _made(NormSaved, x=x, eight=eight, stats=stats, keep=keep, act=ctx.act, drop_p=ctx.drop_p)
         need = ctx.needs_input_grad
         dx, dgamma, dbeta = batch_norm_act_backward(dy, weight, bias, saved, need[0])
         return (dx, dgamma if need[1] else None, dbeta if need[2] else None) + (None,) * 8
