@@ -757,8 +757,11 @@ __device__ __forceinline__ void arrive()
     asm volatile("" ::: "memory");
 }
 
-// 16-bit types.  WR x WC waves of 16 TR x 16 TC outputs.
-template <class T, Kind KA, Kind KB, int WR, int WC, int TR, int TC>
+// 16-bit types.  WR x WC waves of 16 TR x 16 TC outputs.  DEEP: four buffers instead of two, for a grid of at most one
+// workgroup a CU, which has no other to hide its loads behind: 777 x 1003 x 2055 19.4 -> 17.0 us, of which the steps
+// take 0.21 us each, what the matrix units need and L2 gives; where two fit a CU two buffers are faster (26 and
+// 20 us for a product of 315 workgroups).
+template <class T, Kind KA, Kind KB, int WR, int WC, int TR, int TC, bool DEEP>
 __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source sa, Source sb)
 {
     constexpr int W = WR * WC, BR = 16 * TR * WR, BC = 16 * TC * WC, FK = 64;
@@ -771,6 +774,10 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
     __shared__ __align__(1024) char a1[DA::BYTES];
     __shared__ __align__(1024) char b0[DB::BYTES];
     __shared__ __align__(1024) char b1[DB::BYTES];
+    __shared__ __align__(1024) char a2[DA::BYTES];
+    __shared__ __align__(1024) char a3[DA::BYTES];
+    __shared__ __align__(1024) char b2[DB::BYTES];
+    __shared__ __align__(1024) char b3[DB::BYTES];
     // the epilogue's room of a wave: a quarter of the waves share an array
     static_assert(W % 4 == 0 && DA::BYTES == DB::BYTES, "four arrays of one size");
     constexpr int SLAB = 16 * 16 * TC, FIT = DA::BYTES / (W / 4) / 4 / SLAB, SLABS = FIT >= TR ? TR : FIT >= TR / 2 ? TR / 2 : FIT >= TR / 4 ? TR / 4 : 1;
@@ -807,27 +814,36 @@ __global__ __launch_bounds__(64 * WR * WC) void direct_kernel(LinArgs a, Source 
         }
     };
     static_assert(TC <= TR, "a row block for every column block's reads");
+    constexpr int LATER = DEEP ? 2 * (DA::PER + DB::PER) : 0;   // a wave's loads that may still be on their way at a barrier
     load(a0, b0, l_begin);
     load(a1, b1, l_begin + FK);
-    arrive<0>();
+    if constexpr (DEEP) {
+        load(a2, b2, l_begin + 2 * FK);
+        load(a3, b3, l_begin + 3 * FK);
+    }
+    arrive<DEEP ? 3 * (DA::PER + DB::PER) : 0>();
 #pragma unroll
     for (int i = 0; i < TR; ++i) fa[i] = da.read(a0, i, 0);
 #pragma unroll
     for (int j = 0; j < TC; ++j) fb[0][j] = db.read(b0, j, 0);
-    // every load of this wave has arrived and its reads are done before any wave reads the next tile or loads over this
-    // one; loads are issued before the products, not among them
+    // every load of this wave for the next tile has arrived and its reads are done before any wave reads that tile or
+    // loads over this one; loads are issued before the products, not among them
+    auto step = [&](char *ta, char *tb, char *na, char *nb, int64_t l0) {      // this tile, the next one, what comes into this one's place
+        slice(0, ta, tb, 1);
+        arrive<LATER>();
+        load(ta, tb, l0);
+        __builtin_amdgcn_sched_barrier(0);
+        slice(1, na, nb, 0);
+    };
+    constexpr int BUFFERS = DEEP ? 4 : 2;
 #pragma unroll 1
-    for (int64_t l0 = l_begin; l0 < l_end; l0 += 2 * FK) {      // an odd last step is multiplied with zeros
-        slice(0, a0, b0, 1);
-        arrive<0>();
-        load(a0, b0, l0 + 2 * FK);
-        __builtin_amdgcn_sched_barrier(0);
-        slice(1, a1, b1, 0);
-        slice(0, a1, b1, 1);
-        arrive<0>();
-        load(a1, b1, l0 + 3 * FK);
-        __builtin_amdgcn_sched_barrier(0);
-        slice(1, a0, b0, 0);
+    for (int64_t l0 = l_begin; l0 < l_end; l0 += BUFFERS * FK) {               // steps from l_end on are multiplied with zeros
+        step(a0, b0, a1, b1, l0 + BUFFERS * FK);
+        if constexpr (DEEP) {
+            step(a1, b1, a2, b2, l0 + 5 * FK);
+            step(a2, b2, a3, b3, l0 + 6 * FK);
+            step(a3, b3, a0, b0, l0 + 7 * FK);
+        } else step(a1, b1, a0, b0, l0 + 3 * FK);
     }
     __builtin_amdgcn_s_waitcnt(0x0070);                         // the last loads and reads, before LDS is used again
     __syncthreads();
@@ -1209,8 +1225,9 @@ int direct(LinArgs a, const Source &sa, const Source &sb, float *scratch, hipStr
     a.db = nullptr;
     const dim3 grid((unsigned)(p.tiles * p.splits));
     if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((direct32_kernel<KA, KB>), grid, dim3(256), 0, s, a, sa, sb);
-    else if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 8, 4>), grid, dim3(512), 0, s, a, sa, sb);
-    else hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 4, 2>), grid, dim3(512), 0, s, a, sa, sb);
+    else if (huge_tiles(a.R, a.C)) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 8, 4, false>), grid, dim3(512), 0, s, a, sa, sb);
+    else if (p.tiles * p.splits <= CUS) hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 4, 2, true>), grid, dim3(512), 0, s, a, sa, sb);
+    else hipLaunchKernelGGL((direct_kernel<T, KA, KB, 2, 4, 4, 2, false>), grid, dim3(512), 0, s, a, sa, sb);
     if (p.splits > 1) join<T, KA == ALONG && KB == ALONG>(a, s);
     return ok();
 }

@@ -10,6 +10,7 @@
 namespace {
 
 constexpr int BK = 32;                    // steps of l in LDS, tile kernel
+constexpr int CUS = 256;
 
 // the few-rows kernel's products
 bool few_rows(int64_t R, int64_t C, int64_t L)
@@ -26,7 +27,7 @@ Plan cut(int64_t tiles, int64_t L, int64_t step, int64_t few, int64_t want, int6
 {
     Plan p = {tiles, 1, 1};
     const int64_t steps = (L + step - 1) / step;
-    if (tiles > 0 && tiles < few && steps >= 2 * least) p.splits = std::min((want + tiles - 1) / tiles, steps / least);
+    if (tiles > 0 && tiles < few && steps >= 2 * least) p.splits = std::min(want / tiles, steps / least);
     p.l_per = std::max<int64_t>(1, (steps + p.splits - 1) / p.splits) * step;
     p.splits = std::max<int64_t>(1, (L + p.l_per - 1) / p.l_per);
     return p;
@@ -35,13 +36,15 @@ Plan cut(int64_t tiles, int64_t L, int64_t step, int64_t few, int64_t want, int6
 // Tile kernel: 64 x 64 tiles; below 256 workgroups the sum is cut into runs of at least 256 steps.
 Plan plan_for(int64_t R, int64_t C, int64_t L) { return cut(tiles_of(R, C, 64), L, BK, 256, 512, 8); }
 
-// The direct kernel: 256 x 256 tiles where they fill the chip at least once, else 128 x 128 (FP32: always).  Below 96
-// tiles the sum is cut, for two workgroups a CU; above, the kernel that joins the runs costs more than the idle CUs.
-bool huge_tiles(int64_t R, int64_t C) { return tiles_of(R, C, 256) >= 256; }
+// The direct kernel: 256 x 256 tiles where they fill the chip at least once and little of them lies outside the matrix
+// (131072 x 128 x 128, bf16: 26 us by 128 x 128 tiles, 46 by the large ones), else 128 x 128 (FP32: always).  Below 96
+// tiles the sum is cut, 16 bit for one workgroup a CU with four buffers, FP32 for two with two; above, the kernel that
+// joins the runs costs more than the idle CUs.
+bool huge_tiles(int64_t R, int64_t C) { return tiles_of(R, C, 256) >= CUS && 16 * tiles_of(R, C, 256) <= 5 * tiles_of(R, C, 128); }
 Plan direct_plan(int64_t R, int64_t C, int64_t L, bool f32)
 {
     if (f32) return cut(tiles_of(R, C, 128), L, 32, 96, 512, 8);
-    return huge_tiles(R, C) ? cut(tiles_of(R, C, 256), L, 64, 0, 0, 1) : cut(tiles_of(R, C, 128), L, 64, 96, 512, 8);
+    return huge_tiles(R, C) ? cut(tiles_of(R, C, 256), L, 64, 0, 0, 1) : cut(tiles_of(R, C, 128), L, 64, 96, CUS, 8);
 }
 
 // What the direct kernel takes: at least a tile each way, rows within 2^31 bytes of a tile's corner, and enough work that
