@@ -45,6 +45,28 @@ __device__ __forceinline__ Pack<T, N> load_some(const T *p, int n)
     __builtin_memcpy(&r, w, sizeof r);
     return r;
 }
+// The same by one load of the N elements that end with these n (0 < n <= N), moved into place: no branch, so several can
+// be on their way.  ahead: N - n elements stand before p; otherwise element by element.
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> load_ending(const T *p, int n, bool ahead)
+{
+    constexpr int W = sizeof(T) * N / 4;
+    if (!ahead) return load_some<T, N>(p, n);
+    uint32_t w[W];
+    __builtin_memcpy(w, p - (N - n), sizeof w);
+    const uint32_t by = (N - n) * sizeof(T);
+#pragma unroll
+    for (int s = W / 2; s > 0; s /= 2)
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = by & (4 * s) ? (i + s < W ? w[i + s] : 0) : w[i];
+    if constexpr (sizeof(T) < 4) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = __builtin_amdgcn_alignbyte(i + 1 < W ? w[i + 1] : 0, w[i], by & 3);
+    }
+    Pack<T, N> r;
+    __builtin_memcpy(&r, w, sizeof r);
+    return r;
+}
 template <class T, int N>
 __device__ __forceinline__ void store_some(T *p, const Pack<T, N> &r, int n)
 {

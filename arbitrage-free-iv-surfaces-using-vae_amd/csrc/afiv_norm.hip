@@ -44,15 +44,16 @@ struct NormArgs {
     float *dgamma, *dbeta;
 };
 
-// Rows come in groups of four: their loads are issued together, so that a wave has several rows in flight (a row
-// at a time left HBM at 1.5 TB/s).  That needs loads that are not guarded one by one, so it is for lanes that have
-// all of their columns (FULL); the lane at a ragged edge goes row by row.
+// Rows come in groups of four (or two): their loads are issued together, so that a wave has several rows in flight (a row
+// at a time left HBM at 1.5 TB/s).  FULL: the workgroup's lanes have all V of their columns, or none.  Otherwise all of
+// them load as the ragged one must, without branches: its own way, row by row, held the others up (131072 x 299, bf16,
+// backward 307 -> 226 us).
 
 template <bool FULL, class E, int V>
-__device__ __forceinline__ Pack<E, V> take(const E *p, int n)
+__device__ __forceinline__ Pack<E, V> take(const NormArgs &a, const E *p, int n)
 {
     if constexpr (FULL) return load_pack<E, V>(p);
-    else return load_some<E, V>(p, n);
+    else return load_ending<E, V>(p, n, a.N >= V);
 }
 template <bool FULL, class E, int V>
 __device__ __forceinline__ void give(E *p, const Pack<E, V> &v, int n)
@@ -61,13 +62,13 @@ __device__ __forceinline__ void give(E *p, const Pack<E, V> &v, int n)
     else store_some<E, V>(p, v, n);
 }
 
-// calls f(first row, rows) for the rows r0 + ty, + TY, ... below r1, four at a time and then one by one
+// calls f(first row, rows) for the rows r0 + ty, + TY, ... below r1, U at a time and then one by one
 template <bool FULL, int TY, class F>
 __device__ __forceinline__ void each_group(int64_t r0, int64_t r1, int ty, F &&f)
 {
     int64_t r = r0 + ty;
-    if constexpr (FULL)
-        for (; r + 3 * TY < r1; r += 4 * TY) f(r, std::integral_constant<int, 4>());
+    constexpr int U = FULL ? 4 : 2;                 // moving a ragged row's elements into place takes registers
+    for (; r + (U - 1) * TY < r1; r += U * TY) f(r, std::integral_constant<int, U>());
     for (; r < r1; r += TY) f(r, std::integral_constant<int, 1>());
 }
 
@@ -116,12 +117,12 @@ __device__ __forceinline__ void sum_x(const NormArgs &p, const T *__restrict__ x
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0;
     if (n <= 0) return;
-    const Pack<T, V> x0 = take<FULL, T, V>(x + col, n);
+    const Pack<T, V> x0 = take<FULL, T, V>(p, x + col, n);
     each_group<FULL, TY>(r0, r1, ty, [&](int64_t r, auto rows) {
         constexpr int U = decltype(rows)::value;
         Pack<T, V> v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = take<FULL, T, V>(x + (r + u * TY) * p.N + col, n);
+        for (int u = 0; u < U; ++u) v[u] = take<FULL, T, V>(p, x + (r + u * TY) * p.N + col, n);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -192,25 +193,24 @@ __device__ __forceinline__ void normalise(const NormArgs &p, const float (&f)[V]
     }
 }
 
-// outputs (and the checkpoint) of rows r0..r1 at columns col..col+n
+// outputs (and the checkpoint) of rows r0..r1 at columns col..col+n.  Lanes behind the last column are
+// among those that find a checkpoint block's largest magnitude: they take the last lane's columns and store nothing.
 template <bool FULL, class T, int V, int TX>
 __device__ __forceinline__ void apply_rows(const NormArgs &p, const T *__restrict__ x, T *__restrict__ y, int64_t r0, int64_t r1,
-                                           int64_t col, int n, int ty, const Column<V> &c)
+                                           int64_t col, int n, int ty, const Column<V> &c, bool mine)
 {
     constexpr int TY = THREADS / TX, LANES = 32 / V;        // lanes of a checkpoint block
     const int64_t nb = (p.N + 31) / 32;
     with_act(p.act, [&](auto act) {
         each_group<FULL, TY>(r0, r1, ty, [&](int64_t r, auto rows) {
             constexpr int U = decltype(rows)::value;
-            Pack<T, V> v[U] = {};
-            Pack<uint8_t, V> k[U] = {};
-            if (FULL || n > 0) {
+            Pack<T, V> v[U];
+            Pack<uint8_t, V> k[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) v[u] = take<FULL, T, V>(x + (r + u * TY) * p.N + col, n);
-                if (p.keep) {
+            for (int u = 0; u < U; ++u) v[u] = take<FULL, T, V>(p, x + (r + u * TY) * p.N + col, n);
+            if (p.keep) {
 #pragma unroll
-                    for (int u = 0; u < U; ++u) k[u] = take<FULL, uint8_t, V>(p.keep + (r + u * TY) * p.N + col, n);
-                }
+                for (int u = 0; u < U; ++u) k[u] = take<FULL, uint8_t, V>(p, p.keep + (r + u * TY) * p.N + col, n);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -226,7 +226,7 @@ __device__ __forceinline__ void apply_rows(const NormArgs &p, const T *__restric
                     act_both<decltype(act)::value>(z[i], o, d);
                     out.v[i] = (T)(p.keep ? (k[u].v[i] ? o * p.scale : 0.0f) : o);
                 }
-                if (FULL || n > 0) give<FULL, T, V>(y + at, out, n);
+                if (mine) give<FULL, T, V>(y + at, out, n);
                 if (p.codes) {
                     float amax = 0.0f;
 #pragma unroll
@@ -237,7 +237,7 @@ __device__ __forceinline__ void apply_rows(const NormArgs &p, const T *__restric
                     Pack<int8_t, V> q;
 #pragma unroll
                     for (int i = 0; i < V; ++i) q.v[i] = eight_code(f[i], e);
-                    if (FULL || n > 0) {
+                    if (mine) {
                         give<FULL, int8_t, V>(p.codes + at, q, n);
                         if ((col & 31) == 0) p.scales[(r + u * TY) * nb + col / 32] = (uint8_t)e;
                     }
@@ -257,9 +257,10 @@ __global__ __launch_bounds__(THREADS) void stats_kernel(NormArgs p, const T *__r
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
+    const bool whole = p.N % V == 0 || (int64_t)(blockIdx.x + 1) * TX * V <= p.N;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
     double s1[V], s2[V];
-    if (n >= V) sum_x<true, T, V, TX>(p, x, r0, r1, col, n, ty, s1, s2);
+    if (whole) sum_x<true, T, V, TX>(p, x, r0, r1, col, n, ty, s1, s2);
     else sum_x<false, T, V, TX>(p, x, r0, r1, col, n, ty, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
     if (ty == 0) {
@@ -312,14 +313,17 @@ __global__ __launch_bounds__(THREADS) void apply_kernel(NormArgs p, const T *__r
 {
     constexpr int V = Vec<T>::N, TX = WIDE;
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
-    const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
+    const int64_t first = ((int64_t)blockIdx.x * TX + tx) * V;
+    const bool mine = first < p.N;
+    const int64_t col = mine ? first : (p.N - 1) / V * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
+    const bool whole = p.N % V == 0;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
     Column<V> k;
     columns<V>(p, col, n, k);
-    const bool whole = (int64_t)(blockIdx.x + 1) * TX * V <= p.N;       // the lanes of a checkpoint block stay together
-    if (whole) apply_rows<true, T, V, TX>(p, x, y, r0, r1, col, n, ty, k);
-    else apply_rows<false, T, V, TX>(p, x, y, r0, r1, col, n, ty, k);
+    if ((int64_t)(blockIdx.x + 1) * TX * V <= p.N) apply_rows<true, T, V, TX>(p, x, y, r0, r1, col, n, ty, k, true);      // no guards
+    else if (whole) apply_rows<true, T, V, TX>(p, x, y, r0, r1, col, n, ty, k, mine);
+    else apply_rows<false, T, V, TX>(p, x, y, r0, r1, col, n, ty, k, mine);
 }
 
 // A batch of few rows: one workgroup does 32 columns from the sums to the outputs, in one launch.
@@ -329,13 +333,16 @@ __global__ __launch_bounds__(THREADS) void small_forward_kernel(NormArgs p, cons
     constexpr int V = Vec<T>::N, TX = 32 / V;
     __shared__ double lds[SUMS_LDS * TX * V * 2];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
-    const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
+    const int64_t first = ((int64_t)blockIdx.x * TX + tx) * V;
+    const bool mine = first < p.N;
+    const int64_t col = mine ? first : (p.N - 1) / V * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
+    const bool whole = p.N % V == 0 || (int64_t)(blockIdx.x + 1) * TX * V <= p.N;
     double s1[V], s2[V];
-    if (n >= V) sum_x<true, T, V, TX>(p, x, 0, p.M, col, n, ty, s1, s2);
+    if (whole) sum_x<true, T, V, TX>(p, x, 0, p.M, col, n, ty, s1, s2);
     else sum_x<false, T, V, TX>(p, x, 0, p.M, col, n, ty, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
-    if (ty == 0) {
+    if (ty == 0 && mine) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i < n) {
@@ -356,9 +363,9 @@ __global__ __launch_bounds__(THREADS) void small_forward_kernel(NormArgs p, cons
             k.beta[i] = p.beta[col + i];
         }
     }
-    const bool whole = (int64_t)(blockIdx.x + 1) * TX * V <= p.N;
-    if (whole) apply_rows<true, T, V, TX>(p, x, y, 0, p.M, col, n, ty, k);
-    else apply_rows<false, T, V, TX>(p, x, y, 0, p.M, col, n, ty, k);
+    if ((int64_t)(blockIdx.x + 1) * TX * V <= p.N) apply_rows<true, T, V, TX>(p, x, y, 0, p.M, col, n, ty, k, true);      // no guards
+    else if (whole) apply_rows<true, T, V, TX>(p, x, y, 0, p.M, col, n, ty, k, mine);
+    else apply_rows<false, T, V, TX>(p, x, y, 0, p.M, col, n, ty, k, mine);
 }
 
 // ---- backward --------------------------------------------------------------------------------
@@ -377,15 +384,15 @@ struct BackRows {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t row = r + u * ty_step, at = row * p.N + col;
-            d[u] = take<FULL, T, V>(dy + at, n);
+            d[u] = take<FULL, T, V>(p, dy + at, n);
             if constexpr (EIGHT) {
-                q[u] = take<FULL, int8_t, V>(p.codes + at, n);
+                q[u] = take<FULL, int8_t, V>(p, p.codes + at, n);
                 e[u] = p.scales[row * nb + col / 32];
-            } else x[u] = take<FULL, T, V>(xs + at, n);
+            } else x[u] = take<FULL, T, V>(p, xs + at, n);
         }
         if (p.keep) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) k[u] = take<FULL, uint8_t, V>(p.keep + (r + u * ty_step) * p.N + col, n);
+            for (int u = 0; u < U; ++u) k[u] = take<FULL, uint8_t, V>(p, p.keep + (r + u * ty_step) * p.N + col, n);
         }
     }
     // g and h of row u
@@ -470,11 +477,12 @@ __global__ __launch_bounds__(THREADS, 2) void back_sums_kernel(NormArgs p, const
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
+    const bool whole = p.N % V == 0 || (int64_t)(blockIdx.x + 1) * TX * V <= p.N;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
     Column<V> k;
     columns<V>(p, col, n, k);
     double s1[V], s2[V];
-    if (n >= V) sum_g<true, T, V, TX, EIGHT>(p, x, dy, r0, r1, col, n, ty, k, s1, s2);
+    if (whole) sum_g<true, T, V, TX, EIGHT>(p, x, dy, r0, r1, col, n, ty, k, s1, s2);
     else sum_g<false, T, V, TX, EIGHT>(p, x, dy, r0, r1, col, n, ty, k, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
     if (ty == 0) {
@@ -495,6 +503,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_dx_kernel(NormArgs p, const T
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
+    const bool whole = p.N % V == 0 || (int64_t)(blockIdx.x + 1) * TX * V <= p.N;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.M ? r0 + p.rows_per : p.M;
     Column<V> k;
     columns<V>(p, col, n, k);
@@ -504,7 +513,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_dx_kernel(NormArgs p, const T
         mb[i] = i < n ? (float)p.means[col + i] : 0.0f;
         mg[i] = i < n ? (float)p.means[p.N + col + i] : 0.0f;
     }
-    if (n >= V) back_rows<true, T, V, TX, EIGHT>(p, x, dy, dx, r0, r1, col, n, ty, k, mb, mg);
+    if (whole) back_rows<true, T, V, TX, EIGHT>(p, x, dy, dx, r0, r1, col, n, ty, k, mb, mg);
     else back_rows<false, T, V, TX, EIGHT>(p, x, dy, dx, r0, r1, col, n, ty, k, mb, mg);
 }
 
@@ -517,10 +526,11 @@ __global__ __launch_bounds__(THREADS, 2) void small_backward_kernel(NormArgs p, 
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     const int64_t col = ((int64_t)blockIdx.x * TX + tx) * V;
     const int n = (int)(p.N - col < V ? p.N - col : V);
+    const bool whole = p.N % V == 0 || (int64_t)(blockIdx.x + 1) * TX * V <= p.N;
     Column<V> k;
     columns<V>(p, col, n, k);
     double s1[V], s2[V];
-    if (n >= V) sum_g<true, T, V, TX, EIGHT>(p, x, dy, 0, p.M, col, n, ty, k, s1, s2);
+    if (whole) sum_g<true, T, V, TX, EIGHT>(p, x, dy, 0, p.M, col, n, ty, k, s1, s2);
     else sum_g<false, T, V, TX, EIGHT>(p, x, dy, 0, p.M, col, n, ty, k, s1, s2);
     reduce_rows<V, TX>(s1, s2, lds, tx, ty);
     if (ty == 0) {
@@ -541,7 +551,7 @@ __global__ __launch_bounds__(THREADS, 2) void small_backward_kernel(NormArgs p, 
         mb[i] = i < n ? (float)lds[(tx * V + i) * 2] : 0.0f;
         mg[i] = i < n ? (float)lds[(tx * V + i) * 2 + 1] : 0.0f;
     }
-    if (n >= V) back_rows<true, T, V, TX, EIGHT>(p, x, dy, dx, 0, p.M, col, n, ty, k, mb, mg);
+    if (whole) back_rows<true, T, V, TX, EIGHT>(p, x, dy, dx, 0, p.M, col, n, ty, k, mb, mg);
     else back_rows<false, T, V, TX, EIGHT>(p, x, dy, dx, 0, p.M, col, n, ty, k, mb, mg);
 }
 

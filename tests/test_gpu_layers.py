@@ -169,6 +169,20 @@ def test_linear_needed_gradients_only(afiv):
             assert (g is None) if not n else torch.equal(g, e)
 
 
+# at these sizes dz is made by a pass of its own, which sums db as it goes, with or without dW
+@pytest.mark.parametrize("typ,m,k,n", [("bf16", 2048, 512, 300), ("f16", 1999, 1001, 515), ("f32", 1024, 1000, 515)])
+def test_linear_needed_gradients_only_large(afiv, typ, m, k, n):
+    for act in ("none", "gelu", "relu"):
+        x, w, b, _, dy = inputs(TYPES[typ], m, k, n, 3)
+        y, saved = afiv.linear_act_forward(x, w, b, act=act, checkpoint8=act == "relu")
+        every = afiv.linear_act_backward(dy, w, saved)
+        check_backward(dy, w, saved, act, *every)
+        for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, False, True)):
+            got = afiv.linear_act_backward(dy, w, saved, need)
+            for g, e, wanted in zip(got, every, need):
+                assert (g is None) if not wanted else torch.equal(g, e)
+
+
 @pytest.mark.parametrize("typ", TYPES)
 def test_linear_values_that_are_not_finite(afiv, typ):
     """An infinity or NaN of one row reaches that row of y and no other; in FP32 so do magnitudes that do
@@ -471,6 +485,13 @@ def test_norm_forward_and_backward(afiv, typ, m, n):
             var, mean = torch.var_mean(x.double(), dim=0, correction=1)
             within(rm, 0.8 * rm0 + 0.2 * mean, 4 * U * (rm0.abs() + mean.abs()), "running mean")
             within(rv, 0.8 * rv0 + 0.2 * var, 4 * U * (rv0 + var) + 1e-13 * mean.square(), "running var")
+
+
+# workgroups whose last lanes have no columns, or some of theirs, beside full ones
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("m,n", [(700, 300), (700, 299), (1100, 300), (1100, 299), (1100, 3), (4100, 76)])
+def test_norm_ragged_workgroups(afiv, typ, m, n):
+    test_norm_forward_and_backward(afiv, typ, m, n)
 
 
 def test_norm_matches_torch_modules(afiv):
