@@ -10,7 +10,7 @@
 // lies in LDS along l, 32 steps of l a row of 64 bytes, so one matrix instruction's operand is one
 // 16-byte LDS read; operands stored across l are transposed in registers, 4 x 4 elements at a time, on
 // their way in.  dz is formed there too (dy, and z or its 8-bit derivative codes), and so is an 8-bit
-// x: neither ever exists in memory.
+// x: neither exists in memory (but for large products, below).
 //
 // 16-bit types go to v_mfma_f32_16x16x32.  FP32 operands are cut into three BF16 parts of 8 bits,
 // a = a1 + a2 + a3 exactly (each the upper half of what is left), and the six products a1 b1, a1 b2, a2 b1,
@@ -19,8 +19,9 @@
 // An infinity does not split (its rest is NaN); a workgroup that has met one does its tile again with FP32
 // multiply-adds.  Parts below 2^-133 are lost, that is, an element under 2^-110 keeps fewer than 24 bits.
 //
-// Few rows (up to 16) take another kernel: W is read once, straight from memory into the matrix
-// instruction, by as many waves as the layer has.
+// Few rows (up to 32), and small products, take another kernel: W goes straight from memory into the matrix
+// instruction, by as many waves as the layer has.  Large products take a third, whose operands go from memory to LDS
+// as they are; what cannot be read so (dz, an 8-bit x, rows that are not whole 16-byte chunks) is written out first.
 #pragma once
 
 #include "afiv_layer.h"
@@ -486,7 +487,9 @@ __device__ __forceinline__ void plain_sums(const LinArgs &a, f32x4 (&acc)[TR][TC
 }
 
 // Tile of 32 TR x 32 TC outputs, four waves of 16 TR x 16 TC.  The matrix instruction gets B as its
-// first operand: a lane then holds four neighbouring columns of one row of C.
+// first operand: a lane then holds four neighbouring columns of one row of C.  For products too small for the direct
+// kernel, where latency bounds: one step's loads are on their way behind the step before.  Backward of 64 rows, 13 -> 128, in
+// FP32: 9.5 us for dx, dW and db.
 template <class T, Kind KA, Kind KB, int TR, int TC>
 __device__ __forceinline__ void tile(const LinArgs &a, int64_t block, int64_t blocks)
 {
@@ -638,8 +641,9 @@ __global__ __launch_bounds__(THREADS) void join_kernel(LinArgs a)
 }
 
 // ---- large products -------------------------------------------------------------------------------
-// The same product from operands that go from memory to LDS as they are: rows of whole 16-byte chunks.  Operands of that kind are read where they stand; others are written so first, by
-// prepare_kernel: rows of another length, dz, an 8-bit x.
+// The same product from operands that go from memory to LDS as they are: rows of whole 16-byte chunks.  Operands of
+// that kind are read where they stand; others are written so first, by prepare_kernel: rows of another length, dz, an
+// 8-bit x.
 // Steps of 64 (FP32: 32): a tile's rows are 128 bytes along l, or its steps of l are rows of BR elements
 // (across), and lie in LDS as the loads leave them, 1024 consecutive bytes an instruction; what keeps the
 // reads off each other's banks is therefore a permutation of the global addresses: 16-byte chunk c of row r stands
@@ -757,7 +761,9 @@ __device__ __forceinline__ void arrive()
     asm volatile("" ::: "memory");
 }
 
-// 16-bit types.  WR x WC waves of 16 TR x 16 TC outputs.  DEEP: four buffers instead of two, for a grid of at most one
+// 16-bit types.  WR x WC waves of 16 TR x 16 TC outputs.  The matrix units bound it: 16384 x 4096 x 8192 in BF16 with gelu
+// and residual takes 0.91 ms (1.21 PFLOP/s, 58 % of their cycles; the rest is the epilogue and the start of each tile),
+// dW of 16384 x 4096 x 4096 0.40 ms (1.37 PFLOP/s).  DEEP: four buffers instead of two, for a grid of at most one
 // workgroup a CU, which has no other to hide its loads behind: 777 x 1003 x 2055 19.4 -> 17.0 us, of which the steps
 // take 0.21 us each, what the matrix units need and L2 gives; where two fit a CU two buffers are faster (26 and
 // 20 us for a product of 315 workgroups).
@@ -868,7 +874,9 @@ __device__ __forceinline__ bool infinities(const Source &s, int64_t R, int64_t r
 // row of 128 bytes, and each wave splits its fragments on the way to the matrix units: 44 vector instructions a fragment
 // beside the 12 matrix instructions it feeds, which the two units of a SIMD run side by side.  (Parts written to memory
 // as three planes first were 10 bytes an element of extra traffic and half again as many through L2: forward and backward
-// of 8192 x 1024 x 512 took 221 us.)  `a` describes the operands as they came, sa and sb as they are read.
+// of 8192 x 1024 x 512 took 221 us, 195 now: forward 64, dx 56, dW 56.)  Instruction issue bounds it: a matrix
+// instruction (16 cycles) and its 3.7 vector instructions (15) take 34 cycles of a SIMD with two waves, 50 of one with a
+// lone wave, however the two kinds are ordered.  `a` describes the operands as they came, sa and sb as they are read.
 template <Kind KA, Kind KB>
 __global__ __launch_bounds__(256, 2) void direct32_kernel(LinArgs a, Source sa, Source sb)
 {
@@ -975,7 +983,8 @@ __global__ __launch_bounds__(256, 2) void direct32_kernel(LinArgs a, Source sa, 
 
 // An operand for the direct kernels, [rows, cols] -> [rows, ldp], zeros behind cols.  src: x itself, dy with z or its
 // derivative codes (dz = dy f'(z); with `partial`, also the partial column sums of dz in FP32), or an 8-bit checkpoint.
-// rows_per rows a workgroup of 64 lanes (8 columns each) by 4 rows.  out may be NULL (db alone).
+// rows_per rows a workgroup of 64 lanes (8 columns each) by 4 rows.  out may be NULL (db alone).  HBM bounds it: dz of
+// 16384 x 4096 in BF16 from derivative codes 71 us (4.7 TB/s), an 8-bit x 42 us (4.8 TB/s).
 enum Made { COPY, DZ, EIGHT };
 struct PrepArgs {
     const void *src, *pre;
@@ -1109,7 +1118,8 @@ __global__ __launch_bounds__(THREADS) void db_kernel(const float *__restrict__ p
 // steps' loads together (FP32 by its own matrix instruction: memory, not arithmetic, bounds this).  The workgroup's
 // waves take steps of l in turn and are summed in LDS, wave by wave.  It reads A again for every 16 columns and B for
 // every 32 rows, so beyond 32 rows only products too small for that to matter take it: one round of loads, where
-// a tile waits for one after the other.
+// a tile waits for one after the other.  One row of 4096 -> 4096 in BF16: 8.7 us (3.9 TB/s); 100 rows of 128 -> 64 in
+// FP32: 4.1 us.
 template <class T, int WAVES, int GROUPS>
 __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinArgs a)
 {

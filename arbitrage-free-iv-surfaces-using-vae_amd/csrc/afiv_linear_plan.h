@@ -48,8 +48,8 @@ Plan direct_plan(int64_t R, int64_t C, int64_t L, bool f32)
 }
 
 // What the direct kernel takes: at least a tile each way, rows within 2^31 bytes of a tile's corner, and enough work that
-// its few, large tiles fill the chip (16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23 and 12; FP32:
-// 512^3 24 and 16, 4096 x 256 x 256 25 and 29).
+// its few, large tiles fill the chip (measured with two buffers; 16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23
+// and 12; FP32: 512^3 24 and 16, 4096 x 256 x 256 25 and 29).
 bool direct_takes(int64_t R, int64_t C, int64_t L, bool f32)
 {
     return R >= 128 && C >= 128 && L >= 128 && (double)R * (double)C * (double)L >= (f32 ? 1 << 28 : 1 << 27);
