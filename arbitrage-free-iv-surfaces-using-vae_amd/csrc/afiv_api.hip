@@ -725,7 +725,7 @@ int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes,
         if (!dy || (dx && !w) || (dw && !x && (!codes || !scales))) return AFIV_E_NULL;
         if (act != AFIV_ACT_NONE && !pre && !dcodes) return AFIV_E_NULL;
     }
-    const int64_t need = afiv_linear_backward_scratch(M, N, K, dtype, act, !x);
+    const int64_t need = afiv_linear_backward_scratch(M, N, K, dtype, act, dw && !x);
     if (need > 0 && (!scratch || scratch_bytes < need)) return AFIV_E_WORKSPACE;
     return afiv_launch_linear_act_backward(dy, x, x ? nullptr : codes, x ? nullptr : scales, w, pre, pre ? nullptr : dcodes, dtype, act, M,
                                            N, K, dx, dw, db, (float *)scratch, as_stream(stream));

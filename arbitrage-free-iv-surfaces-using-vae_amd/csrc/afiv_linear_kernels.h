@@ -301,6 +301,43 @@ struct Operand {
     }
 };
 
+// db without dW, where no pass over dz sums it: a workgroup sums 128 columns of dz over one run of rows and reads nothing
+// of the layer's input.  A lane holds what it would in the tile kernel (4 columns, every eighth quad of rows), and the runs
+// are that kernel's, so db has the same bits with and without dW.  block: runs by blocks of columns.
+template <class T>
+__device__ __forceinline__ void sum_dz(const LinArgs &a, int64_t block)
+{
+    typedef Operand<T, ACROSS_DZ, 128> Dz;
+    typedef Held<T, ACROSS_DZ> H;
+    static_assert(Dz::UNITS == THREADS, "a unit a thread");
+    __shared__ float lds[BK / 4][128];
+    int c, l;
+    Dz::place(threadIdx.x, c, l);
+    const int64_t blocks = (a.R + 127) / 128, split = block / blocks;
+    const int64_t col0 = (block - split * blocks) * 128, l_begin = split * a.l_per;
+    const int64_t l_end = l_begin + a.l_per < a.L ? l_begin + a.l_per : a.L;
+    float sums[4] = {};
+    Dz next;
+    if (l_begin < l_end) next.load(a, a.A, a.R, col0, l_begin, l_end, threadIdx.x);
+    for (int64_t l0 = l_begin; l0 < l_end; l0 += BK) {
+        const H h = next.h[0];
+        if (l0 + BK < l_end) next.load(a, a.A, a.R, col0, l0 + BK, l_end, threadIdx.x);
+        float f[H::N];
+        values<T, ACROSS_DZ>(a, h, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[j] += (f[j] + f[4 + j]) + (f[8 + j] + f[12 + j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lds[l / 4][c + j] = sums[j];
+    __syncthreads();
+    if (threadIdx.x < 128 && col0 + threadIdx.x < a.R) {
+        float t = 0.0f;
+        for (int i = 0; i < BK / 4; ++i) t += lds[i][threadIdx.x];
+        if (a.splits > 1) a.db_partial[split * a.R + col0 + threadIdx.x] = t;
+        else ((T *)a.db)[col0 + threadIdx.x] = (T)t;
+    }
+}
+
 // W outputs of row i from column j on, from their sums z.  EPI: the forward epilogue.
 template <class T, bool EPI, int W>
 __device__ __forceinline__ void finish(const LinArgs &a, int64_t i, int64_t j, float (&z)[W])
@@ -340,7 +377,7 @@ __device__ __forceinline__ void finish(const LinArgs &a, int64_t i, int64_t j, f
     Pack<T, W> o;
 #pragma unroll
     for (int q = 0; q < W; ++q) o.v[q] = (T)z[q];
-    if (EPI || a.out) store_some<T, W>((T *)a.out + at, o, n);      // no out: only db was asked for
+    store_some<T, W>((T *)a.out + at, o, n);
 }
 
 // A wave's 16 TR x 16 TC outputs from its accumulators (lane = row lane & 15, four columns from 4 (lane >> 4) of
@@ -594,6 +631,21 @@ __global__ __launch_bounds__(THREADS) void both_kernel(LinArgs dx, LinArgs dw, i
     const int64_t block = blockIdx.x;
     if (block < dx_blocks) tile<T, ALONG_DZ, ACROSS, 2, 2>(dx, block, dx_blocks);
     else tile<T, ACROSS_DZ, KX, 2, 2>(dw, block - dx_blocks, gridDim.x - dx_blocks);
+}
+
+template <class T>
+__global__ __launch_bounds__(THREADS) void db_alone_kernel(LinArgs dw)
+{
+    sum_dz<T>(dw, blockIdx.x);
+}
+
+// dx and db in one launch, as above
+template <class T>
+__global__ __launch_bounds__(THREADS) void dx_db_kernel(LinArgs dx, LinArgs dw, int64_t dx_blocks)
+{
+    const int64_t block = blockIdx.x;
+    if (block < dx_blocks) tile<T, ALONG_DZ, ACROSS, 2, 2>(dx, block, dx_blocks);
+    else sum_dz<T>(dw, block - dx_blocks);
 }
 
 // The splits' sums, in a fixed order, and the epilogue: SLICES threads an output of four columns, each over every
@@ -1231,6 +1283,23 @@ int products(LinArgs d, LinArgs e, float *scratch, hipStream_t s)
     return ok();
 }
 
+// db of e (dW's arguments, of which dW is not wanted) and dx, if d describes it
+template <class T>
+int db_alone(const LinArgs *d, LinArgs e, float *scratch, hipStream_t s)
+{
+    tiled(e, d ? scratch + tile_floats(d->R, d->C, d->L) : scratch);
+    const int64_t blocks = (e.R + 127) / 128 * e.splits;
+    if (d) {
+        LinArgs dx = *d;
+        const int64_t dx_blocks = tiled(dx, scratch);
+        hipLaunchKernelGGL(dx_db_kernel<T>, dim3((unsigned)(dx_blocks + blocks)), dim3(THREADS), 0, s, dx, e, dx_blocks);
+        if (dx.splits > 1) join<T, false>(dx, s);
+    } else hipLaunchKernelGGL(db_alone_kernel<T>, dim3((unsigned)blocks), dim3(THREADS), 0, s, e);
+    if (e.splits > 1)
+        hipLaunchKernelGGL(db_kernel<T>, dim3((unsigned)((e.R + 15) / 16)), dim3(THREADS), 0, s, e.db_partial, e.splits, e.R, (T *)e.db);
+    return ok();
+}
+
 template <class T, Kind KA, Kind KB>
 int direct(LinArgs a, const Source &sa, const Source &sb, float *scratch, hipStream_t s)
 {
@@ -1333,7 +1402,7 @@ int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *
     // operands that the direct kernel cannot read in place are written first; a misaligned one of a kind that it
     // could sends the product to the tile kernel
     constexpr int WHOLE = 16 / sizeof(T);
-    const Places p = backward_places(M, N, K, sizeof(T) == 4, act != AFIV_ACT_NONE, !x);
+    const Places p = backward_places(M, N, K, sizeof(T) == 4, act != AFIV_ACT_NONE, dw && !x);
     char *const at = (char *)scratch;
     const bool make_dz = act != AFIV_ACT_NONE || N % WHOLE, make_x = codes || K % WHOLE;
     const bool ready = aligned(scratch) && (make_dz || aligned(dy));
@@ -1352,13 +1421,16 @@ int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *
         if (sums) hipLaunchKernelGGL(db_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(THREADS), 0, s, partial, prep_chunks(M, N), N, (T *)db);
     }
     int rc = ok();
-    if (!rc && dx && M > 0 && (dw || (db && !sums)) && !direct_dx && !direct_dw)
+    const bool only_db = !dw && db && !sums;                     // the input may be missing: no product with it
+    if (!rc && dx && M > 0 && only_db && !direct_dx) return db_alone<T>(&d, e, scratch, s);
+    if (!rc && dx && M > 0 && dw && !direct_dx && !direct_dw)
         return codes ? products<T, ACROSS_EIGHT>(d, e, scratch, s) : products<T, ACROSS>(d, e, scratch, s);
     if (!rc && dx) {
         if (direct_dx) rc = direct<T, ALONG_DZ, ACROSS>(d, g, plain_source<T>(w, N, K, p.w, at, s), scratch, s);
         else rc = product<T, ALONG_DZ, ACROSS>(d, scratch, s);
     }
-    if (rc || (!dw && (!db || sums))) return rc;
+    if (!rc && only_db) rc = db_alone<T>(nullptr, e, scratch, s);
+    if (rc || !dw) return rc;
     if (!direct_dw) return codes ? product<T, ACROSS_DZ, ACROSS_EIGHT>(e, scratch, s) : product<T, ACROSS_DZ, ACROSS>(e, scratch, s);
     if (!codes) {
         const Room none = {};

@@ -288,10 +288,11 @@ int afiv_linear_act(const void *x, const void *w, const void *bias, const void *
 /* Gradients of afiv_linear_act from dy [M,N] T: dx [M,K], dw [N,K], db [N], all T, each NULL if not
  * wanted (the residual's gradient is dy).  The layer's input comes as x [M,K] T or, with x == NULL, as
  * its 8-bit checkpoint (codes, scales); the derivative from pre [M,N] T or, with pre == NULL, from
- * dcodes [M,N] (neither for AFIV_ACT_NONE).  w is needed for dx, the input for dw.  dy times the
- * derivative is rounded to T before the products (FP32: not rounded), db is summed before that rounding. */
+ * dcodes [M,N] (neither for AFIV_ACT_NONE).  w is needed for dx, the input (x, or codes and scales) for
+ * dw; db reads neither.  dy times the derivative is rounded to T before the products (FP32: not
+ * rounded), db is summed before that rounding. */
 /* scratch: 16-byte aligned, at least afiv_linear_act_backward_scratch(M, N, K, dtype, act, from_checkpoint) bytes (NULL where
- * that is 0; from_checkpoint: x will be NULL).  Large products keep there, during the call, what they cannot read in
+ * that is 0; from_checkpoint: x will be NULL and dw is wanted).  Large products keep there, during the call, what they cannot read in
  * place: dz [M,N], the restored x [M,K], rows that are not whole 16-byte chunks. */
 int64_t afiv_linear_act_backward_scratch(int64_t M, int64_t N, int64_t K, int dtype, int act, int from_checkpoint);
 int afiv_linear_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const void *w, const void *pre,

@@ -1,0 +1,59 @@
+"""GPU tests of calls of the layer operators that the header and the docstrings allow beside the usual ones: gradients
+without the operands they do not need, through the C ABI."""
+import ctypes
+
+import pytest
+import torch
+
+from test_gpu_layers import TYPES, U, check_backward, half, inputs, tiny, within
+
+pytestmark = pytest.mark.gpu
+
+
+def abi_backward(afiv, dy, w, saved, k, dx=False, codes=None):
+    """(dx, db) through the C ABI with no dW and no input (codes: a pointer without scales)."""
+    lib, (m, n), t = afiv._lib.lib(), dy.shape, dy.dtype
+
+    def p(v):
+        return None if v is None else ctypes.c_void_p(v.data_ptr())
+    out = torch.full((m, k), float("nan"), dtype=t, device="cuda") if dx else None
+    db = torch.full((n,), float("nan"), dtype=t, device="cuda")
+    dtype, act = afiv.layers.DTYPES[t], afiv.layers.ACTIVATIONS[saved.act]
+    need = lib.afiv_linear_act_backward_scratch(m, n, k, dtype, act, 0)
+    scratch = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    rc = lib.afiv_linear_act_backward(p(dy), None, p(codes), None, p(w) if dx else None, p(saved.pre), p(saved.dcodes), dtype, act, m, n, k,
+                                      p(out), None, p(db), p(scratch) if need else None, need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    return out, db
+
+
+# products of every kind: one tile, a sum cut into runs (up to 16 of them, and more), many tiles, a pass over dz that sums it
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (2, 5, 3), (64, 13, 128), (300, 40, 50), (33, 64, 129), (2500, 24, 130), (40000, 64, 5), (40000, 24, 72),
+                                   (700, 1030, 1100), (1999, 1001, 515), (0, 4, 5)])
+def test_db_without_the_layers_input(afiv, typ, m, k, n):
+    for act, eight in (("none", False), ("gelu", False), ("silu", True), ("relu", False)):
+        x, w, b, _, dy = inputs(TYPES[typ], m, k, n, 7)
+        _, saved = afiv.linear_act_forward(x, w, b, act=act, checkpoint8=eight)
+        every = afiv.linear_act_backward(dy, w, saved)
+        if m:
+            check_backward(dy, w, saved, act, *every)
+        codes = torch.zeros(max(m * k, 1), dtype=torch.int8, device="cuda")
+        for want_dx, c in ((False, None), (True, None), (False, codes)):
+            dx, db = abi_backward(afiv, dy, w, saved, k, want_dx, c)
+            assert torch.equal(db, every[2]), (act, want_dx)
+            assert not want_dx or torch.equal(dx, every[0])
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_db_without_the_layers_input_of_a_misaligned_gradient(afiv, typ):
+    """A size whose dz is read in place, from an address that is no multiple of 16."""
+    t = TYPES[typ]
+    m, k, n = 1500, 520, 1032
+    x, w, b, _, dy = inputs(t, m, k, n, 8)
+    off = torch.empty(m * n + 1, dtype=t, device="cuda")[1:].view(m, n).copy_(dy)
+    _, saved = afiv.linear_act_forward(x, w, b)
+    _, db = abi_backward(afiv, off, w, saved, k)
+    want, tol = dy.double().sum(0), 2 * m * U * dy.double().abs().sum(0)
+    within(db, want, tol + (want.abs() + tol) * half(t) + tiny(t), "db")
+    assert torch.equal(db, afiv.linear_act_backward(off, w, saved)[2])
