@@ -100,7 +100,8 @@ class ConditionalVAE_SingleHeston(nn.Module):
         """``stack(h)`` on the layer operators.  A block is [Linear, BatchNorm1d, activation, Dropout]:
         training takes the linear layer, then normalisation, activation and dropout in one operator; with
         frozen statistics the normalisation is an affine map of the linear layer's output, folded into
-        its weight and bias, and the activation is that layer's epilogue."""
+        its weight and bias, and the activation is that layer's epilogue; a Dropout that is training
+        follows by itself."""
         layers, i = list(stack), 0
         while i < len(layers):
             lin, bn = layers[i], layers[i + 1] if i + 1 < len(layers) else None
@@ -108,17 +109,21 @@ class ConditionalVAE_SingleHeston(nn.Module):
                 h, i = self._linear(lin, h), i + 1
                 continue
             name = next(k for k, kind in _ACTIVATION_TYPES.items() if isinstance(layers[i + 2], kind))
-            drop = layers[i + 3].p if i + 3 < len(layers) and isinstance(layers[i + 3], nn.Dropout) else None
+            drop = layers[i + 3] if i + 3 < len(layers) and isinstance(layers[i + 3], nn.Dropout) else None
+            p = drop.p if drop is not None and drop.training else 0.0        # its own mode, not the normalisation's
             if bn.training:
                 h = self._linear(lin, h)
-                keep = torch.rand(h.shape, device=h.device) >= drop if drop else None
+                keep = torch.rand(h.shape, device=h.device) >= p if 0.0 < p < 1.0 else None
                 bn.num_batches_tracked.add_(1)
                 h = _afiv.batch_norm_act(h, bn.weight, bn.bias, bn.running_mean, bn.running_var, act=name, keep=keep,
-                                         drop_p=drop or 0.0, momentum=bn.momentum, eps=bn.eps, checkpoint8=self.checkpoint8)
+                                         drop_p=0.0 if keep is None else p, momentum=bn.momentum, eps=bn.eps, checkpoint8=self.checkpoint8)
+                p = p if keep is None else 0.0
             else:
                 a = bn.weight * torch.rsqrt(bn.running_var + bn.eps)
                 h = _afiv.linear_act(h, lin.weight * a[:, None], (lin.bias - bn.running_mean) * a + bn.bias, act=name,
                                      checkpoint8=self.checkpoint8)
+            if p:
+                h = F.dropout(h, p)
             i += 3 if drop is None else 4
         return h
 
