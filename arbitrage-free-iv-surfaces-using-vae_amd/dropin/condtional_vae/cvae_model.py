@@ -111,12 +111,18 @@ class ConditionalVAE_SingleHeston(nn.Module):
             name = next(k for k, kind in _ACTIVATION_TYPES.items() if isinstance(layers[i + 2], kind))
             drop = layers[i + 3] if i + 3 < len(layers) and isinstance(layers[i + 3], nn.Dropout) else None
             p = drop.p if drop is not None and drop.training else 0.0        # its own mode, not the normalisation's
-            if bn.training:
+            if bn.training or bn.running_mean is None:
                 h = self._linear(lin, h)
                 keep = torch.rand(h.shape, device=h.device) >= p if 0.0 < p < 1.0 else None
-                bn.num_batches_tracked.add_(1)
-                h = _afiv.batch_norm_act(h, bn.weight, bn.bias, bn.running_mean, bn.running_var, act=name, keep=keep,
-                                         drop_p=0.0 if keep is None else p, momentum=bn.momentum, eps=bn.eps, checkpoint8=self.checkpoint8)
+                mean = var = None
+                momentum = 0.0 if bn.momentum is None else bn.momentum
+                if bn.training and bn.track_running_stats and bn.running_mean is not None:
+                    mean, var = bn.running_mean, bn.running_var
+                    bn.num_batches_tracked.add_(1)
+                    if bn.momentum is None:                              # a mean over all batches
+                        momentum = 1.0 / float(bn.num_batches_tracked)
+                h = _afiv.batch_norm_act(h, bn.weight, bn.bias, mean, var, act=name, keep=keep,
+                                         drop_p=0.0 if keep is None else p, momentum=momentum, eps=bn.eps, checkpoint8=self.checkpoint8)
                 p = p if keep is None else 0.0
             else:
                 a = bn.weight * torch.rsqrt(bn.running_var + bn.eps)

@@ -88,3 +88,34 @@ def test_gradients_with_frozen_statistics_and_dropout(cvae):
         run(model).square().sum().backward()
     for (name, u), v in zip(b.encoder.named_parameters(), a.encoder.parameters()):
         close(u.grad, v.grad, name)
+
+
+@pytest.mark.parametrize("momentum,tracks", [(None, True), (0.3, True), (0.1, False), (None, False)])
+def test_running_statistics_rules_of_the_module(cvae, momentum, tracks):
+    a, b = pair(cvae, dropout=0.0)
+    for model in (a, b):
+        for m in model.modules():
+            if isinstance(m, torch.nn.BatchNorm1d):
+                m.momentum, m.track_running_stats = momentum, tracks
+    batches = [torch.randn(20, 13, dtype=torch.float64) + i for i in range(3)]
+    for model, run in ((a, lambda h: a.encoder(h)), (b, lambda h: b._run_stack(b.encoder, h))):
+        model.train()
+        for h in batches:
+            run(h)
+    for (name, u), v in zip(b.named_buffers(), a.buffers()):
+        close(u.double(), v.double(), name)
+    a.eval(), b.eval()
+    close(b._run_stack(b.encoder, batches[0]), a.encoder(batches[0]))
+
+
+def test_statistics_that_are_not_kept(cvae):
+    """Without running statistics the batch's own serve in evaluation too."""
+    a, b = pair(cvae, dropout=0.0)
+    for model in (a, b):
+        for m in model.modules():
+            if isinstance(m, torch.nn.BatchNorm1d):
+                m.track_running_stats, m.running_mean, m.running_var, m.num_batches_tracked = False, None, None, None
+    h = torch.randn(20, 13, dtype=torch.float64)
+    for mode in (True, False):
+        a.train(mode), b.train(mode)
+        close(b._run_stack(b.encoder, h), a.encoder(h))
