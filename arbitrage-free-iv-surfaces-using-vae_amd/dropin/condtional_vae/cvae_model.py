@@ -93,7 +93,16 @@ class ConditionalVAE_SingleHeston(nn.Module):
             raise ValueError(f"Unknown activation: {name}")
 
     # ---- stacks on the layer operators -----------------------------------------------------
+    @staticmethod
+    def _without_hooks(*modules):
+        """The operators read the modules' weights and never call them, so a hook would be skipped."""
+        for m in modules:
+            if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
+                raise RuntimeError(f"layer_kernels=True does not call {type(m).__name__}, whose hooks would not run: "
+                                   "remove them or use layer_kernels=False")
+
     def _linear(self, layer, h, act="none"):
+        self._without_hooks(layer)
         return _afiv.linear_act(h, layer.weight, layer.bias, act=act, checkpoint8=self.checkpoint8)
 
     def _run_stack(self, stack, h):
@@ -103,6 +112,7 @@ class ConditionalVAE_SingleHeston(nn.Module):
         its weight and bias, and the activation is that layer's epilogue; a Dropout that is training
         follows by itself."""
         layers, i = list(stack), 0
+        self._without_hooks(stack, *layers)
         while i < len(layers):
             lin, bn = layers[i], layers[i + 1] if i + 1 < len(layers) else None
             if not isinstance(bn, nn.BatchNorm1d):

@@ -119,3 +119,16 @@ def test_statistics_that_are_not_kept(cvae):
     for mode in (True, False):
         a.train(mode), b.train(mode)
         close(b._run_stack(b.encoder, h), a.encoder(h))
+
+
+@pytest.mark.parametrize("register", ["register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"])
+def test_hooks_are_refused_not_skipped(cvae, register):
+    """The modules are never called, so a hook on one of them could not run."""
+    _, b = pair(cvae, dropout=0.5)
+    h = torch.randn(20, 13, dtype=torch.float64)
+    for module, call in [(m, lambda: b._run_stack(b.encoder, h)) for m in (b.encoder, *b.encoder)] + [(b.fc_mu, lambda: b._linear(b.fc_mu, h[:, :b.fc_mu.in_features]))]:
+        handle = getattr(module, register)(lambda *args: None)
+        with pytest.raises(RuntimeError, match="hooks"):
+            call()
+        handle.remove()
+    assert b._run_stack(b.encoder, h).shape[0] == 20
