@@ -119,6 +119,8 @@ class ConditionalVAE_SingleHeston(nn.Module):
                 h, i = self._linear(lin, h), i + 1
                 continue
             name = next(k for k, kind in _ACTIVATION_TYPES.items() if isinstance(layers[i + 2], kind))
+            if name == "leaky_relu" and layers[i + 2].negative_slope != 0.2:
+                raise ValueError(f"layer_kernels=True has leaky_relu with slope 0.2 only, got {layers[i + 2].negative_slope}")
             drop = layers[i + 3] if i + 3 < len(layers) and isinstance(layers[i + 3], nn.Dropout) else None
             p = drop.p if drop is not None and drop.training else 0.0        # its own mode, not the normalisation's
             if bn.training or bn.running_mean is None:

@@ -132,3 +132,13 @@ def test_hooks_are_refused_not_skipped(cvae, register):
             call()
         handle.remove()
     assert b._run_stack(b.encoder, h).shape[0] == 20
+
+
+def test_another_slope_is_refused(cvae):
+    """The operators' leaky_relu has one slope; the module's may be set."""
+    _, b = pair(cvae, dropout=0.0, encoder_activation="leaky_relu")
+    h = torch.randn(20, 13, dtype=torch.float64)
+    b._run_stack(b.encoder, h)
+    next(m for m in b.encoder if isinstance(m, torch.nn.LeakyReLU)).negative_slope = 0.1
+    with pytest.raises(ValueError, match="slope"):
+        b._run_stack(b.encoder, h)
