@@ -54,6 +54,8 @@ def _stack(widths, act, dropout):
 
 
 class ConditionalVAE_SingleHeston(nn.Module):
+    layer_kernels = checkpoint8 = False      # models pickled before these arguments existed carry neither
+
     def __init__(self, param_dim=5, conditioning_dim=8, latent_dim=4, hidden_dims=[128, 64, 32],
                  encoder_activation="tanh", decoder_activation="relu", dropout=0.15,
                  feller_penalty_weight=1.0, beta=0.1, arbitrage_penalty_weight=2.0,

@@ -142,3 +142,13 @@ def test_another_slope_is_refused(cvae):
     next(m for m in b.encoder if isinstance(m, torch.nn.LeakyReLU)).negative_slope = 0.1
     with pytest.raises(ValueError, match="slope"):
         b._run_stack(b.encoder, h)
+
+
+def test_models_pickled_without_the_option(cvae):
+    """A whole model pickled before the option existed has none of its attributes: it runs on its torch layers."""
+    a, _ = pair(cvae, dropout=0.0)
+    del a.__dict__["layer_kernels"], a.__dict__["checkpoint8"]
+    a.train()
+    x, c, z = (torch.randn(6, k, dtype=torch.float64) for k in (5, 8, 4))
+    a.encode(x, c)
+    a.decode(z, c)
