@@ -3,8 +3,8 @@ batch normalisation with activation and dropout; 8-bit activation checkpoints.
 
 These are the pieces of the conditional VAE's [Linear, BatchNorm1d, activation, Dropout] stacks
 (cvae_model.py:64-105), forward and backward, for layers of any width.  ``linear_act`` and
-``batch_norm_act`` are differentiable; their ``_forward`` / ``_backward`` halves are for training loops
-that hold the backward pass themselves (graph capture, pipelines).  Every function takes CUDA tensors
+``batch_norm_act`` are differentiable in reverse mode; their ``_forward`` / ``_backward`` halves are for training
+loops that hold the backward pass themselves (graph capture, pipelines).  Forward-mode tangents are refused.  Every function takes CUDA tensors
 in float32, bfloat16 or float16, enqueues on torch's current stream of the tensors' device and does not
 synchronise.  Inputs that are not contiguous are copied first.
 """
@@ -14,6 +14,7 @@ from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -46,10 +47,17 @@ def _act(name: str) -> int:
         raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
 
 
+def _is_plain(t, what: str) -> None:
+    """A tensor without a forward-mode tangent: the kernels would drop it, which reads as a derivative of zero."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a torch.Tensor")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what} has a forward-mode tangent: the layer operators differentiate in reverse mode only")
+
+
 def _first(x, what: str) -> torch.Tensor:
     """The operand that sets the device and the element type."""
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{what} must be a torch.Tensor")
+    _is_plain(x, what)
     if not x.is_cuda:
         raise ValueError(f"{what} is on {x.device}: the layer kernels need a GPU (no CPU fallback)")
     if x.dtype not in DTYPES:
@@ -65,8 +73,7 @@ def _plain(t: torch.Tensor) -> torch.Tensor:
 
 def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = False) -> torch.Tensor:
     """Another operand: on x's device, of x's type (or one of ``dtypes``), of the given shape."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{what} must be a torch.Tensor")
+    _is_plain(t, what)
     if t.get_device() != x.get_device():
         raise ValueError(f"{what} is on {t.device}, expected {x.device}")
     if (t.dtype != x.dtype) if dtypes is None else (t.dtype not in dtypes):
@@ -264,6 +271,11 @@ class _LinearAct(torch.autograd.Function):
 
 
 def _graph(*tensors) -> bool:
+    """Whether autograd records the call."""
+    if forward_ad._current_level >= 0:                   # inside Function.apply tangents can no longer be seen
+        for t in tensors:
+            if isinstance(t, torch.Tensor):
+                _is_plain(t, "an operand")
     if torch.is_grad_enabled():
         for t in tensors:
             if isinstance(t, torch.Tensor) and t.requires_grad:

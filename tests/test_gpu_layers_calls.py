@@ -57,3 +57,36 @@ def test_db_without_the_layers_input_of_a_misaligned_gradient(afiv, typ):
     want, tol = dy.double().sum(0), 2 * m * U * dy.double().abs().sum(0)
     within(db, want, tol + (want.abs() + tol) * half(t) + tiny(t), "db")
     assert torch.equal(db, afiv.linear_act_backward(off, w, saved)[2])
+
+
+def test_transforms_that_the_operators_do_not_know(afiv):
+    """Forward-mode tangents, and torch.func's wrapped tensors, are refused on every operand; nothing is computed from them."""
+    from torch.autograd import forward_ad
+    x, w, b, r, dy = inputs(torch.float32, 6, 5, 4, 1, residual=True)
+    gamma, beta = torch.ones(5, device="cuda"), torch.zeros(5, device="cuda")
+    mean, var = torch.zeros(5, device="cuda"), torch.ones(5, device="cuda")
+    _, saved = afiv.linear_act_forward(x, w, b, act="tanh")
+    _, norm = afiv.batch_norm_act_forward(x, gamma, beta, act="tanh")
+    linear = lambda *a: afiv.linear_act(a[0], a[1], a[2], residual=a[3], act="tanh")      # noqa: E731
+    bn = lambda *a: afiv.batch_norm_act(*a, mean, var, act="tanh")                        # noqa: E731
+    for call, args in ((linear, (x, w, b, r)), (bn, (x, gamma, beta)), (lambda *a: afiv.linear_act_backward(*a, saved)[0], (dy, w)),
+                       (lambda *a: afiv.batch_norm_act_backward(*a, norm)[0], (x, gamma, beta))):
+        for i in range(len(args)):
+            for grad in (False, True):
+                with forward_ad.dual_level():
+                    a = [v.clone().requires_grad_(grad) for v in args]
+                    a[i] = forward_ad.make_dual(a[i], torch.ones_like(a[i]))
+                    with pytest.raises(NotImplementedError, match="tangent"):
+                        call(*a)
+            rest = list(args)
+
+            def one(v):
+                return call(*rest[:i], v, *rest[i + 1:])
+            with pytest.raises(NotImplementedError, match="tangent"):
+                torch.func.jvp(one, (args[i],), (torch.ones_like(args[i]),))
+    for call, args in ((linear, (x, w, b, r)), (bn, (x, gamma, beta))):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda v: call(v, *args[1:]).sum())(x)
+        with pytest.raises(RuntimeError):
+            torch.vmap(lambda v: call(v, *args[1:]))(torch.stack([x, x]))
+    assert not mean.any() and bool((var == 1).all())

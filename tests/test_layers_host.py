@@ -123,3 +123,23 @@ def test_abi_limits_match_the_wrappers(afiv):
         assert re.search(r"AFIV_ACT_%s = %d\b" % (name.upper(), value), text)
     for name, value in (("F32", 0), ("BF16", 1), ("F16", 2)):
         assert re.search(r"AFIV_%s = %d\b" % (name, value), text)
+
+
+def test_forward_mode_tangents_are_refused(afiv):
+    """A tangent that an operator cannot carry on must not vanish.  (Operands beside the first need a GPU: test_gpu_layers_calls.py.)"""
+    from torch.autograd import forward_ad
+    x, w = torch.randn(4, 8), torch.randn(3, 8)
+    calls = (afiv.checkpoint8, lambda v: afiv.linear_act(v, w), lambda v: afiv.linear_act_forward(v, w),
+             lambda v: afiv.batch_norm_act(v, torch.ones(8), torch.zeros(8)))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+                call(dual)
+            with pytest.raises(ValueError, match="no CPU fallback"):          # a tensor without one goes on to the next check
+                call(x)
+    for call in calls:
+        with pytest.raises(NotImplementedError, match="tangent"):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
