@@ -80,8 +80,11 @@ __device__ __forceinline__ void store_some(T *p, const Pack<T, N> &r, int n)
 constexpr float AFIV_SLOPE = 0.2f;      // leaky_relu: the slope of the reference's stacks (cvae_model.py:118)
 
 // f(z) and f'(z); whichever the caller drops costs nothing.  Built on the hardware's 2^x and reciprocal (1 ulp
-// each) and, for erfc, a polynomial: within 7e-7 of the value (12 FP32 half steps) at a third of the library
-// functions' instructions, which an epilogue of 128 outputs a lane feels.
+// each) and, for erfc, a polynomial, at a third of the library functions' instructions, which an epilogue of 128
+// outputs a lane feels.  Relative errors, in FP32 half steps (2^-24): gelu 16 + 1.5 z^2, silu 8 + 2 |z|, tanh' 12 + 4 |z|,
+// gelu' and silu' as gelu and silu, of the sum of their terms' magnitudes.  The growing part comes from the exponent
+// alone: its two or three roundings stand for a number that 2^x multiplies up, and it is only felt where f or f' is about
+// to vanish; in absolute terms all are within a few half steps of max(1, |z|).
 template <int ACT>
 __device__ __forceinline__ void act_both(float z, float &f, float &d)
 {

@@ -90,3 +90,32 @@ def test_transforms_that_the_operators_do_not_know(afiv):
         with pytest.raises(RuntimeError):
             torch.vmap(lambda v: call(v, *args[1:]))(torch.stack([x, x]))
     assert not mean.any() and bool((var == 1).all())
+
+
+# Relative errors in FP32 half steps: f = (constant of 2^x, the reciprocal, the polynomial and a handful of roundings)
+# + (two or three roundings of the exponent's argument, multiplied up by the argument: z^2 / 2 of exp(-z^2 / 2), |z| of
+# exp(-|z|), 2 |z| of exp(-2 |z|))
+@pytest.mark.parametrize("m", [30, 4000])
+def test_activations_keep_their_relative_accuracy_in_the_tails(afiv, m):
+    one = torch.ones(1, 1, device="cuda")
+    for act, lo, hi in (("gelu", -12.0, 6.0), ("silu", -80.0, 20.0), ("tanh", -30.0, 30.0)):
+        x = torch.linspace(lo, hi, m, device="cuda").view(m, 1) + 1e-3          # with one weight of 1 the pre-activation is x itself
+        y, saved = afiv.linear_act_forward(x, one, act=act)
+        assert torch.equal(saved.pre, x)
+        d = afiv.linear_act_backward(torch.ones_like(x), one, saved, (True, False, False))[0].double()
+        z, y = x.double(), y.double()
+        a = z.abs()
+        if act == "gelu":
+            tail = 0.5 * torch.special.erfcx(a / 2 ** 0.5) * torch.exp(-z * z / 2)
+            phi, pdf = torch.where(z > 0, 1 - tail, tail), torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+            value, slope, terms, steps, dsteps = z * phi, phi + z * pdf, phi + a * pdf, 16 + 1.5 * z * z, 16 + 1.5 * z * z
+        elif act == "silu":
+            p, q = 1 / (1 + torch.exp(-z)), 1 / (1 + torch.exp(z))
+            value, slope, terms, steps, dsteps = z * p, p + z * p * q, p + a * p * q, 8 + 2 * a, 8 + 2 * a
+        else:
+            e = torch.exp(-2 * a)
+            value, slope = torch.tanh(z), 4 * e / (1 + e) ** 2
+            terms, steps, dsteps = slope, 16.0, 12 + 4 * a
+        for got, want, tol, what in ((y, value, steps * U * value.abs(), "value"), (d, slope, dsteps * U * terms, "derivative")):
+            off = (got - want).abs() / tol
+            assert float(off.max()) <= 1, (act, what, float(off.max()), float(z.flatten()[off.argmax()]))
