@@ -215,7 +215,7 @@ def linear_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     """``act(x @ weight.T + bias) + residual`` and what its backward pass needs: (y, LinearSaved).
     x [..., in], weight [out, in], bias [out], residual [..., out], all of one type.  With ``checkpoint8``
     the input and the activation's derivative are kept in 8 bits (33/32 and 1 byte an element);
-    otherwise they are the input itself and the pre-activation in x's type (relu, leaky_relu: its sign,
+    otherwise they are the input itself and the pre-activation rounded to x's type (relu, leaky_relu: its sign,
     one byte)."""
     signs = act in ("relu", "leaky_relu")
     want_codes = signs or (checkpoint8 and act != "none")
@@ -315,7 +315,8 @@ def batch_norm_act_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     """``keep / (1 - drop_p) * act(batch_norm(x))`` with the batch's own statistics, and what its backward pass
     needs: (y, NormSaved).  x [rows, features]; weight (gamma) and bias (beta) float32 [features]; running_mean and
     running_var (both or none) float32 [features], updated in place as nn.BatchNorm1d does; keep: bool or
-    uint8 mask of x's shape, needed where drop_p > 0.  With ``checkpoint8`` x is kept in 8 bits."""
+    uint8 mask of x's shape, needed where drop_p > 0.  With ``checkpoint8`` x is kept in 8 bits, and the backward
+    pass takes the activation's derivative from those (relu's side too)."""
     code = _act(act)
     v = _first(x, "x")
     if v.dim() != 2 or v.shape[1] < 1:

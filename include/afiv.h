@@ -254,7 +254,9 @@ int afiv_ensemble_stats_groups(const double *iv, const uint8_t *select, int64_t 
  * The reference runs them, and their gradients, in PyTorch on the CPU.  No object: weights are the
  * caller's device arrays, scratch too.  Outputs must not overlap inputs or each other, except where
  * said.  Arrays need no alignment beyond their elements'.  `dtype` is the element type of the arrays
- * written as [..] T; sums and everything between input and output are FP32 or wider. */
+ * written as [..] T; sums and what lies between input and output are FP32 or wider, except where said.
+ * FP32 products are sums of BF16 products of each factor's three parts: a product is off by up to
+ * 2^-21 of itself (2^-25 in the mean), and factors below 2^-110 keep fewer than 24 bits. */
 enum { AFIV_F32 = 0, AFIV_BF16 = 1, AFIV_F16 = 2 };
 enum {
     AFIV_ACT_NONE = 0,
@@ -278,7 +280,9 @@ int afiv_checkpoint8_restore(const int8_t *codes, const uint8_t *scales, int dty
 /* y [M,N] = act(x [M,K] w [N,K]^T + bias [N]) + residual [M,N], all T; bias and residual may be NULL.
  * For the backward pass one of these is kept, or both NULL: pre_out [M,N] T = the pre-activation, or
  * dcodes_out [M,N] = the activation's derivative in 8 bits (multiples of 1/200; relu and leaky_relu:
- * the sign; unused and may be NULL for AFIV_ACT_NONE).  M >= 0; 1 <= N, K <= 2^24.
+ * the sign; unused and may be NULL for AFIV_ACT_NONE).  pre_out rounds to T, and the backward pass takes the
+ * derivative there: off by up to |f''(z)| times half a step of T at z (tanh in BF16: up to 1.6 % of f' at
+ * |z| = 3).  M >= 0; 1 <= N, K <= 2^24.
  * scratch: 16-byte aligned device memory of at least afiv_linear_act_scratch(M, N, K, dtype) bytes (NULL where that
  * is 0). */
 int64_t afiv_linear_act_scratch(int64_t M, int64_t N, int64_t K, int dtype);
@@ -315,7 +319,9 @@ int afiv_norm_act(const void *x, const float *gamma, const float *beta, const ui
                   int8_t *codes_out, uint8_t *scales_out, double *scratch, void *stream);
 
 /* Gradients of afiv_norm_act from dy [M,N] T: dx [M,N] T (or NULL), dgamma, dbeta [N] float.  The input comes as
- * x [M,N] T or, with x == NULL, as its 8-bit checkpoint (codes, scales). */
+ * x [M,N] T or, with x == NULL, as its 8-bit checkpoint (codes, scales): then x's normalised value and the
+ * activation's derivative are those of the restored x, so an element whose pre-activation lies within
+ * the checkpoint's error of zero may take the other side of relu or leaky_relu than it did forward. */
 int afiv_norm_act_backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *scales, const float *gamma,
                            const float *beta, const uint8_t *keep, const double *stats, int dtype, int act, int64_t M, int64_t N,
                            double drop_p, void *dx, float *dgamma, float *dbeta, double *scratch, void *stream);

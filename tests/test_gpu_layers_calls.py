@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from test_gpu_layers import TYPES, U, check_backward, half, inputs, tiny, within
+from test_gpu_layers import ACTS, SECOND, TYPES, U, act64, check_backward, check_forward, der64, half, inputs, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +119,42 @@ def test_activations_keep_their_relative_accuracy_in_the_tails(afiv, m):
         for got, want, tol, what in ((y, value, steps * U * value.abs(), "value"), (d, slope, dsteps * U * terms, "derivative")):
             off = (got - want).abs() / tol
             assert float(off.max()) <= 1, (act, what, float(off.max()), float(z.flatten()[off.argmax()]))
+
+
+# The whole gradient, from the layer's inputs and not from what the forward pass saved: the saved pre-activation is rounded
+# to T (half(T) |z|, times f''), its side is FP32's (relu, leaky_relu), 8-bit derivatives are off by 1/400 and 8-bit inputs
+# by less than a step of their block
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("m,k,n", [(64, 40, 30), (1500, 264, 520), (1501, 261, 515)])
+def test_gradients_against_the_formula_from_the_inputs(afiv, typ, m, k, n, eight):
+    t = TYPES[typ]
+    for act in ACTS:
+        x, w, b, _, dy = inputs(t, m, k, n, 17)
+        _, saved = afiv.linear_act_forward(x, w, b, act=act, checkpoint8=eight)
+        dx, dw, db = afiv.linear_act_backward(dy, w, saved)
+        xd, wd, g = x.double(), w.double(), dy.double()
+        z, mag = xd @ wd.T + b.double(), xd.abs() @ wd.abs().T + b.double().abs()
+        zerr = (2 * k + 8) * U * mag
+        if act in ("relu", "leaky_relu"):
+            derr = torch.where(z.abs() <= zerr, 1.0, 0.0).double() + 2 * U
+        elif eight and act != "none":
+            derr = SECOND[act] * zerr + 16 * U * (1 + z.abs()) + 0.5 / 200 + 4 * U
+        else:
+            derr = SECOND[act] * (zerr + (z.abs() + zerr) * half(t) + tiny(t)) + 16 * U * (1 + z.abs())
+        if act == "none":
+            derr = torch.zeros_like(z)
+        dz = g * der64(z, act)
+        e = g.abs() * derr + 2 * U * dz.abs()
+        eh = e + (half(t) * (dz.abs() + e) + tiny(t) if act != "none" and t != torch.float32 else 0.0)
+        xerr = torch.zeros_like(xd)
+        if eight:
+            xerr = torch.exp2(saved.eight.scales.double() - 133).repeat_interleave(32, 1)[:, :k]
+        for got, a, c, err, length, what in ((dx, dz, wd, eh @ wd.abs(), n, "dx"),
+                                             (dw, dz.T, xd, eh.T @ (xd.abs() + xerr) + dz.abs().T @ xerr, m, "dw")):
+            want = a @ c
+            tol = err + (2 * length + 8) * U * (a.abs() @ c.abs() + err)
+            within(got, want, tol + (want.abs() + tol) * half(t) + tiny(t), what)
+        want = dz.sum(0)
+        tol = e.sum(0) + 2 * m * U * (dz.abs() + e).sum(0)
+        within(db, want, tol + (want.abs() + tol) * half(t) + tiny(t), "db")
