@@ -1,11 +1,13 @@
 """GPU tests of calls of the layer operators that the header and the docstrings allow beside the usual ones: gradients
 without the operands they do not need, through the C ABI."""
 import ctypes
+import dataclasses
+import types
 
 import pytest
 import torch
 
-from test_gpu_layers import ACTS, SECOND, TYPES, U, act64, check_backward, check_forward, der64, half, inputs, tiny, within
+from test_gpu_layers import ACTS, SECOND, TYPES, U, check_backward, check_forward, check_norm, der64, half, inputs, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +160,98 @@ def test_gradients_against_the_formula_from_the_inputs(afiv, typ, m, k, n, eight
         want = dz.sum(0)
         tol = e.sum(0) + 2 * m * U * (dz.abs() + e).sum(0)
         within(db, want, tol + (want.abs() + tol) * half(t) + tiny(t), "db")
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_large_products_of_misaligned_operands(afiv, typ):
+    """Sizes whose operands are read in place where they are aligned; here each in turn, and all, stand one element off."""
+    t = TYPES[typ]
+    m, k, n = 1500, 520, 1032
+    x, w, b, r, dy = inputs(t, m, k, n, 9, residual=True)
+
+    def off(v):
+        return torch.empty(v.numel() + 1, dtype=t, device="cuda")[1:].view(v.shape).copy_(v)
+    for which in ("x", "w", "dy", "all"):
+        xs, ws, ds = (off(v) if which in (name, "all") else v for name, v in (("x", x), ("w", w), ("dy", dy)))
+        bs, rs = (off(b), off(r)) if which == "all" else (b, r)
+        for act, eight in (("none", False), ("gelu", False), ("leaky_relu", True)):
+            y, saved = afiv.linear_act_forward(xs, ws, bs, residual=rs, act=act, checkpoint8=eight)
+            check_forward(x, w, b, r, act, y, saved)
+            check_backward(dy, w, saved, act, *afiv.linear_act_backward(ds, ws, saved))
+
+
+@pytest.mark.parametrize("typ,m,k,n", [("f16", 1501, 777, 1029), ("bf16", 2048, 512, 1024), ("f32", 2048, 260, 515)])
+def test_large_steps_in_graphs_and_on_streams(afiv, typ, m, k, n):
+    """Steps whose operands are prepared in scratch memory: two captured graphs replayed on new inputs, and two streams at
+    once, give the eager step's bits."""
+    def step(x, w, b, dy, act):
+        y, saved = afiv.linear_act_forward(x, w, b, act=act, checkpoint8=True)
+        return (y, *afiv.linear_act_backward(dy, w, saved))
+    acts = ("gelu", "tanh")
+    static = [[v for v in inputs(TYPES[typ], m, k, n, 50 + i) if v is not None] for i in range(2)]
+    step(*static[0], "gelu")
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s, act in zip(static, acts):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(*s, act))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for seed in (60, 70, 80):
+        news = [[v for v in inputs(TYPES[typ], m, k, n, seed + i) if v is not None] for i in range(2)]
+        for s, new in zip(static, news):
+            for a, c in zip(s, new):
+                a.copy_(c)
+        for g in graphs:
+            g.replay()
+        eager = [step(*new, act) for new, act in zip(news, acts)]
+        torch.cuda.synchronize()
+        at_once = []
+        for new, act, stream in zip(news, acts, streams):
+            with torch.cuda.stream(stream):
+                at_once.append(step(*new, act))
+        torch.cuda.synchronize()
+        for got in (outs, at_once):
+            assert all(torch.equal(a, c) for g, e in zip(got, eager) for a, c in zip(g, e))
+
+
+@pytest.mark.parametrize("k,n", [(264, 136), (261, 131)])
+def test_large_products_beyond_32_bits(afiv, k, n):
+    """More than 2^31 elements in x and dx, through the kernels for large products: rows at the start, about the 2^31st
+    element, about the 2^32nd byte and at the end; the others are zeros."""
+    m = (1 << 23) + 77
+    torch.manual_seed(13)
+    w = torch.randn(n, k, device="cuda").half()
+    x, dy = torch.zeros(m, k, dtype=torch.float16, device="cuda"), torch.zeros(m, n, dtype=torch.float16, device="cuda")
+    cross = (1 << 31) // k
+    rows = torch.cat([torch.arange(a, b, device="cuda") for a, b in ((0, 60), (cross // 2 - 40, cross // 2 + 40), (cross - 40, cross + 40), (m - 150, m))])
+    x[rows], dy[rows] = torch.randn(len(rows), k, device="cuda").half(), torch.randn(len(rows), n, device="cuda").half()
+    for eight in (False, True):
+        y, saved = afiv.linear_act_forward(x, w, act="relu", checkpoint8=eight)
+        assert int(y.any(1).sum()) == int(y[rows].any(1).sum())
+        dx, dw, db = afiv.linear_act_backward(dy, w, saved)
+        few = dataclasses.replace(afiv.linear_act_forward(x[rows], w, act="relu", checkpoint8=eight)[1], dcodes=saved.dcodes[rows])
+        check_forward(x[rows], w, None, None, "relu", y[rows], few)
+        assert not eight or torch.equal(saved.eight.codes[rows], few.eight.codes)
+        check_backward(dy[rows], w, few, "relu", dx[rows], dw, db)          # rows of zeros add nothing to dW and db
+        assert int(dx.any(1).sum()) == int(dx[rows].any(1).sum())
+        del y, dx, saved
+
+
+def test_norm_beyond_32_bits(afiv):
+    """More than 2^31 elements: columns at both ends against the formula (a column's result depends on it alone)."""
+    m, n = (1 << 22) + 5, 520
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(m, n, generator=g, device="cuda", dtype=torch.float16)
+    dy = torch.randn(m, n, generator=g, device="cuda", dtype=torch.float16)
+    keep = torch.rand(m, n, generator=g, device="cuda", dtype=torch.float16) >= 0.25
+    gamma, beta = 0.5 + torch.rand(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+    for eight in (False, True):
+        y, saved = afiv.batch_norm_act_forward(x, gamma, beta, act="silu", keep=keep, drop_p=0.25, checkpoint8=eight)
+        dx, dgamma, dbeta = afiv.batch_norm_act_backward(dy, gamma, beta, saved)
+        back = saved.eight.restore() if eight else None
+        for c in (slice(0, 3), slice(n - 3, n)):
+            part = types.SimpleNamespace(stats=saved.stats[:, c], eight=types.SimpleNamespace(restore=lambda: back[:, c]) if eight else None)
+            check_norm(x[:, c], gamma[c], beta[c], keep[:, c], 0.25, "silu", dy[:, c], y[:, c], part, dx[:, c], dgamma[c], dbeta[c])
+        del y, dx, saved, back
