@@ -1423,8 +1423,9 @@ int backward(const void *dy, const void *x, const int8_t *codes, const uint8_t *
     }
     int rc = ok();
     const bool only_db = !dw && db && !sums;                     // the input may be missing: no product with it
-    if (!rc && dx && M > 0 && only_db && !direct_dx) return db_alone<T>(&d, e, scratch, s);
-    if (!rc && dx && M > 0 && dw && !direct_dx && !direct_dw)
+    const bool joint = dx && M > 0 && one_launch(M, N, K);
+    if (!rc && joint && only_db && !direct_dx) return db_alone<T>(&d, e, scratch, s);
+    if (!rc && joint && dw && !direct_dx && !direct_dw)
         return codes ? products<T, ACROSS_EIGHT>(d, e, scratch, s) : products<T, ACROSS>(d, e, scratch, s);
     if (!rc && dx) {
         if (direct_dx) rc = direct<T, ALONG_DZ, ACROSS>(d, g, plain_source<T>(w, N, K, p.w, at, s), scratch, s);

@@ -36,6 +36,14 @@ Plan cut(int64_t tiles, int64_t L, int64_t step, int64_t few, int64_t want, int6
 // Tile kernel: 64 x 64 tiles; below 256 workgroups the sum is cut into runs of at least 256 steps.
 Plan plan_for(int64_t R, int64_t C, int64_t L) { return cut(tiles_of(R, C, 64), L, BK, 256, 512, 8); }
 
+// Both backward products in one launch: it has fewer than 2^32 work items, 256 a workgroup, and each product alone may
+// come near that.
+bool one_launch(int64_t M, int64_t N, int64_t K)
+{
+    const Plan dx = plan_for(M, K, N), dw = plan_for(N, K, M);
+    return dx.tiles * dx.splits + dw.tiles * dw.splits < 1 << 24;
+}
+
 // The direct kernel: 256 x 256 tiles where they fill the chip at least once and little of them lies outside the matrix
 // (131072 x 128 x 128, bf16: 26 us by 128 x 128 tiles, 46 by the large ones), else 128 x 128 (FP32: always).  Below 96
 // tiles the sum is cut, 16 bit for one workgroup a CU with four buffers, FP32 for two with two; above, the kernel that

@@ -255,8 +255,10 @@ int afiv_ensemble_stats_groups(const double *iv, const uint8_t *select, int64_t 
  * caller's device arrays, scratch too.  Outputs must not overlap inputs or each other, except where
  * said.  Arrays need no alignment beyond their elements'.  `dtype` is the element type of the arrays
  * written as [..] T; sums and what lies between input and output are FP32 or wider, except where said.
- * FP32 products are sums of BF16 products of each factor's three parts: a product is off by up to
- * 2^-21 of itself (2^-25 in the mean), and factors below 2^-110 keep fewer than 24 bits. */
+ * FP32 products (but for few rows or little work) are sums of BF16 products of each factor's three parts:
+ * a product is off by up to 2^-21 of itself (2^-25 in the mean), and factors below 2^-110 keep fewer
+ * than 24 bits.  A matrix spans fewer than 2^24 tiles of 64 x 64 elements (a launch's limit of work
+ * items), else AFIV_E_SHAPE. */
 enum { AFIV_F32 = 0, AFIV_BF16 = 1, AFIV_F16 = 2 };
 enum {
     AFIV_ACT_NONE = 0,

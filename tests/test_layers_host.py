@@ -143,3 +143,36 @@ def test_forward_mode_tangents_are_refused(afiv):
     for call in calls:
         with pytest.raises(NotImplementedError, match="tangent"):
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
+
+
+PLAN_PROGRAM = r"""
+#include "afiv_linear_plan.h"
+#include <cstdio>
+int main()
+{
+    long long m, n, k;
+    while (std::scanf("%lld %lld %lld", &m, &n, &k) == 3) {
+        const Plan dx = plan_for(m, k, n), dw = plan_for(n, k, m);
+        std::printf("%d %lld %lld\n", (int)one_launch(m, n, k), (long long)(dx.tiles * dx.splits), (long long)(dw.tiles * dw.splits));
+    }
+}
+"""
+
+
+def test_joint_launches_stay_within_a_launch(tmp_path):
+    """dx and dW share a launch only while their workgroups of 256 number fewer than 2^24; either alone does at any size that
+    the entry points accept."""
+    import os
+    import subprocess
+    root = os.path.join(os.path.dirname(__file__), "..")
+    (tmp_path / "plan.cpp").write_text(PLAN_PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-w", "-I", os.path.join(root, "include"), "-I",
+                    os.path.join(root, "arbitrage-free-iv-surfaces-using-vae_amd", "csrc"), "-o", str(tmp_path / "plan"), str(tmp_path / "plan.cpp")], check=True)
+    sizes = [(64, 128, 13), (131072, 64, 128), ((1 << 30) - 64, 1, 64), ((1 << 30) - 64, 64, 64), ((1 << 30) - 64 * 600, 1, 64), ((1 << 24) - 64, 1, 4096)]
+    out = subprocess.run([str(tmp_path / "plan")], input="\n".join("%d %d %d" % s for s in sizes), capture_output=True, text=True, check=True).stdout
+    joint = []
+    for (m, n, k), line in zip(sizes, out.splitlines()):
+        one, dx, dw = map(int, line.split())
+        assert dx < 1 << 24 and dw < 1 << 24 and bool(one) == (dx + dw < 1 << 24), (m, n, k)
+        joint.append(bool(one))
+    assert joint == [True, True, False, False, True, False]
