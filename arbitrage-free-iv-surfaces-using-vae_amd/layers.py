@@ -47,17 +47,18 @@ def _act(name: str) -> int:
         raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
 
 
-def _is_plain(t, what: str) -> None:
-    """A tensor without a forward-mode tangent: the kernels would drop it, which reads as a derivative of zero."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{what} must be a torch.Tensor")
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+def _refuse_tangent(t: torch.Tensor, what: str) -> None:
+    """Inside a forward-mode level: the kernels would drop a tangent, which reads as a derivative of zero."""
+    if forward_ad.unpack_dual(t).tangent is not None:
         raise NotImplementedError(f"{what} has a forward-mode tangent: the layer operators differentiate in reverse mode only")
 
 
 def _first(x, what: str) -> torch.Tensor:
     """The operand that sets the device and the element type."""
-    _is_plain(x, what)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what} must be a torch.Tensor")
+    if forward_ad._current_level >= 0:
+        _refuse_tangent(x, what)
     if not x.is_cuda:
         raise ValueError(f"{what} is on {x.device}: the layer kernels need a GPU (no CPU fallback)")
     if x.dtype not in DTYPES:
@@ -73,7 +74,10 @@ def _plain(t: torch.Tensor) -> torch.Tensor:
 
 def _like(t, x: torch.Tensor, shape, what: str, dtypes=None, output: bool = False) -> torch.Tensor:
     """Another operand: on x's device, of x's type (or one of ``dtypes``), of the given shape."""
-    _is_plain(t, what)
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a torch.Tensor")
+    if forward_ad._current_level >= 0:
+        _refuse_tangent(t, what)
     if t.get_device() != x.get_device():
         raise ValueError(f"{what} is on {t.device}, expected {x.device}")
     if (t.dtype != x.dtype) if dtypes is None else (t.dtype not in dtypes):
@@ -275,7 +279,7 @@ def _graph(*tensors) -> bool:
     if forward_ad._current_level >= 0:                   # inside Function.apply tangents can no longer be seen
         for t in tensors:
             if isinstance(t, torch.Tensor):
-                _is_plain(t, "an operand")
+                _refuse_tangent(t, "an operand")
     if torch.is_grad_enabled():
         for t in tensors:
             if isinstance(t, torch.Tensor) and t.requires_grad:
