@@ -304,7 +304,9 @@ struct Operand {
 
 // db without dW, where no pass over dz sums it: a workgroup sums 128 columns of dz over one run of rows and reads nothing
 // of the layer's input.  A lane holds what it would in the tile kernel (4 columns, every eighth quad of rows), and the runs
-// are that kernel's, so db has the same bits with and without dW.  block: runs by blocks of columns.
+// are that kernel's, so db has the same bits with and without dW.  block: runs by blocks of columns.  Loads bound it, one step
+// on its way behind the step before: 131072 x 64 in BF16 with gelu's derivative 36 us (0.9 TB/s; with the product that took
+// 68), 64 x 4096 6 us (41).
 template <class T>
 __device__ __forceinline__ void sum_dz(const LinArgs &a, int64_t block)
 {
@@ -815,8 +817,8 @@ __device__ __forceinline__ void arrive()
 }
 
 // 16-bit types.  WR x WC waves of 16 TR x 16 TC outputs.  The matrix units bound it: 16384 x 4096 x 8192 in BF16 with gelu
-// and residual takes 0.91 ms (1.21 PFLOP/s, 58 % of their cycles; the rest is the epilogue and the start of each tile),
-// dW of 16384 x 4096 x 4096 0.40 ms (1.37 PFLOP/s).  DEEP: four buffers instead of two, for a grid of at most one
+// and residual takes 0.92 ms (1.19 PFLOP/s, 57 % of their cycles; the rest is the epilogue and the start of each tile),
+// dW of 16384 x 4096 x 4096 0.38 ms (1.44 PFLOP/s).  DEEP: four buffers instead of two, for a grid of at most one
 // workgroup a CU, which has no other to hide its loads behind: 777 x 1003 x 2055 19.4 -> 17.0 us, of which the steps
 // take 0.21 us each, what the matrix units need and L2 gives; where two fit a CU two buffers are faster (26 and
 // 20 us for a product of 315 workgroups).
@@ -927,7 +929,7 @@ __device__ __forceinline__ bool infinities(const Source &s, int64_t R, int64_t r
 // row of 128 bytes, and each wave splits its fragments on the way to the matrix units: 44 vector instructions a fragment
 // beside the 12 matrix instructions it feeds, which the two units of a SIMD run side by side.  (Parts written to memory
 // as three planes first were 10 bytes an element of extra traffic and half again as many through L2: forward and backward
-// of 8192 x 1024 x 512 took 221 us, 195 now: forward 64, dx 56, dW 56.)  Instruction issue bounds it: a matrix
+// of 8192 x 1024 x 512 took 221 us, 191 now: forward 61 to 66 from card to card, dx 53 to 57, dW 53 to 56.)  Instruction issue bounds it: a matrix
 // instruction (16 cycles) and its 3.7 vector instructions (15) take 34 cycles of a SIMD with two waves, 50 of one with a
 // lone wave, however the two kinds are ordered.  `a` describes the operands as they came, sa and sb as they are read.
 template <Kind KA, Kind KB>
@@ -1037,7 +1039,7 @@ __global__ __launch_bounds__(256, 2) void direct32_kernel(LinArgs a, Source sa, 
 // An operand for the direct kernels, [rows, cols] -> [rows, ldp], zeros behind cols.  src: x itself, dy with z or its
 // derivative codes (dz = dy f'(z); with `partial`, also the partial column sums of dz in FP32), or an 8-bit checkpoint.
 // rows_per rows a workgroup of 64 lanes (8 columns each) by 4 rows.  out may be NULL (db alone).  HBM bounds it: dz of
-// 16384 x 4096 in BF16 from derivative codes 71 us (4.7 TB/s), an 8-bit x 42 us (4.8 TB/s).
+// 16384 x 4096 in BF16 from derivative codes 78 us (4.3 TB/s), an 8-bit x 42 us (4.8 TB/s).
 enum Made { COPY, DZ, EIGHT };
 struct PrepArgs {
     const void *src, *pre;

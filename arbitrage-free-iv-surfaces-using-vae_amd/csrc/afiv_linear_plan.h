@@ -56,8 +56,12 @@ Plan direct_plan(int64_t R, int64_t C, int64_t L, bool f32)
 }
 
 // What the direct kernel takes: at least a tile each way, rows within 2^31 bytes of a tile's corner, and enough work that
-// its few, large tiles fill the chip (measured with two buffers; 16 bit: 512^3 15 us by it, 17 by the tile kernel; 300^3 23
-// and 12; FP32: 512^3 24 and 16, 4096 x 256 x 256 25 and 29).
+// its few, large tiles fill the chip.  us in a captured graph, by it and by the tile kernel, forward / dx / dW:
+//   16 bit, whole rows   256^3  6.1 6.7 / 7.5 10 / 7.7 13       512^3  7.7 10.7 / 9.2 13.7 / 9.6 16.6     1024^3  17 17 / 17 31 / 17 43
+//   16 bit, ragged rows  300^3  11.6 10.4 / 14.5 14.4 / 15 21   777 x 333 x 500  13 10.5 / 15.9 17 / 19.5 26
+//   FP32                 512^3  20 14 / 21 17 / 20 22           768^3  25 20.5 / 25 23 / 24.5 27          1024^3  31 31 / 31 43 / 31 62
+// One threshold a type stands for all of these: 16 bit, between whole rows, which it does faster from 2^24 on, and ragged
+// ones, which a pass has to write out for it first; FP32, where dW gains (2^27) before dx and the forward product do (2^30).
 bool direct_takes(int64_t R, int64_t C, int64_t L, bool f32)
 {
     return R >= 128 && C >= 128 && L >= 128 && (double)R * (double)C * (double)L >= (f32 ? 1 << 28 : 1 << 27);

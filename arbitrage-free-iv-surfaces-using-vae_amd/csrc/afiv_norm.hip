@@ -11,8 +11,8 @@
 // statistics need every row before the first output), the backward pass reads x or its 8-bit
 // checkpoint, dy and keep twice.  Column sums go row chunk by row chunk: P chunks give P partial
 // sums, added in chunk order by a second kernel, so results do not depend on scheduling.
-// 131072 x 1024 in BF16 with dropout and an 8-bit checkpoint: statistics 67 us (4.0 TB/s), outputs 160 us (5.0 TB/s),
-// backward sums 164 us (3.3 TB/s), dx 182 us (4.5 TB/s); a copy reaches 4.95.  64 x 128: 7.1 and 6.3 us, one launch each.
+// 131072 x 1024 in BF16 with dropout and an 8-bit checkpoint: statistics 68 us (3.9 TB/s), outputs 164 us (4.9 TB/s),
+// backward sums 168 us (3.2 TB/s), dx 183 us (4.4 TB/s); a copy reaches 4.95.  64 x 128: 7.2 and 6.4 us, one launch each.
 //
 // Statistics are FP64 sums of d = x - x0 and d^2, x0 = the column's first element: var = E[d^2] - E[d]^2 then cancels
 // only as far as x0 lies from the mean (without the shift a column of mean 1e5 and variance 1 lost five
