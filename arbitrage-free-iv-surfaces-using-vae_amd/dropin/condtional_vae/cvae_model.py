@@ -103,9 +103,9 @@ class ConditionalVAE_SingleHeston(nn.Module):
                 raise RuntimeError(f"layer_kernels=True does not call {type(m).__name__}, whose hooks would not run: "
                                    "remove them or use layer_kernels=False")
 
-    def _linear(self, layer, h, act="none"):
+    def _linear(self, layer, h):
         self._without_hooks(layer)
-        return _afiv.linear_act(h, layer.weight, layer.bias, act=act, checkpoint8=self.checkpoint8)
+        return _afiv.linear_act(h, layer.weight, layer.bias, checkpoint8=self.checkpoint8)
 
     def _run_stack(self, stack, h):
         """``stack(h)`` on the layer operators.  A block is [Linear, BatchNorm1d, activation, Dropout]:
@@ -125,13 +125,14 @@ class ConditionalVAE_SingleHeston(nn.Module):
                 raise ValueError(f"layer_kernels=True has leaky_relu with slope 0.2 only, got {layers[i + 2].negative_slope}")
             drop = layers[i + 3] if i + 3 < len(layers) and isinstance(layers[i + 3], nn.Dropout) else None
             p = drop.p if drop is not None and drop.training else 0.0        # its own mode, not the normalisation's
-            if bn.training or bn.running_mean is None:
+            mean, var = bn.running_mean, bn.running_var
+            if bn.training or mean is None:
                 h = self._linear(lin, h)
                 keep = torch.rand(h.shape, device=h.device) >= p if 0.0 < p < 1.0 else None
-                mean = var = None
                 momentum = 0.0 if bn.momentum is None else bn.momentum
-                if bn.training and bn.track_running_stats and bn.running_mean is not None:
-                    mean, var = bn.running_mean, bn.running_var
+                if mean is None or not bn.track_running_stats:
+                    mean = var = None
+                else:
                     bn.num_batches_tracked.add_(1)
                     if bn.momentum is None:                              # a mean over all batches
                         momentum = 1.0 / float(bn.num_batches_tracked)
@@ -139,8 +140,8 @@ class ConditionalVAE_SingleHeston(nn.Module):
                                          drop_p=0.0 if keep is None else p, momentum=momentum, eps=bn.eps, checkpoint8=self.checkpoint8)
                 p = p if keep is None else 0.0
             else:
-                a = bn.weight * torch.rsqrt(bn.running_var + bn.eps)
-                h = _afiv.linear_act(h, lin.weight * a[:, None], (lin.bias - bn.running_mean) * a + bn.bias, act=name,
+                a = bn.weight * torch.rsqrt(var + bn.eps)
+                h = _afiv.linear_act(h, lin.weight * a[:, None], (lin.bias - mean) * a + bn.bias, act=name,
                                      checkpoint8=self.checkpoint8)
             if p:
                 h = F.dropout(h, p)
