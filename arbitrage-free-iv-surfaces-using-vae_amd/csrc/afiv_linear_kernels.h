@@ -13,7 +13,7 @@
 // x: neither exists in memory (but for large products, below).
 //
 // 16-bit types go to v_mfma_f32_16x16x32, and dz is rounded to T for it (db is summed before): held in two parts it would
-// double both products, 830 of 1430 us at 16384 x 4096 x 4096, and layers whose gradients are of type T round there anyway.  FP32 operands are cut into three BF16 parts of 8 bits,
+// double both products, 820 of 1460 us at 16384 x 4096 x 4096, and layers whose gradients are of type T round there anyway.  FP32 operands are cut into three BF16 parts of 8 bits,
 // a = a1 + a2 + a3 exactly (each the upper half of what is left), and the six products a1 b1, a1 b2, a2 b1,
 // a1 b3, a2 b2, a3 b1 are summed in FP32: what is dropped is at most 2^-21 of a product (a2 b3 and a3 b2, 2^-22 each) and
 // 2^-25 in the mean, half an FP32 rounding, and six BF16 products cost 6/16 of one FP32 matrix instruction's time.
